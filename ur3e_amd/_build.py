@@ -12,9 +12,11 @@ import time
 HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(HERE, "csrc", "ur3e_batch.hip")
 SRC_VN = os.path.join(HERE, "csrc", "ur3e_vecnorm.hip")
+SRC_PL = os.path.join(HERE, "csrc", "ur3e_policy.hip")  # the operators of ur3e_amd/rl/ops.py
 SRC_MJCF = os.path.join(HERE, "csrc", "ur3e_mjcf.cpp")  # host only: the MJCF / YAML entry points
 SRC_GATHER = os.path.join(HERE, "csrc", "ur3e_gather.cpp")  # host only: the RCCL gather entry point
-DEPS = [SRC, SRC_VN, SRC_MJCF, SRC_GATHER, os.path.join(HERE, "..", "include", "ur3e_vecnorm.h"), os.path.join(HERE, "csrc", "ur3e_engine.h"), os.path.join(HERE, "csrc", "ur3e_wave.h"), os.path.join(HERE, "csrc", "ur3e_wave_r.h"),
+DEPS = [SRC, SRC_VN, SRC_PL, SRC_MJCF, SRC_GATHER, os.path.join(HERE, "..", "include", "ur3e_vecnorm.h"),
+        os.path.join(HERE, "..", "include", "ur3e_policy.h"), os.path.join(HERE, "csrc", "ur3e_engine.h"), os.path.join(HERE, "csrc", "ur3e_wave.h"), os.path.join(HERE, "csrc", "ur3e_wave_r.h"),
         os.path.join(HERE, "csrc", "detmath.h"), os.path.join(HERE, "csrc", "gen_main_tree.h"),
         os.path.join(HERE, "csrc", "convex.h"), os.path.join(HERE, "csrc", "ur3e_cvx_wave.h"),
         os.path.join(HERE, "..", "include", "ur3e_model.h"), os.path.join(HERE, "..", "include", "ur3e_batch.h")]
@@ -28,6 +30,10 @@ FLAGS = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-ffp-contract=off", "-fP
          # Without it every step kernel is scratch-free at 207-212 VGPRs (ur3e_batch.hip kernels)
          "-mllvm", "-disable-machine-licm",
          "-Wno-unused-result"]
+# the policy operators are float kernels of their own: contraction to FMAs and loop-invariant motion as the
+# compiler chooses, but no packed float instructions (some of their forms have given wrong results on gfx950)
+FLAGS_PL = ["--offload-arch=gfx950", "-O3", "-std=c++17", "-fPIC", "-Xclang", "-target-feature", "-Xclang",
+            "-packed-fp32-ops", "-Wno-unused-result"]
 
 
 def gen_main_tree() -> str:
@@ -125,7 +131,7 @@ OBJ = os.path.join(HERE, "_lib", "obj")
 # compile writes a depfile (hipcc -MD) next to its object, so an object is stale when any file it actually
 # included is newer; before the first build (no depfile yet) every header of the tree counts.
 HEADERS = [d for d in DEPS if d.endswith(".h")] + [GEN_PY]
-SOURCES = [SRC, SRC_VN, SRC_MJCF, SRC_GATHER]
+SOURCES = [SRC, SRC_VN, SRC_PL, SRC_MJCF, SRC_GATHER]
 
 
 def _newer(out: str, deps) -> bool:
@@ -161,7 +167,8 @@ def _objects(defs, tag, force, verbose):
         objs.append(obj)
         deps = _depfile_deps(dep)
         if force or _newer(obj, [src] + (deps if deps is not None else HEADERS)):
-            cmd = ([HIPCC] + [f for f in FLAGS if f != "-shared"] + (defs if src == SRC else [])
+            flags = FLAGS_PL if src == SRC_PL else [f for f in FLAGS if f != "-shared"]
+            cmd = ([HIPCC] + flags + (defs if src == SRC else [])
                    + ["-MD", "-MF", dep, "-c", "-o", obj, src])
             if verbose:
                 print(" ".join(cmd))

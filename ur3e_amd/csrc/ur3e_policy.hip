@@ -1,0 +1,811 @@
+/* Operators of a policy with memory (include/ur3e_policy.h): attention with a decaying state and keyed
+ * dropout.
+ *
+ * Attention over a sequence (k_attn_walk).  One wave owns one (sequence, head, slab of value channels) and walks
+ * its tokens in chunks of 16 with the state S [dk][slab] in registers.  With chunk-local positions i, j and
+ * the state S that enters the chunk:
+ *     o_i  = scale gamma^(i+1) S^T q_i + sum_{j <= i} scale gamma^(i-j) (q_i . k_j) v_j
+ *     S'   = gamma^n S + sum_j gamma^(n-1-j) k_j v_j^T
+ * All four products are 16 x 16 matrix instructions, and the register layouts chain without a trip through LDS:
+ * the scores are formed transposed (P^T = K Q^T), which leaves them as the right operand of O^T = V^T P^T, and the
+ * accumulators of S are the left operand of S^T Q^T as they stand.  That leaves two forms of a token
+ * tile: "rows" (lane: one token, 4 x KT consecutive channels) and "columns" (lane: KT consecutive channels of four
+ * tokens), both read straight from memory in whole cache lines.  Products are permutation invariant in the
+ * contracted index, so channel d of a tile pair is KT * position + tile in either form.
+ *
+ * Gradients are the same walk with other operands.  G_t = scale q_t do_t^T + a_{t+1} G_{t+1} is the state
+ * of the reversed sequence, so
+ *     dq = walk(do, v, k) on S^T,  dk = reversed walk(v, do, q) on G^T,  dv = reversed walk(k, q, do) on G.
+ */
+#include <hip/hip_runtime.h>
+
+#include <stdint.h>
+
+#include "../../include/ur3e_batch.h"
+#include "../../include/ur3e_policy.h"
+
+int ur3e_internal_fail(int code, const char* msg);
+
+#define PL_CHK(x)                                                                       \
+  do {                                                                                  \
+    hipError_t _e = (x);                                                                \
+    if (_e != hipSuccess) return ur3e_internal_fail(UR3E_EHIP, hipGetErrorString(_e));  \
+  } while (0)
+
+typedef float f4 __attribute__((ext_vector_type(4)));
+
+struct Bf16 { unsigned short x; };
+typedef _Float16 F16;
+
+__device__ __forceinline__ float to_f(float x) { return x; }
+__device__ __forceinline__ float to_f(Bf16 x) { return __builtin_bit_cast(float, (unsigned)x.x << 16); }
+__device__ __forceinline__ float to_f(F16 x) { return (float)x; }
+/* round to nearest even, once, where a result leaves the kernel */
+template <class T> __device__ __forceinline__ T from_f(float x);
+template <> __device__ __forceinline__ float from_f<float>(float x) { return x; }
+template <> __device__ __forceinline__ F16 from_f<F16>(float x) { return (F16)x; }
+template <> __device__ __forceinline__ Bf16 from_f<Bf16>(float x) {
+  return __builtin_bit_cast(Bf16, (__bf16)x);
+}
+
+/* N consecutive elements; VEC: aligned to min(16, N * sizeof(T)) bytes */
+template <class T, int N, bool VEC> __device__ __forceinline__ void ld_n(const T* p, float* x) {
+  if constexpr (VEC) {
+    constexpr int B = N * (int)sizeof(T) < 16 ? N * (int)sizeof(T) : 16;
+    constexpr int E = B / (int)sizeof(T);
+    struct alignas(B) Pack { T e[E]; };
+#pragma unroll
+    for (int c = 0; c < N / E; c++) {
+      const Pack v = reinterpret_cast<const Pack*>(p)[c];
+#pragma unroll
+      for (int i = 0; i < E; i++) x[c * E + i] = to_f(v.e[i]);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) x[i] = to_f(p[i]);
+  }
+}
+template <class T, int N, bool VEC> __device__ __forceinline__ void st_n(T* p, const float* x) {
+  if constexpr (VEC) {
+    constexpr int B = N * (int)sizeof(T) < 16 ? N * (int)sizeof(T) : 16;
+    constexpr int E = B / (int)sizeof(T);
+    struct alignas(B) Pack { T e[E]; };
+#pragma unroll
+    for (int c = 0; c < N / E; c++) {
+      Pack v;
+#pragma unroll
+      for (int i = 0; i < E; i++) v.e[i] = from_f<T>(x[c * E + i]);
+      reinterpret_cast<Pack*>(p)[c] = v;
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) p[i] = from_f<T>(x[i]);
+  }
+}
+
+/* One walk: which tensors play q, k and v, and which way time runs.  `kdim` channels are contracted in the
+   scores (and are the state's rows), `vdim` are read out. */
+struct Tok {
+  const void* p;
+  long long sb, st, sh;
+  int hdiv; /* head = query head / hdiv */
+};
+struct Walk {
+  Tok q, k, v, o;
+  void* out;
+  long long srow, scol;   /* strides of a [dk][dv] state as this walk's [kdim][vdim] */
+  const float* s_in;      /* [b][h][dk * dv] or null */
+  float* s_out;           /* or null */
+  float* ws;              /* [b][h][split][kdim * vdim]: split s holds the state that enters it (nsplit > 1) */
+  int reversed;
+  int out_f32;            /* out is float whatever the token type (gradients that are summed over heads) */
+  float in_scale, p_scale, w_scale; /* on the read-out of the entering state, on the scores, on k in the state */
+};
+struct WalkArgs {
+  Walk w[3];
+  int nw; /* walks of this launch, all of the same tile shape */
+  int b, t, h, kdim, vdim, slabs, nsplit, split_len;
+  const float* log_decay;
+  const unsigned char* starts;
+  long long starts_sb, starts_st;
+  const int* lengths;
+};
+
+/* gamma^n with gamma^0 = 1 whatever gamma (log_decay = -inf is a head without memory) */
+__device__ __forceinline__ float pw(float l, int n) { return n == 0 ? 1.0f : expf((float)n * l); }
+
+__device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
+
+/* KT, VT: tiles of 16 key channels and of 16 value channels per wave.  STATE: only the state at the end of
+   each split (from zero), for sequences that several waves share. */
+template <class T, int KT, int VT, bool VEC, bool STATE>
+__global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
+  const int lane = threadIdx.x & 63, idx = lane & 15, g = lane >> 4;
+  /* the wave's task in scalar registers, and with it every address base and loop bound */
+  const unsigned task = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const int nsp = STATE ? a.nsplit - 1 : a.nsplit;
+  unsigned r = task;
+  const int slab = (int)(r % a.slabs); r /= a.slabs;
+  const int wi = (int)(r % a.nw); r /= a.nw;
+  const int split = (int)(r % nsp); r /= nsp;
+  const int h = (int)(r % a.h); r /= a.h;
+  if (r >= (unsigned)a.b) return;
+  const int b = (int)r;
+  const Walk& w = a.w[wi];
+  const int v0 = slab * 16 * VT;
+  const float l = a.log_decay[h];
+  int len = a.t;
+  if (a.lengths) {
+    len = a.lengths[b];
+    len = len < 0 ? 0 : len > a.t ? a.t : len;
+  }
+  int lo = split * a.split_len, hi = lo + a.split_len < a.t ? lo + a.split_len : a.t;
+  const T* q = (const T*)w.q.p + b * w.q.sb + (h / w.q.hdiv) * w.q.sh;
+  const T* k = (const T*)w.k.p + b * w.k.sb + (h / w.k.hdiv) * w.k.sh;
+  const T* v = (const T*)w.v.p + b * w.v.sb + (h / w.v.hdiv) * w.v.sh + v0;
+  const unsigned char* starts = a.starts ? a.starts + b * a.starts_sb : nullptr;
+  T* out = (T*)w.out + b * w.o.sb + (h / w.o.hdiv) * w.o.sh + v0;
+  float* outf = (float*)w.out + b * w.o.sb + (h / w.o.hdiv) * w.o.sh + v0;
+  const int vleft = a.vdim - v0; /* channels of this slab and behind it */
+
+  /* padding: zeros */
+  if (!STATE) {
+    for (int t = (len > lo ? len : lo) + g; t < hi; t += 4)
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++) {
+        const int d = VT * idx + nt;
+        if (d < vleft) {
+          if (w.out_f32) outf[(long long)t * w.o.st + d] = 0.0f;
+          else out[(long long)t * w.o.st + d] = from_f<T>(0.0f);
+        }
+      }
+  }
+  hi = hi < len ? hi : len;
+
+  const int srow = (int)w.srow, scol = (int)w.scol;
+  const long long bh = (long long)b * a.h + h;
+  const long long elems = (long long)a.kdim * a.vdim;
+  f4 S[KT][VT];
+#pragma unroll
+  for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+    for (int nt = 0; nt < VT; nt++) S[mt][nt] = f4{0, 0, 0, 0};
+  const float* s_in = STATE ? nullptr : a.nsplit > 1 ? w.ws + (bh * a.nsplit + split) * elems
+                                                     : w.s_in ? w.s_in + bh * elems : nullptr;
+  if (s_in) {
+#pragma unroll
+    for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int dk = KT * (4 * g + e) + mt, dv = VT * idx + nt;
+          if (dk < a.kdim && dv < vleft) S[mt][nt][e] = s_in[dk * srow + (v0 + dv) * scol];
+        }
+  }
+
+  const int e0 = w.reversed ? 0 : 1; /* the entering state has decayed by one step at position 0, or by none yet */
+  float dm[4], wk16[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) {
+    const int j = 4 * g + e;
+    dm[e] = idx >= j ? w.p_scale * pw(l, idx - j) : 0.0f;
+    wk16[e] = w.w_scale * pw(l, 15 - j + (1 - e0));
+  }
+  const float fi = w.in_scale * pw(l, idx + e0), g16 = pw(l, 16);
+
+  int single = 0; /* tokens left to take one by one */
+  for (int p = lo; p < hi;) {
+    int n = hi - p < 16 ? hi - p : 16;
+    if (single) n = 1;
+    /* token of position x */
+    const long long t0 = w.reversed ? len - 1 - p : p;
+    const int step = w.reversed ? -1 : 1;
+    float kr[KT][4], kt[KT][4], qr[KT][4], vt[VT][4];
+    const bool row_ok = idx < n;
+    const long long trow = t0 + step * (row_ok ? idx : 0);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int d = KT * (4 * g + e);
+      float xk[KT], xq[KT];
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++) xk[mt] = xq[mt] = 0.0f;
+      if (!STATE) {
+        if constexpr (VEC) {
+          if (row_ok && d < a.kdim) {
+            ld_n<T, KT, true>(k + trow * w.k.st + d, xk);
+            ld_n<T, KT, true>(q + trow * w.q.st + d, xq);
+          }
+        } else {
+#pragma unroll
+          for (int mt = 0; mt < KT; mt++)
+            if (row_ok && d + mt < a.kdim) {
+              xk[mt] = to_f(k[trow * w.k.st + d + mt]);
+              xq[mt] = to_f(q[trow * w.q.st + d + mt]);
+            }
+        }
+      }
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++) { kr[mt][e] = xk[mt]; qr[mt][e] = xq[mt]; }
+    }
+    float bad = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int j = 4 * g + e;
+      const long long tc = t0 + step * (j < n ? j : 0);
+      float xk[KT], xv[VT];
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++) xk[mt] = 0.0f;
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++) xv[nt] = 0.0f;
+      if constexpr (VEC) {
+        if (j < n && KT * idx < a.kdim) ld_n<T, KT, true>(k + tc * w.k.st + KT * idx, xk);
+        if (j < n && VT * idx < vleft) ld_n<T, VT, true>(v + tc * w.v.st + VT * idx, xv);
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < KT; mt++)
+          if (j < n && KT * idx + mt < a.kdim) xk[mt] = to_f(k[tc * w.k.st + KT * idx + mt]);
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++)
+          if (j < n && VT * idx + nt < vleft) xv[nt] = to_f(v[tc * w.v.st + VT * idx + nt]);
+      }
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++) kt[mt][e] = xk[mt];
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++) { vt[nt][e] = xv[nt]; bad = fmaf(xv[nt], 0.0f, bad); }
+    }
+    /* a value that is not finite must not meet the zeros of the mask (0 * inf): its chunk is taken token by
+       token, where every product belongs to the token */
+    if (n > 1 && __any(bad != 0.0f)) { single = n; continue; }
+
+    /* bit i: an episode starts between positions i - 1 and i */
+    unsigned brk = 0;
+    if (starts) {
+      const int x = p + idx;
+      const long long ts = w.reversed ? len - x : x;
+      const bool f = row_ok && x < hi && !(w.reversed && x == 0) && starts[ts * a.starts_st];
+      brk = (unsigned)(__ballot(f) & 0xffffu);
+    }
+
+    if (!STATE) {
+      f4 pt = {0, 0, 0, 0};
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) pt = mfma4(kr[mt][e], qr[mt][e], pt);
+      const unsigned upto = (2u << idx) - 1u; /* breaks at or in front of this lane's position */
+      float ps[4];
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int j = 4 * g + e;
+        const bool ok = idx >= j && (brk & upto & ~((2u << j) - 1u)) == 0;
+        ps[e] = ok ? pt[e] * dm[e] : 0.0f;
+      }
+      const bool from_state = (brk & upto) == 0;
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++) {
+        f4 o = {0, 0, 0, 0};
+#pragma unroll
+        for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) o = mfma4(S[mt][nt][e], qr[mt][e], o);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e] = from_state ? o[e] * fi : 0.0f;
+#pragma unroll
+        for (int e = 0; e < 4; e++) o = mfma4(vt[nt][e], ps[e], o);
+/* o[e]: channel VT * (4 g + e) + nt of token idx */
+        if (row_ok) {
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const int d = VT * (4 * g + e) + nt;
+            if (d < vleft) {
+              if (w.out_f32) outf[trow * w.o.st + d] = o[e];
+              else out[trow * w.o.st + d] = from_f<T>(o[e]);
+            }
+          }
+        }
+      }
+    }
+
+    const float gn = n == 16 ? g16 : pw(l, n);
+    const bool keep = brk == 0;
+#pragma unroll
+    for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) S[mt][nt][e] = keep ? S[mt][nt][e] * gn : 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int j = 4 * g + e;
+      const float wk = n == 16 ? wk16[e] : w.w_scale * pw(l, j < n ? n - 1 - j + (1 - e0) : 0);
+      const bool ok = j < n && (brk >> (j + 1)) == 0;
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++) kt[mt][e] = ok ? kt[mt][e] * wk : 0.0f;
+    }
+#pragma unroll
+    for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) S[mt][nt] = mfma4(kt[mt][e], vt[nt][e], S[mt][nt]);
+    p += n;
+    if (single) single--;
+  }
+
+  float* s_out = nullptr;
+  if (STATE) s_out = w.ws + (bh * a.nsplit + split + 1) * elems;
+  else if (split == a.nsplit - 1 && w.s_out) s_out = w.s_out + bh * elems;
+  if (s_out) {
+    /* the state in front of a start that the first token carries gets no gradient */
+    const bool cut = !STATE && w.reversed && starts && len > 0 && starts[0];
+#pragma unroll
+    for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int dk = KT * (4 * g + e) + mt, dv = VT * idx + nt;
+          if (dk < a.kdim && dv < vleft) s_out[dk * srow + (v0 + dv) * scol] = cut ? 0.0f : S[mt][nt][e];
+        }
+  }
+}
+
+/* States that enter each split: ws[s] holds split s - 1's own sum (k_attn_walk, STATE) and becomes
+   X_s = gamma^(tokens of split s - 1) X_{s-1} + ws[s], X_0 = s_in; the decay is 0 across an episode start. */
+__global__ __launch_bounds__(256) void k_attn_join(WalkArgs a) {
+  const Walk& w = a.w[blockIdx.z];
+  const long long bh = blockIdx.y;
+  const int b = (int)(bh / a.h), h = (int)(bh % a.h);
+  const long long elems = (long long)a.kdim * a.vdim;
+  const float l = a.log_decay[h];
+  int len = a.t;
+  if (a.lengths) {
+    len = a.lengths[b];
+    len = len < 0 ? 0 : len > a.t ? a.t : len;
+  }
+  const int e = blockIdx.x * 256 + threadIdx.x;
+  float* ws = w.ws + bh * a.nsplit * elems;
+  float x = 0.0f;
+  if (e < elems && w.s_in) x = w.s_in[bh * elems + e];
+  for (int s = 0;; s++) {
+    if (e < elems) ws[s * elems + e] = x;
+    if (s == a.nsplit - 1) break;
+    int lo = s * a.split_len, hi = lo + a.split_len;
+    hi = hi < len ? hi : len;
+    lo = lo < hi ? lo : hi;
+    bool brk = false;
+    if (a.starts) {
+      const unsigned char* st = a.starts + b * a.starts_sb;
+      for (int p = lo + (int)threadIdx.x; p < hi; p += 256)
+        if (!(w.reversed && p == 0)) brk |= st[(w.reversed ? len - p : p) * a.starts_st] != 0;
+      brk = __syncthreads_or(brk);
+    }
+    if (e < elems) x = (brk ? 0.0f : x * pw(l, hi - lo)) + ws[(s + 1) * elems + e];
+  }
+}
+
+/* sums of the per-query-head gradients over the heads that share a key / value head */
+template <class T>
+__global__ __launch_bounds__(256) void k_attn_group_sum(const float* __restrict__ src, T* __restrict__ dst, int b, int t,
+                                                        int h, int hk, int d, long long sb, long long st, long long sh) {
+  const long long n = (long long)b * t * hk * d;
+  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
+    const int c = (int)(i % d);
+    long long r = i / d;
+    const int kh = (int)(r % hk); r /= hk;
+    const int tt = (int)(r % t);
+    const int bb = (int)(r / t);
+    const int grp = h / hk;
+    const float* s = src + (((long long)bb * t + tt) * h + kh * grp) * d + c;
+    float x = 0.0f;
+    for (int k = 0; k < grp; k++) x += s[(long long)k * d];
+    dst[bb * sb + tt * st + kh * sh + c] = from_f<T>(x);
+  }
+}
+
+/* ---- one token -----------------------------------------------------------------------------------
+   A wave owns one (sequence, head): lanes are CL groups of VW channels of v by 64 / CL rows of the state, rows
+   streamed once: S' = a S + k v^T stored, o += q S' kept per lane and summed over the row groups at the end. */
+struct StepArgs {
+  Tok q, k, v, o;
+  int b, h, kdim, vdim;
+  float scale;
+  const float* log_decay;
+  const unsigned char* starts;
+  long long starts_sb;
+  const float* s_in;
+  float* s_out;
+};
+template <class T, int VW> __global__ __launch_bounds__(256) void k_attn_step(StepArgs a, int cl_log) {
+  const int lane = threadIdx.x & 63;
+  const long long bh = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
+  if (bh >= (long long)a.b * a.h) return;
+  const int b = (int)(bh / a.h), h = (int)(bh % a.h);
+  const int CL = 1 << cl_log, RG = 64 >> cl_log;
+  const int c = lane & (CL - 1), r0 = lane >> cl_log;
+  const bool cut = a.starts && a.starts[b * a.starts_sb];
+  const float decay = cut ? 0.0f : expf(a.log_decay[h]);
+  const T* q = (const T*)a.q.p + b * a.q.sb + h / a.q.hdiv * a.q.sh;
+  const T* k = (const T*)a.k.p + b * a.k.sb + h / a.k.hdiv * a.k.sh;
+  const T* v = (const T*)a.v.p + b * a.v.sb + h / a.v.hdiv * a.v.sh;
+  T* o = (T*)a.o.p + b * a.o.sb + h / a.o.hdiv * a.o.sh;
+  const long long base = bh * a.kdim * a.vdim;
+  struct alignas(4 * VW) Pack { float e[VW]; };
+  for (int c0 = 0; c0 < a.vdim; c0 += CL * VW) {
+    const int d = c0 + c * VW;
+    const bool ok = d < a.vdim; /* VW divides vdim */
+    float vv[VW], acc[VW];
+#pragma unroll
+    for (int i = 0; i < VW; i++) { vv[i] = ok ? to_f(v[d + i]) : 0.0f; acc[i] = 0.0f; }
+#pragma unroll 4
+    for (int rr = 0; rr < a.kdim; rr += RG) {
+      const int row = rr + r0;
+      if (ok && row < a.kdim) {
+        const long long at = base + (long long)row * a.vdim + d;
+        const float kk = to_f(k[row]), qq = to_f(q[row]);
+        Pack s;
+        if (cut) {
+#pragma unroll
+          for (int i = 0; i < VW; i++) s.e[i] = 0.0f;
+        } else {
+          s = *reinterpret_cast<const Pack*>(a.s_in + at);
+        }
+#pragma unroll
+        for (int i = 0; i < VW; i++) {
+          s.e[i] = fmaf(kk, vv[i], cut ? 0.0f : decay * s.e[i]);
+          acc[i] = fmaf(qq, s.e[i], acc[i]);
+        }
+        if (a.s_out) *reinterpret_cast<Pack*>(a.s_out + at) = s;
+      }
+    }
+#pragma unroll
+    for (int i = 0; i < VW; i++) {
+      for (int m = CL; m < 64; m <<= 1) acc[i] += __shfl_xor(acc[i], m);
+      if (ok && r0 == 0) o[d + i] = from_f<T>(acc[i] * a.scale);
+    }
+  }
+}
+
+/* ---- keyed dropout ------------------------------------------------------------------------------- */
+
+/* Philox4x32-10 (Salmon et al., 2011), as the env's reset noise uses it */
+__device__ __forceinline__ void philox(unsigned c0, unsigned c1, unsigned c2, unsigned c3, unsigned k0, unsigned k1,
+                                       unsigned out[4]) {
+#pragma unroll
+  for (int r = 0; r < 10; r++) {
+    const unsigned long long p0 = (unsigned long long)0xD2511F53u * c0, p1 = (unsigned long long)0xCD9E8D57u * c2;
+    const unsigned n0 = (unsigned)(p1 >> 32) ^ c1 ^ k0, n2 = (unsigned)(p0 >> 32) ^ c3 ^ k1;
+    c1 = (unsigned)p1;
+    c3 = (unsigned)p0;
+    c0 = n0;
+    c2 = n2;
+    k0 += 0x9E3779B9u;
+    k1 += 0xBB67AE85u;
+  }
+  out[0] = c0; out[1] = c1; out[2] = c2; out[3] = c3;
+}
+
+/* a thread takes the 8 columns of one Philox call */
+template <class T, bool VEC>
+__global__ __launch_bounds__(256) void k_keyed_dropout(long long rows, int cols, const T* x, long long xs, const T* res,
+                                                       long long rs, T* y, long long ys, const long long* ids,
+                                                       unsigned long long seed, unsigned sub, unsigned count, float up) {
+  const unsigned blocks = (unsigned)(cols + 7) / 8;
+  const long long n = rows * blocks;
+  const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+  if (i >= n) return;
+  const long long row = i / blocks;
+  const unsigned j = (unsigned)(i % blocks);
+  const unsigned long long id = ids ? (unsigned long long)ids[row] : (unsigned long long)row;
+  const int c0 = 8 * (int)j;
+  float xv[8], rv[8];
+  const int m = cols - c0 < 8 ? cols - c0 : 8;
+  if constexpr (VEC) {
+    ld_n<T, 8, true>(x + row * xs + c0, xv);
+    if (res) ld_n<T, 8, true>(res + row * rs + c0, rv);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++) {
+      xv[e] = e < m ? to_f(x[row * xs + c0 + e]) : 0.0f;
+      rv[e] = res && e < m ? to_f(res[row * rs + c0 + e]) : 0.0f;
+    }
+  }
+  unsigned u[4];
+  philox(j, (unsigned)id, (unsigned)(id >> 32), sub, (unsigned)seed, (unsigned)(seed >> 32), u);
+#pragma unroll
+  for (int e = 0; e < 8; e++) {
+    const unsigned d = e & 1 ? u[e >> 1] >> 16 : u[e >> 1] & 0xffffu;
+    float z = d < count ? xv[e] * up : 0.0f; /* a dropped element is 0 whatever it held */
+    if (res) z += rv[e];
+    xv[e] = z;
+  }
+  if constexpr (VEC) {
+    st_n<T, 8, true>(y + row * ys + c0, xv);
+  } else {
+#pragma unroll
+    for (int e = 0; e < 8; e++)
+      if (e < m) y[row * ys + c0 + e] = from_f<T>(xv[e]);
+  }
+}
+
+/* ---- host ------------------------------------------------------------------------------------- */
+
+static int bad_arg(const char* msg) { return ur3e_internal_fail(UR3E_EINVAL, msg); }
+
+static int elem_size(int dtype) { return dtype == UR3E_F32 ? 4 : 2; }
+
+static int attn_check(const ur3e_attn_t* a) {
+  if (!a) return bad_arg("attention: null argument");
+  if (a->dtype < UR3E_F32 || a->dtype > UR3E_F16) return bad_arg("attention: dtype must be 0 (float), 1 (bfloat16) or 2 (half)");
+  if (a->b < 0 || a->t < 0 || a->heads < 1 || a->kv_heads < 1) return bad_arg("attention: need b >= 0, t >= 0, heads >= 1, kv_heads >= 1");
+  if (a->heads % a->kv_heads) return bad_arg("attention: kv_heads must divide heads");
+  if (a->dk < 1 || a->dk > UR3E_ATTN_MAX_DIM || a->dv < 1 || a->dv > UR3E_ATTN_MAX_DIM)
+    return bad_arg("attention: dk and dv must be in [1, 128]");
+  if ((long long)a->b * a->heads > 4194303) return bad_arg("attention: b * heads must be below 2^22");
+  if (a->b == 0) return UR3E_OK;
+  if (!a->log_decay) return bad_arg("attention: null log_decay");
+  if (a->t > 0 && (!a->q.p || !a->k.p || !a->v.p)) return bad_arg("attention: null q, k or v");
+  return UR3E_OK;
+}
+
+static int pow2_tiles(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : 8; }
+
+struct Plan {
+  int kt, vt, slabs, nsplit, split_len;
+};
+
+/* Tiles: the state of a wave is kdim x 16 vt floats, at most 64 registers a lane, so vt is at most 2 at 128 key
+   channels.  Splits: ~2 waves a SIMD (2,048) fill the card. */
+static Plan plan_of(int b, int t, int h, int kdim, int vdim, int walks) {
+  Plan p;
+  p.kt = pow2_tiles(kdim);
+  p.vt = pow2_tiles(vdim);
+  const int most = p.kt == 8 ? 2 : 4;
+  if (p.vt > most) p.vt = most;
+  p.slabs = (vdim + 16 * p.vt - 1) / (16 * p.vt);
+  const long long waves = (long long)b * h * p.slabs * walks;
+  p.nsplit = 1;
+  p.split_len = t > 0 ? t : 1;
+  if (waves < 1024 && t >= 256) {
+    long long want = (2048 + waves - 1) / (waves > 0 ? waves : 1);
+    long long most_splits = t / 128;
+    if (want > most_splits) want = most_splits;
+    if (want > 1) {
+      p.split_len = (int)(((t + want - 1) / want + 15) / 16 * 16);
+      p.nsplit = (t + p.split_len - 1) / p.split_len;
+    }
+  }
+  return p;
+}
+
+static size_t walk_bytes(const Plan& p, long long b, int h, int kdim, int vdim) {
+  return p.nsplit > 1 ? (size_t)b * h * p.nsplit * kdim * vdim * sizeof(float) : 0;
+}
+
+static bool aligned(const Tok& t, int e, int kt, int d) {
+  const int by = kt * e < 16 ? kt * e : 16;
+  return d % kt == 0 && (uintptr_t)t.p % by == 0 && t.sb * e % by == 0 && t.st * e % by == 0 && t.sh * e % by == 0;
+}
+
+template <class T, int KT, int VT, bool VEC> static int walk_launch(const WalkArgs& a, hipStream_t s) {
+  const long long streams = (long long)a.b * a.h * a.nw * a.slabs;
+  if (a.nsplit > 1) {
+    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, true>), dim3((unsigned)((streams * (a.nsplit - 1) + 3) / 4)), dim3(256), 0, s, a);
+    PL_CHK(hipGetLastError());
+    hipLaunchKernelGGL(k_attn_join, dim3((a.kdim * a.vdim + 255) / 256, (unsigned)(a.b * a.h), (unsigned)a.nw), dim3(256), 0, s, a);
+    PL_CHK(hipGetLastError());
+  }
+  hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false>), dim3((unsigned)((streams * a.nsplit + 3) / 4)), dim3(256), 0, s, a);
+  PL_CHK(hipGetLastError());
+  return UR3E_OK;
+}
+template <class T, int KT, int VT> static int walk_vec(const WalkArgs& a, hipStream_t s) {
+  bool vec = true;
+  for (int i = 0; i < a.nw; i++)
+    vec = vec && aligned(a.w[i].q, sizeof(T), KT, a.kdim) && aligned(a.w[i].k, sizeof(T), KT, a.kdim) &&
+          aligned(a.w[i].v, sizeof(T), VT, a.vdim);
+  return vec ? walk_launch<T, KT, VT, true>(a, s) : walk_launch<T, KT, VT, false>(a, s);
+}
+template <class T, int KT> static int walk_vt(const WalkArgs& a, int vt, hipStream_t s) {
+  if (vt == 1) return walk_vec<T, KT, 1>(a, s);
+  if (vt == 2) return walk_vec<T, KT, 2>(a, s);
+  if constexpr (KT < 8) return walk_vec<T, KT, 4>(a, s);
+  return ur3e_internal_fail(UR3E_EINVAL, "attention: no such tile");
+}
+template <class T> static int walk_kt(const WalkArgs& a, const Plan& p, hipStream_t s) {
+  switch (p.kt) {
+    case 1: return walk_vt<T, 1>(a, p.vt, s);
+    case 2: return walk_vt<T, 2>(a, p.vt, s);
+    case 4: return walk_vt<T, 4>(a, p.vt, s);
+    default: return walk_vt<T, 8>(a, p.vt, s);
+  }
+}
+static int walk_run(int dtype, const WalkArgs& a, const Plan& p, hipStream_t s) {
+  if (dtype == UR3E_F32) return walk_kt<float>(a, p, s);
+  if (dtype == UR3E_BF16) return walk_kt<Bf16>(a, p, s);
+  return walk_kt<F16>(a, p, s);
+}
+
+static Tok tok_of(const ur3e_tokens_t& x, int hdiv) { return Tok{x.p, x.sb, x.st, x.sh, hdiv}; }
+
+static WalkArgs args_of(const ur3e_attn_t* a, int kdim, int vdim, const Plan& p) {
+  WalkArgs w = {};
+  w.b = a->b; w.t = a->t; w.h = a->heads; w.kdim = kdim; w.vdim = vdim;
+  w.slabs = p.slabs; w.nsplit = p.nsplit; w.split_len = p.split_len;
+  w.log_decay = a->log_decay;
+  w.starts = a->starts; w.starts_sb = a->starts_sb; w.starts_st = a->starts_st;
+  w.lengths = a->lengths;
+  return w;
+}
+
+static size_t up16(size_t x) { return (x + 255) / 256 * 256; }
+
+static size_t attn_bytes(const ur3e_attn_t* a, int backward) {
+  if (!backward) return walk_bytes(plan_of(a->b, a->t, a->heads, a->dk, a->dv, 1), a->b, a->heads, a->dk, a->dv);
+  const int same = pow2_tiles(a->dk) == pow2_tiles(a->dv) && a->dk == a->dv;
+  const Plan p1 = plan_of(a->b, a->t, a->heads, a->dv, a->dk, same ? 3 : 2), p2 = same ? p1 : plan_of(a->b, a->t, a->heads, a->dk, a->dv, 1);
+  size_t n = 2 * up16(walk_bytes(p1, a->b, a->heads, a->dv, a->dk)) + up16(walk_bytes(p2, a->b, a->heads, a->dk, a->dv));
+  if (a->heads != a->kv_heads) n += up16((size_t)a->b * a->t * a->heads * a->dk * 4) + up16((size_t)a->b * a->t * a->heads * a->dv * 4);
+  return n;
+}
+
+extern "C" int ur3e_attn_workspace(const ur3e_attn_t* a, int backward, size_t* bytes) {
+  const int rc = attn_check(a);
+  if (rc) return rc;
+  if (!bytes) return bad_arg("attention: null bytes");
+  *bytes = attn_bytes(a, backward);
+  return UR3E_OK;
+}
+
+extern "C" int ur3e_attn_forward(const ur3e_attn_t* a, const ur3e_tokens_t* out, float* s_out, void* workspace,
+                                 size_t workspace_bytes, void* stream) {
+  int rc = attn_check(a);
+  if (rc) return rc;
+  if (a->b == 0) return UR3E_OK;
+  if (!out || (a->t > 0 && !out->p)) return bad_arg("attention: null out");
+  if (workspace_bytes < attn_bytes(a, 0) || (attn_bytes(a, 0) && !workspace)) return bad_arg("attention: workspace too small");
+  const Plan p = plan_of(a->b, a->t, a->heads, a->dk, a->dv, 1);
+  WalkArgs w = args_of(a, a->dk, a->dv, p);
+  const int grp = a->heads / a->kv_heads;
+  w.nw = 1;
+  Walk& f = w.w[0];
+  f.q = tok_of(a->q, 1); f.k = tok_of(a->k, grp); f.v = tok_of(a->v, grp); f.o = tok_of(*out, 1);
+  f.out = out->p;
+  f.srow = a->dv; f.scol = 1;
+  f.s_in = a->s0; f.s_out = s_out; f.ws = (float*)workspace;
+  f.in_scale = f.p_scale = a->scale; f.w_scale = 1.0f;
+  return walk_run(a->dtype, w, p, (hipStream_t)stream);
+}
+
+extern "C" int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dout, const float* ds_out,
+                                  const ur3e_tokens_t* dq, const ur3e_tokens_t* dk, const ur3e_tokens_t* dv, float* ds0,
+                                  void* workspace, size_t workspace_bytes, void* stream) {
+  int rc = attn_check(a);
+  if (rc) return rc;
+  if (a->b == 0) return UR3E_OK;
+  if (!dout || !dq || !dk || !dv) return bad_arg("attention: null gradient");
+  if (a->t > 0 && (!dout->p || !dq->p || !dk->p || !dv->p)) return bad_arg("attention: null gradient");
+  if (workspace_bytes < attn_bytes(a, 1) || (attn_bytes(a, 1) && !workspace)) return bad_arg("attention: workspace too small");
+  hipStream_t s = (hipStream_t)stream;
+  const int grp = a->heads / a->kv_heads;
+  const bool same = a->dk == a->dv;
+  const Plan p1 = plan_of(a->b, a->t, a->heads, a->dv, a->dk, same ? 3 : 2), p2 = same ? p1 : plan_of(a->b, a->t, a->heads, a->dk, a->dv, 1);
+  char* ws = (char*)workspace;
+  const size_t n1 = up16(walk_bytes(p1, a->b, a->heads, a->dv, a->dk)), n2 = up16(walk_bytes(p2, a->b, a->heads, a->dk, a->dv));
+  float *fk = nullptr, *fv = nullptr;
+  if (grp > 1) {
+    fk = (float*)(ws + 2 * n1 + n2);
+    fv = (float*)(ws + 2 * n1 + n2 + up16((size_t)a->b * a->t * a->heads * a->dk * 4));
+  }
+  const Tok tq = tok_of(a->q, 1), tk = tok_of(a->k, grp), tv = tok_of(a->v, grp), tdo = tok_of(*dout, 1);
+  auto wide = [&](int d) { return Tok{nullptr, (long long)a->t * a->heads * d, (long long)a->heads * d, d, 1}; };
+  Walk q = {}, k = {}, v = {};
+  /* dq = walk(do, v, k) on S^T */
+  q.q = tdo; q.k = tv; q.v = tk; q.o = tok_of(*dq, 1); q.out = dq->p;
+  q.srow = 1; q.scol = a->dv;
+  q.s_in = a->s0; q.ws = (float*)ws;
+  q.in_scale = q.p_scale = a->scale; q.w_scale = 1.0f;
+  /* dk = reversed walk(v, do, q) on G^T */
+  k.q = tv; k.k = tdo; k.v = tq; k.o = grp > 1 ? wide(a->dk) : tok_of(*dk, 1); k.out = grp > 1 ? (void*)fk : dk->p;
+  k.out_f32 = grp > 1;
+  k.srow = 1; k.scol = a->dv;
+  k.s_in = ds_out; k.ws = (float*)(ws + n1);
+  k.reversed = 1;
+  k.in_scale = 1.0f; k.p_scale = k.w_scale = a->scale;
+  /* dv = reversed walk(k, q, do) on G */
+  v.q = tk; v.k = tq; v.v = tdo; v.o = grp > 1 ? wide(a->dv) : tok_of(*dv, 1); v.out = grp > 1 ? (void*)fv : dv->p;
+  v.out_f32 = grp > 1;
+  v.srow = a->dv; v.scol = 1;
+  v.s_in = ds_out; v.s_out = ds0; v.ws = (float*)(ws + 2 * n1);
+  v.reversed = 1;
+  v.in_scale = 1.0f; v.p_scale = v.w_scale = a->scale;
+  WalkArgs w = args_of(a, a->dv, a->dk, p1);
+  w.w[0] = q; w.w[1] = k;
+  w.nw = 2;
+  if (same) { w.w[2] = v; w.nw = 3; }
+  rc = walk_run(a->dtype, w, p1, s);
+  if (rc) return rc;
+  if (!same) {
+    WalkArgs x = args_of(a, a->dk, a->dv, p2);
+    x.w[0] = v;
+    x.nw = 1;
+    rc = walk_run(a->dtype, x, p2, s);
+    if (rc) return rc;
+  }
+  if (grp > 1 && a->t > 0) {
+    const long long m = (long long)a->b * a->t * a->kv_heads;
+    auto sum = [&](const float* src, const ur3e_tokens_t& d, int c) {
+      const long long blocks = (m * c + 255) / 256;
+      const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
+      if (a->dtype == UR3E_F32) hipLaunchKernelGGL(k_attn_group_sum<float>, grid, dim3(256), 0, s, src, (float*)d.p, a->b, a->t, a->heads, a->kv_heads, c, d.sb, d.st, d.sh);
+      else if (a->dtype == UR3E_BF16) hipLaunchKernelGGL(k_attn_group_sum<Bf16>, grid, dim3(256), 0, s, src, (Bf16*)d.p, a->b, a->t, a->heads, a->kv_heads, c, d.sb, d.st, d.sh);
+      else hipLaunchKernelGGL(k_attn_group_sum<F16>, grid, dim3(256), 0, s, src, (F16*)d.p, a->b, a->t, a->heads, a->kv_heads, c, d.sb, d.st, d.sh);
+      return hipGetLastError();
+    };
+    PL_CHK(sum(fk, *dk, a->dk));
+    PL_CHK(sum(fv, *dv, a->dv));
+  }
+  return UR3E_OK;
+}
+
+extern "C" int ur3e_attn_step(const ur3e_attn_t* a, const ur3e_tokens_t* out, const float* state_in, float* state_out,
+                              void* stream) {
+  int rc = attn_check(a);
+  if (rc) return rc;
+  if (a->t != 1) return bad_arg("attention step: t must be 1");
+  if (a->lengths) return bad_arg("attention step: lengths must be null");
+  if (a->b == 0) return UR3E_OK;
+  if (!out || !out->p || !state_in) return bad_arg("attention step: null out or state");
+  StepArgs s = {};
+  const int grp = a->heads / a->kv_heads;
+  s.q = tok_of(a->q, 1); s.k = tok_of(a->k, grp); s.v = tok_of(a->v, grp); s.o = tok_of(*out, 1);
+  s.b = a->b; s.h = a->heads; s.kdim = a->dk; s.vdim = a->dv;
+  s.scale = a->scale; s.log_decay = a->log_decay;
+  s.starts = a->starts; s.starts_sb = a->starts_sb;
+  s.s_in = state_in; s.s_out = state_out;
+  const bool v4 = a->dv % 4 == 0 && (uintptr_t)state_in % 16 == 0 && (uintptr_t)state_out % 16 == 0;
+  const int groups = v4 ? a->dv / 4 : a->dv;
+  int cl = 0;
+  while ((1 << cl) < groups && cl < 6) cl++;
+  const dim3 grid((unsigned)(((long long)a->b * a->heads + 3) / 4));
+  hipStream_t st = (hipStream_t)stream;
+#define STEP(T)                                                                              \
+  if (v4) hipLaunchKernelGGL((k_attn_step<T, 4>), grid, dim3(256), 0, st, s, cl);            \
+  else hipLaunchKernelGGL((k_attn_step<T, 1>), grid, dim3(256), 0, st, s, cl);
+  if (a->dtype == UR3E_F32) { STEP(float) } else if (a->dtype == UR3E_BF16) { STEP(Bf16) } else { STEP(F16) }
+#undef STEP
+  PL_CHK(hipGetLastError());
+  return UR3E_OK;
+}
+
+template <class T>
+static int dropout_launch(long long rows, int cols, const void* x, long long xs, const void* res, long long rs, void* y,
+                          long long ys, const long long* ids, unsigned long long seed, unsigned sub, int count, hipStream_t s) {
+  const long long n = rows * ((cols + 7) / 8);
+  const float up = count ? 65536.0f / (float)count : 0.0f;
+  constexpr int E = 16 / (int)sizeof(T);
+  auto al = [](const void* p, long long st) { return (uintptr_t)p % 16 == 0 && st % E == 0; };
+  const bool vec = cols % 8 == 0 && al(x, xs) && al(y, ys) && (!res || al(res, rs));
+  const dim3 grid((unsigned)((n + 255) / 256));
+  if (vec) hipLaunchKernelGGL((k_keyed_dropout<T, true>), grid, dim3(256), 0, s, rows, cols, (const T*)x, xs, (const T*)res, rs, (T*)y, ys, ids, seed, sub, (unsigned)count, up);
+  else hipLaunchKernelGGL((k_keyed_dropout<T, false>), grid, dim3(256), 0, s, rows, cols, (const T*)x, xs, (const T*)res, rs, (T*)y, ys, ids, seed, sub, (unsigned)count, up);
+  PL_CHK(hipGetLastError());
+  return UR3E_OK;
+}
+
+extern "C" int ur3e_keyed_dropout(int dtype, long long rows, int cols, const void* x, long long x_stride,
+                                  const void* residual, long long residual_stride, void* y, long long y_stride,
+                                  const long long* row_ids, unsigned long long seed, unsigned int substream,
+                                  int keep_count, void* stream) {
+  if (dtype < UR3E_F32 || dtype > UR3E_F16) return bad_arg("dropout: dtype must be 0 (float), 1 (bfloat16) or 2 (half)");
+  if (rows < 0 || cols < 0) return bad_arg("dropout: need rows >= 0 and cols >= 0");
+  if (keep_count < 0 || keep_count > 65536) return bad_arg("dropout: keep_count must be in [0, 65536]");
+  if (rows == 0 || cols == 0) return UR3E_OK;
+  if (!x || !y) return bad_arg("dropout: null argument");
+  if (rows > 0xffffff00LL || rows * (((long long)cols + 7) / 8) > 0xffffff00LL) return bad_arg("dropout: too many elements for one call");
+  hipStream_t s = (hipStream_t)stream;
+  if (dtype == UR3E_F32) return dropout_launch<float>(rows, cols, x, x_stride, residual, residual_stride, y, y_stride, row_ids, seed, substream, keep_count, s);
+  if (dtype == UR3E_BF16) return dropout_launch<Bf16>(rows, cols, x, x_stride, residual, residual_stride, y, y_stride, row_ids, seed, substream, keep_count, s);
+  return dropout_launch<F16>(rows, cols, x, x_stride, residual, residual_stride, y, y_stride, row_ids, seed, substream, keep_count, s);
+}
