@@ -12,7 +12,7 @@
  *
  * Element types: 0 float, 1 bfloat16, 2 IEEE half, the same for every token tensor of a call.  States,
  * log_decay and all sums are float.  All pointers are device pointers on the current HIP device; strides
- * are in elements, the channels of a token are contiguous.  Work is enqueued on `stream`; nothing is kept
+ * are in elements, the channels of a token are contiguous, token strides are not negative.  Work is enqueued on `stream`; nothing is kept
  * between calls, and a call may be captured into a graph.  Results do not depend on timing (no atomics).
  *
  * Errors: UR3E_EINVAL / UR3E_EHIP (ur3e_batch.h) with ur3e_last_error(); nothing is launched on EINVAL.

@@ -33,6 +33,8 @@ int ur3e_internal_fail(int code, const char* msg);
   } while (0)
 
 typedef float f4 __attribute__((ext_vector_type(4)));
+typedef unsigned u2 __attribute__((ext_vector_type(2)));
+typedef unsigned u4 __attribute__((ext_vector_type(4)));
 
 struct Bf16 { unsigned short x; };
 typedef _Float16 F16;
@@ -91,20 +93,21 @@ struct Tok {
   int hdiv; /* head = query head / hdiv */
 };
 struct Walk {
-  Tok q, k, v, o;
-  void* out;
-  long long srow, scol;   /* strides of a [dk][dv] state as this walk's [kdim][vdim] */
-  const float* s_in;      /* [b][h][dk * dv] or null */
-  float* s_out;           /* or null */
-  float* ws;              /* [b][h][split][kdim * vdim]: split s holds the state that enters it (nsplit > 1) */
+  Tok q, k, v, o;           /* o.p is written */
+  const float* s_in;        /* [b][h][dk * dv] or null */
+  float* s_out;             /* or null */
+  float* ws;                /* [b][h][split][kdim * vdim]: split s holds the state that enters it (nsplit > 1) */
+  int state_t;              /* a [dk][dv] state is this walk's transposed: kdim = dv */
   int reversed;
-  int out_f32;            /* out is float whatever the token type (gradients that are summed over heads) */
+  int out_f32;              /* out is float whatever the token type (gradients that are summed over heads) */
   float in_scale, p_scale, w_scale; /* on the read-out of the entering state, on the scores, on k in the state */
 };
 struct WalkArgs {
   Walk w[3];
   int nw; /* walks of this launch, all of the same tile shape */
   int b, t, h, kdim, vdim, slabs, nsplit, split_len;
+  int chunk;     /* 16, or 1 where tokens lie too far apart for 30-bit offsets inside a chunk */
+  int state_vec; /* states may be moved KT or VT floats at a time */
   const float* log_decay;
   const unsigned char* starts;
   long long starts_sb, starts_st;
@@ -116,10 +119,87 @@ __device__ __forceinline__ float pw(float l, int n) { return n == 0 ? 1.0f : exp
 
 __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_amdgcn_mfma_f32_16x16x4f32(a, b, c, 0, 0, 0); }
 
+/* Every tile is read and written through buffer instructions, whose bounds check stands in for a branch: a lane
+   without an element carries an offset past the 2^30 bytes of the resource, reads 0 and writes nothing, so
+   the loads of a chunk issue back to back.  FAR_T (no such token) and FAR_D (no such channel) stay past the
+   limit when both are added. */
+#define FAR_T 0x80000000u
+#define FAR_D 0x40000000u
+typedef __amdgpu_buffer_rsrc_t Rsrc;
+__device__ __forceinline__ unsigned at(unsigned off, bool there, unsigned far) { return there ? off : far; }
+__device__ __forceinline__ Rsrc rsrc_of(const void* p) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)FAR_D, 0x00027000);
+}
+
+/* N consecutive elements as dwords; VEC: aligned to min(16, N * sizeof(T)) bytes and all there or none, else
+   one element to a dword, `left` of them there */
+template <class T, int N, bool VEC> struct Raw {
+  static constexpr int B = N * (int)sizeof(T);
+  static constexpr int D = VEC ? (B + 3) / 4 : N;
+  unsigned d[D];
+  __device__ __forceinline__ void load(Rsrc r, unsigned off, int left) {
+    if constexpr (VEC) {
+      if constexpr (B == 2) d[0] = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+      else if constexpr (B == 4) d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+      else if constexpr (B == 8) {
+        const u2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
+        d[0] = x.x; d[1] = x.y;
+      } else {
+#pragma unroll
+        for (int i = 0; i < B / 16; i++) {
+          const u4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * i, 0, 0);
+          d[4 * i] = x.x; d[4 * i + 1] = x.y; d[4 * i + 2] = x.z; d[4 * i + 3] = x.w;
+        }
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < N; i++) {
+        const unsigned o = at(off + i * (int)sizeof(T), i < left, FAR_T);
+        if constexpr (sizeof(T) == 2) d[i] = __builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0);
+        else d[i] = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+      }
+    }
+  }
+  __device__ __forceinline__ float get(int i) const {
+    if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, d[i]);
+    else {
+      const unsigned short h = VEC ? (unsigned short)(d[i / 2] >> (16 * (i & 1))) : (unsigned short)d[i];
+      return to_f(__builtin_bit_cast(T, h));
+    }
+  }
+};
+template <class T, int N, bool VEC> __device__ __forceinline__ void store_n(Rsrc r, unsigned off, int left, const float* x) {
+  if constexpr (VEC) {
+    constexpr int B = N * (int)sizeof(T);
+    unsigned d[(B + 3) / 4] = {};
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      if constexpr (sizeof(T) == 4) d[i] = __builtin_bit_cast(unsigned, x[i]);
+      else d[i / 2] |= (unsigned)__builtin_bit_cast(unsigned short, from_f<T>(x[i])) << (16 * (i & 1));
+    }
+    if constexpr (B == 2) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)d[0], r, off, 0, 0);
+    else if constexpr (B == 4) __builtin_amdgcn_raw_buffer_store_b32(d[0], r, off, 0, 0);
+    else if constexpr (B == 8) __builtin_amdgcn_raw_buffer_store_b64(u2{d[0], d[1]}, r, off, 0, 0);
+    else {
+#pragma unroll
+      for (int i = 0; i < B / 16; i++)
+        __builtin_amdgcn_raw_buffer_store_b128(u4{d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]}, r, off + 16 * i, 0, 0);
+    }
+  } else {
+#pragma unroll
+    for (int i = 0; i < N; i++) {
+      const unsigned o = at(off + i * (int)sizeof(T), i < left, FAR_T);
+      if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x[i]), r, o, 0, 0);
+      else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, from_f<T>(x[i])), r, o, 0, 0);
+    }
+  }
+}
+
 /* KT, VT: tiles of 16 key channels and of 16 value channels per wave.  STATE: only the state at the end of
    each split (from zero), for sequences that several waves share. */
 template <class T, int KT, int VT, bool VEC, bool STATE>
 __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
+  constexpr int ES = (int)sizeof(T);
   const int lane = threadIdx.x & 63, idx = lane & 15, g = lane >> 4;
   /* the wave's task in scalar registers, and with it every address base and loop bound */
   const unsigned task = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -131,223 +211,289 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   const int h = (int)(r % a.h); r /= a.h;
   if (r >= (unsigned)a.b) return;
   const int b = (int)r;
-  const Walk& w = a.w[wi];
-  const int v0 = slab * 16 * VT;
+  const Walk w = a.w[wi];
+  const int kdim = a.kdim, vdim = a.vdim, chunk = a.chunk, nsplit = a.nsplit;
+  const long long starts_st = a.starts_st;
+  const int v0 = slab * 16 * VT, vleft = vdim - v0; /* first channel of this slab, channels from there on */
   const float l = a.log_decay[h];
   int len = a.t;
   if (a.lengths) {
     len = a.lengths[b];
     len = len < 0 ? 0 : len > a.t ? a.t : len;
   }
-  int lo = split * a.split_len, hi = lo + a.split_len < a.t ? lo + a.split_len : a.t;
-  const T* q = (const T*)w.q.p + b * w.q.sb + (h / w.q.hdiv) * w.q.sh;
-  const T* k = (const T*)w.k.p + b * w.k.sb + (h / w.k.hdiv) * w.k.sh;
-  const T* v = (const T*)w.v.p + b * w.v.sb + (h / w.v.hdiv) * w.v.sh + v0;
+  const int lo = split * a.split_len, end = lo + a.split_len < a.t ? lo + a.split_len : a.t;
+  const int hi = end < len ? end : len;
+  const bool rev = w.reversed;
+  const char* q = (const char*)w.q.p + ES * (b * w.q.sb + (h / w.q.hdiv) * w.q.sh);
+  const char* k = (const char*)w.k.p + ES * (b * w.k.sb + (h / w.k.hdiv) * w.k.sh);
+  const char* v = (const char*)w.v.p + ES * (b * w.v.sb + (h / w.v.hdiv) * w.v.sh + v0);
+  const int os = w.out_f32 ? 4 : ES;
+  char* out = (char*)const_cast<void*>(w.o.p) + os * (b * w.o.sb + (h / w.o.hdiv) * w.o.sh + v0);
+  const long long qst = ES * w.q.st, kst = ES * w.k.st, vst = ES * w.v.st, ost = os * w.o.st;
   const unsigned char* starts = a.starts ? a.starts + b * a.starts_sb : nullptr;
-  T* out = (T*)w.out + b * w.o.sb + (h / w.o.hdiv) * w.o.sh + v0;
-  float* outf = (float*)w.out + b * w.o.sb + (h / w.o.hdiv) * w.o.sh + v0;
-  const int vleft = a.vdim - v0; /* channels of this slab and behind it */
 
-  /* padding: zeros */
-  if (!STATE) {
-    for (int t = (len > lo ? len : lo) + g; t < hi; t += 4)
+  /* byte offsets of a lane's channels: row form (group e of KT or VT channels at tile width x (4 g + e)) ... */
+  unsigned kd[4], od[4];
 #pragma unroll
-      for (int nt = 0; nt < VT; nt++) {
-        const int d = VT * idx + nt;
-        if (d < vleft) {
-          if (w.out_f32) outf[(long long)t * w.o.st + d] = 0.0f;
-          else out[(long long)t * w.o.st + d] = from_f<T>(0.0f);
-        }
-      }
+  for (int e = 0; e < 4; e++) {
+    const int dk = KT * (4 * g + e), dv = VT * (4 * g + e);
+    kd[e] = at(dk * ES, dk < kdim, FAR_D);
+    od[e] = at(dv * os, dv < vleft, FAR_D);
   }
-  hi = hi < len ? hi : len;
+  const unsigned kidx = at(KT * idx * ES, KT * idx < kdim, FAR_D), vidx = at(VT * idx * ES, VT * idx < vleft, FAR_D);
+  /* ... and of its tokens, for chunks of n: the lowest token of the chunk is the base */
+  unsigned qrow, krow, orow, kcol[4], vcol[4];
+  auto place = [&](int n) {
+    const unsigned back = n - 1 - idx, rel = rev ? back : idx;
+    qrow = at(rel * (unsigned)qst, idx < n, FAR_T);
+    krow = at(rel * (unsigned)kst, idx < n, FAR_T);
+    orow = at(rel * (unsigned)ost, idx < n, FAR_T);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int j = 4 * g + e;
+      const unsigned backj = n - 1 - j, rc = rev ? backj : j;
+      kcol[e] = at(rc * (unsigned)kst, j < n, FAR_T) + kidx;
+      vcol[e] = at(rc * (unsigned)vst, j < n, FAR_T) + vidx;
+    }
+  };
+  auto put = [&](int n, long long low, const float (&o)[4][VT]) {
+    const Rsrc ro = rsrc_of(out + low * ost);
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const unsigned off = orow + od[e];
+      const int left = vleft - VT * (4 * g + e);
+      if (w.out_f32) store_n<float, VT, VEC>(ro, off, left, o[e]);
+      else store_n<T, VT, VEC>(ro, off, left, o[e]);
+    }
+  };
 
-  const int srow = (int)w.srow, scol = (int)w.scol;
+  /* padding: zeros, in forward order whatever the walk */
+  if (!STATE) {
+    const float zero[4][VT] = {};
+    for (int t = len > lo ? len : lo; t < end; t += chunk) {
+      const int n = end - t < chunk ? end - t : chunk;
+      orow = at(idx * (unsigned)ost, idx < n, FAR_T);
+      put(n, t, zero);
+    }
+  }
+
   const long long bh = (long long)b * a.h + h;
-  const long long elems = (long long)a.kdim * a.vdim;
+  const long long elems = (long long)kdim * vdim;
   f4 S[KT][VT];
-#pragma unroll
-  for (int mt = 0; mt < KT; mt++)
-#pragma unroll
-    for (int nt = 0; nt < VT; nt++) S[mt][nt] = f4{0, 0, 0, 0};
-  const float* s_in = STATE ? nullptr : a.nsplit > 1 ? w.ws + (bh * a.nsplit + split) * elems
+  const float* s_in = STATE ? nullptr : nsplit > 1 ? w.ws + (bh * nsplit + split) * elems
                                                      : w.s_in ? w.s_in + bh * elems : nullptr;
+  /* S[mt][nt][e]: key channel KT (4 g + e) + mt, value channel v0 + VT idx + nt */
+  const unsigned srow = 4 * (w.state_t ? 1 : vdim), scol = 4 * (w.state_t ? kdim : 1);
+  auto state_off = [&](int dk, int dv) {
+    return at(dk * srow, dk < kdim, FAR_T) + at((v0 + dv) * scol, dv < vleft, FAR_D);
+  };
   if (s_in) {
+    const Rsrc rs = rsrc_of(s_in);
+    if (a.state_vec && !w.state_t) {
 #pragma unroll
-    for (int mt = 0; mt < KT; mt++)
+      for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          Raw<float, VT, true> x;
+          x.load(rs, state_off(KT * (4 * g + e) + mt, VT * idx), VT);
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++) S[mt][nt][e] = x.get(nt);
+        }
+    } else if (a.state_vec) {
 #pragma unroll
       for (int nt = 0; nt < VT; nt++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const int dk = KT * (4 * g + e) + mt, dv = VT * idx + nt;
-          if (dk < a.kdim && dv < vleft) S[mt][nt][e] = s_in[dk * srow + (v0 + dv) * scol];
+          Raw<float, KT, true> x;
+          x.load(rs, state_off(KT * (4 * g + e), VT * idx + nt), KT);
+#pragma unroll
+          for (int mt = 0; mt < KT; mt++) S[mt][nt][e] = x.get(mt);
         }
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            Raw<float, 1, true> x;
+            x.load(rs, state_off(KT * (4 * g + e) + mt, VT * idx + nt), 1);
+            S[mt][nt][e] = x.get(0);
+          }
+    }
+  } else {
+#pragma unroll
+    for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++) S[mt][nt] = f4{0, 0, 0, 0};
   }
 
-  const int e0 = w.reversed ? 0 : 1; /* the entering state has decayed by one step at position 0, or by none yet */
-  float dm[4], wk16[4];
+  const int e0 = rev ? 0 : 1; /* the entering state has decayed by one step at position 0, or by none yet */
+  float dm[4], wk[4];
 #pragma unroll
   for (int e = 0; e < 4; e++) {
     const int j = 4 * g + e;
     dm[e] = idx >= j ? w.p_scale * pw(l, idx - j) : 0.0f;
-    wk16[e] = w.w_scale * pw(l, 15 - j + (1 - e0));
   }
-  const float fi = w.in_scale * pw(l, idx + e0), g16 = pw(l, 16);
+  const float fi = w.in_scale * pw(l, idx + e0);
+  float gn = 1.0f;
 
   int single = 0; /* tokens left to take one by one */
+  int placed = 0;
   for (int p = lo; p < hi;) {
-    int n = hi - p < 16 ? hi - p : 16;
+    int n = hi - p < chunk ? hi - p : chunk;
     if (single) n = 1;
-    /* token of position x */
-    const long long t0 = w.reversed ? len - 1 - p : p;
-    const int step = w.reversed ? -1 : 1;
-    float kr[KT][4], kt[KT][4], qr[KT][4], vt[VT][4];
-    const bool row_ok = idx < n;
-    const long long trow = t0 + step * (row_ok ? idx : 0);
+    if (n != placed) {
+      placed = n;
+      place(n);
+      gn = pw(l, n);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int j = 4 * g + e;
+        wk[e] = j < n ? w.w_scale * pw(l, n - 1 - j + (1 - e0)) : 0.0f;
+      }
+    }
+    const long long low = rev ? len - p - n : p;
+    const Rsrc rk = rsrc_of(k + low * kst), rv = rsrc_of(v + low * vst);
+    Raw<T, KT, VEC> kr[4], qr[4], kc[4];
+    Raw<T, VT, VEC> vc[4];
+    if (!STATE) {
+      const Rsrc rq = rsrc_of(q + low * qst);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int left = kdim - KT * (4 * g + e);
+        kr[e].load(rk, krow + kd[e], left);
+        qr[e].load(rq, qrow + kd[e], left);
+      }
+    }
 #pragma unroll
     for (int e = 0; e < 4; e++) {
-      const int d = KT * (4 * g + e);
-      float xk[KT], xq[KT];
-#pragma unroll
-      for (int mt = 0; mt < KT; mt++) xk[mt] = xq[mt] = 0.0f;
-      if (!STATE) {
-        if constexpr (VEC) {
-          if (row_ok && d < a.kdim) {
-            ld_n<T, KT, true>(k + trow * w.k.st + d, xk);
-            ld_n<T, KT, true>(q + trow * w.q.st + d, xq);
-          }
-        } else {
-#pragma unroll
-          for (int mt = 0; mt < KT; mt++)
-            if (row_ok && d + mt < a.kdim) {
-              xk[mt] = to_f(k[trow * w.k.st + d + mt]);
-              xq[mt] = to_f(q[trow * w.q.st + d + mt]);
-            }
-        }
-      }
-#pragma unroll
-      for (int mt = 0; mt < KT; mt++) { kr[mt][e] = xk[mt]; qr[mt][e] = xq[mt]; }
+      vc[e].load(rv, vcol[e], vleft - VT * idx);
+      kc[e].load(rk, kcol[e], kdim - KT * idx);
     }
-    float bad = 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int j = 4 * g + e;
-      const long long tc = t0 + step * (j < n ? j : 0);
-      float xk[KT], xv[VT];
-#pragma unroll
-      for (int mt = 0; mt < KT; mt++) xk[mt] = 0.0f;
-#pragma unroll
-      for (int nt = 0; nt < VT; nt++) xv[nt] = 0.0f;
-      if constexpr (VEC) {
-        if (j < n && KT * idx < a.kdim) ld_n<T, KT, true>(k + tc * w.k.st + KT * idx, xk);
-        if (j < n && VT * idx < vleft) ld_n<T, VT, true>(v + tc * w.v.st + VT * idx, xv);
-      } else {
-#pragma unroll
-        for (int mt = 0; mt < KT; mt++)
-          if (j < n && KT * idx + mt < a.kdim) xk[mt] = to_f(k[tc * w.k.st + KT * idx + mt]);
-#pragma unroll
-        for (int nt = 0; nt < VT; nt++)
-          if (j < n && VT * idx + nt < vleft) xv[nt] = to_f(v[tc * w.v.st + VT * idx + nt]);
-      }
-#pragma unroll
-      for (int mt = 0; mt < KT; mt++) kt[mt][e] = xk[mt];
-#pragma unroll
-      for (int nt = 0; nt < VT; nt++) { vt[nt][e] = xv[nt]; bad = fmaf(xv[nt], 0.0f, bad); }
-    }
-    /* a value that is not finite must not meet the zeros of the mask (0 * inf): its chunk is taken token by
-       token, where every product belongs to the token */
-    if (n > 1 && __any(bad != 0.0f)) { single = n; continue; }
-
     /* bit i: an episode starts between positions i - 1 and i */
     unsigned brk = 0;
     if (starts) {
-      const int x = p + idx;
-      const long long ts = w.reversed ? len - x : x;
-      const bool f = row_ok && x < hi && !(w.reversed && x == 0) && starts[ts * a.starts_st];
-      brk = (unsigned)(__ballot(f) & 0xffffu);
+      /* position x of a reversed walk is token len - 1 - x, behind the start that token len - x may carry */
+      const Rsrc rs = rsrc_of(starts + (rev ? low + 1 : low) * starts_st);
+      const bool there = (idx < n) & ((p + idx != 0) | !rev);
+      const unsigned back = n - 1 - idx, rel = rev ? back : idx;
+      const unsigned f = __builtin_amdgcn_raw_buffer_load_b8(rs, at(rel * (unsigned)starts_st, there, FAR_T), 0, 0);
+      brk = (unsigned)(__ballot(f != 0) & 0xffffu);
     }
+
+    /* a value that is not finite must not meet the zeros of the mask (0 * inf): its chunk is taken token by
+       token, where every product belongs to the token */
+    float bad = 0.0f;
+#pragma unroll
+    for (int e = 0; e < 4; e++)
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++) bad = fmaf(vc[e].get(nt), 0.0f, bad);
+    if (n > 1 && __any(bad != 0.0f)) { single = n; continue; }
 
     if (!STATE) {
       f4 pt = {0, 0, 0, 0};
 #pragma unroll
       for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) pt = mfma4(kr[mt][e], qr[mt][e], pt);
+        for (int e = 0; e < 4; e++) pt = mfma4(kr[e].get(mt), qr[e].get(mt), pt);
       const unsigned upto = (2u << idx) - 1u; /* breaks at or in front of this lane's position */
-      float ps[4];
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const int j = 4 * g + e;
-        const bool ok = idx >= j && (brk & upto & ~((2u << j) - 1u)) == 0;
-        ps[e] = ok ? pt[e] * dm[e] : 0.0f;
+        const float x = pt[e] * dm[e];
+        const bool ok = (idx >= j) & ((brk & upto & ~((2u << j) - 1u)) == 0);
+        pt[e] = ok ? x : 0.0f;
       }
       const bool from_state = (brk & upto) == 0;
+      float o[4][VT];
 #pragma unroll
       for (int nt = 0; nt < VT; nt++) {
-        f4 o = {0, 0, 0, 0};
+        f4 x = {0, 0, 0, 0};
 #pragma unroll
         for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) o = mfma4(S[mt][nt][e], qr[mt][e], o);
+          for (int e = 0; e < 4; e++) x = mfma4(S[mt][nt][e], qr[e].get(mt), x);
 #pragma unroll
-        for (int e = 0; e < 4; e++) o[e] = from_state ? o[e] * fi : 0.0f;
-#pragma unroll
-        for (int e = 0; e < 4; e++) o = mfma4(vt[nt][e], ps[e], o);
-/* o[e]: channel VT * (4 g + e) + nt of token idx */
-        if (row_ok) {
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const int d = VT * (4 * g + e) + nt;
-            if (d < vleft) {
-              if (w.out_f32) outf[trow * w.o.st + d] = o[e];
-              else out[trow * w.o.st + d] = from_f<T>(o[e]);
-            }
-          }
+        for (int e = 0; e < 4; e++) {
+          const float y = x[e] * fi;
+          x[e] = from_state ? y : 0.0f;
         }
+#pragma unroll
+        for (int e = 0; e < 4; e++) x = mfma4(vc[e].get(nt), pt[e], x);
+#pragma unroll
+        for (int e = 0; e < 4; e++) o[e][nt] = x[e];
       }
+      /* o[e][nt]: channel VT (4 g + e) + nt of token idx */
+      put(n, low, o);
     }
 
-    const float gn = n == 16 ? g16 : pw(l, n);
     const bool keep = brk == 0;
 #pragma unroll
     for (int mt = 0; mt < KT; mt++)
 #pragma unroll
       for (int nt = 0; nt < VT; nt++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) S[mt][nt][e] = keep ? S[mt][nt][e] * gn : 0.0f;
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const int j = 4 * g + e;
-      const float wk = n == 16 ? wk16[e] : w.w_scale * pw(l, j < n ? n - 1 - j + (1 - e0) : 0);
-      const bool ok = j < n && (brk >> (j + 1)) == 0;
-#pragma unroll
-      for (int mt = 0; mt < KT; mt++) kt[mt][e] = ok ? kt[mt][e] * wk : 0.0f;
-    }
+        for (int e = 0; e < 4; e++) {
+          const float x = S[mt][nt][e] * gn;
+          S[mt][nt][e] = keep ? x : 0.0f;
+        }
 #pragma unroll
     for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-      for (int nt = 0; nt < VT; nt++)
+      for (int e = 0; e < 4; e++) {
+        const bool ok = (brk >> (4 * g + e + 1)) == 0;
+        const float x = kc[e].get(mt) * wk[e], kw = ok ? x : 0.0f;
 #pragma unroll
-        for (int e = 0; e < 4; e++) S[mt][nt] = mfma4(kt[mt][e], vt[nt][e], S[mt][nt]);
+        for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma4(kw, vc[e].get(nt), S[mt][nt]);
+      }
     p += n;
     if (single) single--;
   }
 
   float* s_out = nullptr;
-  if (STATE) s_out = w.ws + (bh * a.nsplit + split + 1) * elems;
-  else if (split == a.nsplit - 1 && w.s_out) s_out = w.s_out + bh * elems;
+  if (STATE) s_out = w.ws + (bh * nsplit + split + 1) * elems;
+  else if (split == nsplit - 1 && w.s_out) s_out = w.s_out + bh * elems;
   if (s_out) {
     /* the state in front of a start that the first token carries gets no gradient */
-    const bool cut = !STATE && w.reversed && starts && len > 0 && starts[0];
+    if (!STATE && rev && starts && len > 0 && starts[0]) {
 #pragma unroll
-    for (int mt = 0; mt < KT; mt++)
+      for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++) S[mt][nt] = f4{0, 0, 0, 0};
+    }
+    const Rsrc rs = rsrc_of(s_out);
+    if (a.state_vec && !w.state_t) {
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          float x[VT];
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++) x[nt] = S[mt][nt][e];
+          store_n<float, VT, true>(rs, state_off(KT * (4 * g + e) + mt, VT * idx), VT, x);
+        }
+    } else if (a.state_vec) {
 #pragma unroll
       for (int nt = 0; nt < VT; nt++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const int dk = KT * (4 * g + e) + mt, dv = VT * idx + nt;
-          if (dk < a.kdim && dv < vleft) s_out[dk * srow + (v0 + dv) * scol] = cut ? 0.0f : S[mt][nt][e];
+          float x[KT];
+#pragma unroll
+          for (int mt = 0; mt < KT; mt++) x[mt] = S[mt][nt][e];
+          store_n<float, KT, true>(rs, state_off(KT * (4 * g + e), VT * idx + nt), KT, x);
         }
+    } else {
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float x = S[mt][nt][e];
+            store_n<float, 1, true>(rs, state_off(KT * (4 * g + e) + mt, VT * idx + nt), 1, &x);
+          }
+    }
   }
 }
 
@@ -544,6 +690,7 @@ static int attn_check(const ur3e_attn_t* a) {
     return bad_arg("attention: dk and dv must be in [1, 128]");
   if ((long long)a->b * a->heads > 4194303) return bad_arg("attention: b * heads must be below 2^22");
   if (a->b == 0) return UR3E_OK;
+  if (a->q.st < 0 || a->k.st < 0 || a->v.st < 0 || a->starts_st < 0) return bad_arg("attention: token strides must not be negative");
   if (!a->log_decay) return bad_arg("attention: null log_decay");
   if (a->t > 0 && (!a->q.p || !a->k.p || !a->v.p)) return bad_arg("attention: null q, k or v");
   return UR3E_OK;
@@ -583,6 +730,7 @@ static size_t walk_bytes(const Plan& p, long long b, int h, int kdim, int vdim) 
   return p.nsplit > 1 ? (size_t)b * h * p.nsplit * kdim * vdim * sizeof(float) : 0;
 }
 
+/* groups of kt channels can be moved whole: all there or none, on their boundary */
 static bool aligned(const Tok& t, int e, int kt, int d) {
   const int by = kt * e < 16 ? kt * e : 16;
   return d % kt == 0 && (uintptr_t)t.p % by == 0 && t.sb * e % by == 0 && t.st * e % by == 0 && t.sh * e % by == 0;
@@ -600,20 +748,32 @@ template <class T, int KT, int VT, bool VEC> static int walk_launch(const WalkAr
   PL_CHK(hipGetLastError());
   return UR3E_OK;
 }
-template <class T, int KT, int VT> static int walk_vec(const WalkArgs& a, hipStream_t s) {
+template <class T, int KT, int VT> static int walk_vec(WalkArgs& a, hipStream_t s) {
   bool vec = true;
+  a.state_vec = 1;
+  a.chunk = 16;
+  /* 16 tokens within the 30-bit offsets of a chunk, else token by token */
+  const long long far = ((1LL << 30) - 1024) / 64;
+  if (a.starts_st > far) a.chunk = 1;
+  for (int i = 0; i < a.nw; i++) {
+    const Walk& w = a.w[i];
+    if (w.q.st > far || w.k.st > far || w.v.st > far || w.o.st > far) a.chunk = 1;
+    const int by = 4 * (w.state_t ? KT : VT) < 16 ? 4 * (w.state_t ? KT : VT) : 16;
+    if ((w.state_t ? a.kdim % KT : a.vdim % VT) || (uintptr_t)w.s_in % by || (uintptr_t)w.s_out % by || (uintptr_t)w.ws % by)
+      a.state_vec = 0;
+  }
   for (int i = 0; i < a.nw; i++)
     vec = vec && aligned(a.w[i].q, sizeof(T), KT, a.kdim) && aligned(a.w[i].k, sizeof(T), KT, a.kdim) &&
-          aligned(a.w[i].v, sizeof(T), VT, a.vdim);
+          aligned(a.w[i].v, sizeof(T), VT, a.vdim) && aligned(a.w[i].o, a.w[i].out_f32 ? 4 : (int)sizeof(T), VT, a.vdim);
   return vec ? walk_launch<T, KT, VT, true>(a, s) : walk_launch<T, KT, VT, false>(a, s);
 }
-template <class T, int KT> static int walk_vt(const WalkArgs& a, int vt, hipStream_t s) {
+template <class T, int KT> static int walk_vt(WalkArgs& a, int vt, hipStream_t s) {
   if (vt == 1) return walk_vec<T, KT, 1>(a, s);
   if (vt == 2) return walk_vec<T, KT, 2>(a, s);
   if constexpr (KT < 8) return walk_vec<T, KT, 4>(a, s);
   return ur3e_internal_fail(UR3E_EINVAL, "attention: no such tile");
 }
-template <class T> static int walk_kt(const WalkArgs& a, const Plan& p, hipStream_t s) {
+template <class T> static int walk_kt(WalkArgs& a, const Plan& p, hipStream_t s) {
   switch (p.kt) {
     case 1: return walk_vt<T, 1>(a, p.vt, s);
     case 2: return walk_vt<T, 2>(a, p.vt, s);
@@ -621,7 +781,7 @@ template <class T> static int walk_kt(const WalkArgs& a, const Plan& p, hipStrea
     default: return walk_vt<T, 8>(a, p.vt, s);
   }
 }
-static int walk_run(int dtype, const WalkArgs& a, const Plan& p, hipStream_t s) {
+static int walk_run(int dtype, WalkArgs& a, const Plan& p, hipStream_t s) {
   if (dtype == UR3E_F32) return walk_kt<float>(a, p, s);
   if (dtype == UR3E_BF16) return walk_kt<Bf16>(a, p, s);
   return walk_kt<F16>(a, p, s);
@@ -664,6 +824,7 @@ extern "C" int ur3e_attn_forward(const ur3e_attn_t* a, const ur3e_tokens_t* out,
   if (rc) return rc;
   if (a->b == 0) return UR3E_OK;
   if (!out || (a->t > 0 && !out->p)) return bad_arg("attention: null out");
+  if (out->st < 0) return bad_arg("attention: token strides must not be negative");
   if (workspace_bytes < attn_bytes(a, 0) || (attn_bytes(a, 0) && !workspace)) return bad_arg("attention: workspace too small");
   const Plan p = plan_of(a->b, a->t, a->heads, a->dk, a->dv, 1);
   WalkArgs w = args_of(a, a->dk, a->dv, p);
@@ -671,8 +832,6 @@ extern "C" int ur3e_attn_forward(const ur3e_attn_t* a, const ur3e_tokens_t* out,
   w.nw = 1;
   Walk& f = w.w[0];
   f.q = tok_of(a->q, 1); f.k = tok_of(a->k, grp); f.v = tok_of(a->v, grp); f.o = tok_of(*out, 1);
-  f.out = out->p;
-  f.srow = a->dv; f.scol = 1;
   f.s_in = a->s0; f.s_out = s_out; f.ws = (float*)workspace;
   f.in_scale = f.p_scale = a->scale; f.w_scale = 1.0f;
   return walk_run(a->dtype, w, p, (hipStream_t)stream);
@@ -686,6 +845,7 @@ extern "C" int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dou
   if (a->b == 0) return UR3E_OK;
   if (!dout || !dq || !dk || !dv) return bad_arg("attention: null gradient");
   if (a->t > 0 && (!dout->p || !dq->p || !dk->p || !dv->p)) return bad_arg("attention: null gradient");
+  if (dout->st < 0 || dq->st < 0 || dk->st < 0 || dv->st < 0) return bad_arg("attention: token strides must not be negative");
   if (workspace_bytes < attn_bytes(a, 1) || (attn_bytes(a, 1) && !workspace)) return bad_arg("attention: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   const int grp = a->heads / a->kv_heads;
@@ -699,24 +859,23 @@ extern "C" int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dou
     fv = (float*)(ws + 2 * n1 + n2 + up16((size_t)a->b * a->t * a->heads * a->dk * 4));
   }
   const Tok tq = tok_of(a->q, 1), tk = tok_of(a->k, grp), tv = tok_of(a->v, grp), tdo = tok_of(*dout, 1);
-  auto wide = [&](int d) { return Tok{nullptr, (long long)a->t * a->heads * d, (long long)a->heads * d, d, 1}; };
+  auto wide = [&](const float* p, int d) { return Tok{p, (long long)a->t * a->heads * d, (long long)a->heads * d, d, 1}; };
   Walk q = {}, k = {}, v = {};
   /* dq = walk(do, v, k) on S^T */
-  q.q = tdo; q.k = tv; q.v = tk; q.o = tok_of(*dq, 1); q.out = dq->p;
-  q.srow = 1; q.scol = a->dv;
+  q.q = tdo; q.k = tv; q.v = tk; q.o = tok_of(*dq, 1);
+  q.state_t = 1;
   q.s_in = a->s0; q.ws = (float*)ws;
   q.in_scale = q.p_scale = a->scale; q.w_scale = 1.0f;
   /* dk = reversed walk(v, do, q) on G^T */
-  k.q = tv; k.k = tdo; k.v = tq; k.o = grp > 1 ? wide(a->dk) : tok_of(*dk, 1); k.out = grp > 1 ? (void*)fk : dk->p;
+  k.q = tv; k.k = tdo; k.v = tq; k.o = grp > 1 ? wide(fk, a->dk) : tok_of(*dk, 1);
   k.out_f32 = grp > 1;
-  k.srow = 1; k.scol = a->dv;
+  k.state_t = 1;
   k.s_in = ds_out; k.ws = (float*)(ws + n1);
   k.reversed = 1;
   k.in_scale = 1.0f; k.p_scale = k.w_scale = a->scale;
   /* dv = reversed walk(k, q, do) on G */
-  v.q = tk; v.k = tq; v.v = tdo; v.o = grp > 1 ? wide(a->dv) : tok_of(*dv, 1); v.out = grp > 1 ? (void*)fv : dv->p;
+  v.q = tk; v.k = tq; v.v = tdo; v.o = grp > 1 ? wide(fv, a->dv) : tok_of(*dv, 1);
   v.out_f32 = grp > 1;
-  v.srow = a->dv; v.scol = 1;
   v.s_in = ds_out; v.s_out = ds0; v.ws = (float*)(ws + 2 * n1);
   v.reversed = 1;
   v.in_scale = 1.0f; v.p_scale = v.w_scale = a->scale;
