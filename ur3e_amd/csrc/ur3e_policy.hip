@@ -96,7 +96,8 @@ struct Walk {
   Tok q, k, v, o;           /* o.p is written */
   const float* s_in;        /* [b][h][dk * dv] or null */
   float* s_out;             /* or null */
-  float* ws;                /* [b][h][split][kdim * vdim]: split s holds the state that enters it (nsplit > 1) */
+  float* ws;                /* nsplit > 1: [b][h][split][kdim * vdim], split s holds the state that enters it, */
+  float* wf;                /* and [b][h][split], what split s - 1 multiplies the state by */
   int state_t;              /* a [dk][dv] state is this walk's transposed: kdim = dv */
   int reversed;
   int out_f32;              /* out is float whatever the token type (gradients that are summed over heads) */
@@ -192,6 +193,60 @@ template <class T, int N, bool VEC> __device__ __forceinline__ void store_n(Rsrc
       if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x[i]), r, o, 0, 0);
       else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, from_f<T>(x[i])), r, o, 0, 0);
     }
+  }
+}
+
+/* whether one of the elements is an infinity or a NaN: its exponent carries into the sign's place */
+template <class T, int N, bool VEC> __device__ __forceinline__ unsigned not_finite(const Raw<T, N, VEC>& x) {
+  constexpr unsigned abs = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
+  constexpr unsigned one = sizeof(T) == 4 ? 0x00800000u : __is_same(T, Bf16) ? 0x00800080u : 0x04000400u;
+  unsigned r = 0;
+#pragma unroll
+  for (int i = 0; i < Raw<T, N, VEC>::D; i++) r |= (x.d[i] & abs) + one;
+  return r & ~abs;
+}
+
+/* bfloat16 fragments, two elements to a dword.  A 32-bit operand enters the matrix instructions as the sum of
+   its leading parts of 8 bits each: two (error 2^-17) for scores and state, whose results are rounded to 2^-9
+   on the way out, three (2^-25) for what is added to the state. */
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, b2{(__bf16)lo, (__bf16)hi});
+}
+/* hi = the packed leading parts of x0, x1; x0, x1 become the rest */
+__device__ __forceinline__ unsigned split_bf16(float& x0, float& x1) {
+  const unsigned hi = pack_bf16(x0, x1);
+  x0 -= __builtin_bit_cast(float, hi << 16);
+  x1 -= __builtin_bit_cast(float, hi & 0xffff0000u);
+  return hi;
+}
+/* the K = 32 shape throughout, half empty where four elements are all there is: a K = 16 instruction right behind
+   a K = 32 one on the same accumulators read them before the first had written (the compiler had put one wait
+   state between the two; measured at one tile, where nothing else stands between them) */
+__device__ __forceinline__ f4 mfma32(u4 a, u4 b, f4 c) {
+  typedef __bf16 b8 __attribute__((ext_vector_type(8)));
+  return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
+}
+/* the 4 KT elements of a lane's row form, four to a u2: element KT e + mt of group e, tile mt */
+template <int KT, bool VEC> __device__ __forceinline__ void pack_row(const Raw<Bf16, KT, VEC> (&x)[4], u2 (&y)[KT]) {
+  unsigned d[2 * KT];
+  if constexpr (VEC && KT > 1) {
+#pragma unroll
+    for (int i = 0; i < 2 * KT; i++) d[i] = x[i / (KT / 2)].d[i % (KT / 2)];
+  } else {
+#pragma unroll
+    for (int i = 0; i < 2 * KT; i++) d[i] = x[2 * i / KT].d[2 * i % KT] | x[(2 * i + 1) / KT].d[(2 * i + 1) % KT] << 16;
+  }
+#pragma unroll
+  for (int i = 0; i < KT; i++) y[i] = u2{d[2 * i], d[2 * i + 1]};
+}
+/* the four tokens of tile nt in the column form */
+template <int VT, bool VEC> __device__ __forceinline__ u2 pack_col(const Raw<Bf16, VT, VEC> (&x)[4], int nt) {
+  if constexpr (VEC && VT > 1) {
+    const unsigned sel = nt & 1 ? 0x07060302u : 0x05040100u; /* the high or the low halves of two dwords */
+    return u2{__builtin_amdgcn_perm(x[1].d[nt / 2], x[0].d[nt / 2], sel), __builtin_amdgcn_perm(x[3].d[nt / 2], x[2].d[nt / 2], sel)};
+  } else {
+    return u2{x[0].d[nt] | x[1].d[nt] << 16, x[2].d[nt] | x[3].d[nt] << 16};
   }
 }
 
@@ -338,7 +393,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   const float fi = w.in_scale * pw(l, idx + e0);
   float gn = 1.0f;
 
-  int single = 0; /* tokens left to take one by one */
+  float through = 1.0f; /* STATE: what the split multiplies an entering state by */
+  int single = 0;       /* tokens left to take one by one */
   int placed = 0;
   for (int p = lo; p < hi;) {
     int n = hi - p < chunk ? hi - p : chunk;
@@ -384,20 +440,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 
     /* a value that is not finite must not meet the zeros of the mask (0 * inf): its chunk is taken token by
        token, where every product belongs to the token */
-    float bad = 0.0f;
+    unsigned bad = 0;
 #pragma unroll
-    for (int e = 0; e < 4; e++)
-#pragma unroll
-      for (int nt = 0; nt < VT; nt++) bad = fmaf(vc[e].get(nt), 0.0f, bad);
-    if (n > 1 && __any(bad != 0.0f)) { single = n; continue; }
+    for (int e = 0; e < 4; e++) bad |= not_finite(vc[e]);
+    if (n > 1 && __any(bad != 0)) { single = n; continue; }
 
-    if (!STATE) {
-      f4 pt = {0, 0, 0, 0};
-#pragma unroll
-      for (int mt = 0; mt < KT; mt++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) pt = mfma4(kr[e].get(mt), qr[e].get(mt), pt);
-      const unsigned upto = (2u << idx) - 1u; /* breaks at or in front of this lane's position */
+    const unsigned upto = (2u << idx) - 1u; /* breaks at or in front of this lane's position */
+    const bool from_state = (brk & upto) == 0, keep = brk == 0;
+    auto scores = [&](f4& pt) { /* the scores of token idx with keys 4 g + e, masked and decayed */
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const int j = 4 * g + e;
@@ -405,54 +455,120 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         const bool ok = (idx >= j) & ((brk & upto & ~((2u << j) - 1u)) == 0);
         pt[e] = ok ? x : 0.0f;
       }
-      const bool from_state = (brk & upto) == 0;
-      float o[4][VT];
+    };
+    auto entering = [&](f4& x) { /* the read-out of the entering state for token idx */
 #pragma unroll
-      for (int nt = 0; nt < VT; nt++) {
-        f4 x = {0, 0, 0, 0};
+      for (int e = 0; e < 4; e++) {
+        const float y = x[e] * fi;
+        x[e] = from_state ? y : 0.0f;
+      }
+    };
+    auto decay = [&] {
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) {
+            const float x = S[mt][nt][e] * gn;
+            S[mt][nt][e] = keep ? x : 0.0f;
+          }
+    };
+    auto key = [&](int mt, int e) { /* k of token 4 g + e as it enters the state behind the chunk */
+      const float x = kc[e].get(mt) * wk[e];
+      return (brk >> (4 * g + e + 1)) == 0 ? x : 0.0f;
+    };
+    float o[4][VT]; /* o[e][nt]: channel VT (4 g + e) + nt of token idx */
+    if constexpr (__is_same(T, Bf16)) {
+      u2 vq[VT];
+#pragma unroll
+      for (int nt = 0; nt < VT; nt++) vq[nt] = pack_col<VT, VEC>(vc, nt);
+      if (!STATE) {
+        u2 kq[KT], qq[KT];
+        pack_row<KT, VEC>(kr, kq);
+        pack_row<KT, VEC>(qr, qq);
+        f4 pt = {0, 0, 0, 0};
+        if constexpr (KT == 1) pt = mfma32(u4{kq[0].x, kq[0].y, 0, 0}, u4{qq[0].x, qq[0].y, 0, 0}, pt);
+#pragma unroll
+        for (int i = 0; i + 1 < KT; i += 2)
+          pt = mfma32(u4{kq[i].x, kq[i].y, kq[i + 1].x, kq[i + 1].y}, u4{qq[i].x, qq[i].y, qq[i + 1].x, qq[i + 1].y}, pt);
+        scores(pt);
+        float p0 = pt[0], p1 = pt[1], p2 = pt[2], p3 = pt[3];
+        const unsigned h0 = split_bf16(p0, p1), h1 = split_bf16(p2, p3);
+        const u4 ph = {h0, h1, pack_bf16(p0, p1), pack_bf16(p2, p3)};
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++) {
+          f4 x = {0, 0, 0, 0};
+#pragma unroll
+          for (int i = 0; i < KT; i++) {
+            /* the state's elements of the four channels in qq[i] */
+            float s0 = S[4 * i % KT][nt][4 * i / KT], s1 = S[(4 * i + 1) % KT][nt][(4 * i + 1) / KT],
+                  s2 = S[(4 * i + 2) % KT][nt][(4 * i + 2) / KT], s3 = S[(4 * i + 3) % KT][nt][(4 * i + 3) / KT];
+            const unsigned a0 = split_bf16(s0, s1), a1 = split_bf16(s2, s3);
+            x = mfma32(u4{a0, a1, pack_bf16(s0, s1), pack_bf16(s2, s3)}, u4{qq[i].x, qq[i].y, qq[i].x, qq[i].y}, x);
+          }
+          entering(x);
+          x = mfma32(u4{vq[nt].x, vq[nt].y, vq[nt].x, vq[nt].y}, ph, x);
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[e][nt] = x[e];
+        }
+        put(n, low, o);
+      }
+      decay();
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++) {
+        float k0 = key(mt, 0), k1 = key(mt, 1), k2 = key(mt, 2), k3 = key(mt, 3);
+        const unsigned h0 = split_bf16(k0, k1), h1 = split_bf16(k2, k3), m0 = split_bf16(k0, k1), m1 = split_bf16(k2, k3);
+        const u4 rest = {pack_bf16(k0, k1), pack_bf16(k2, k3), 0, 0};
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++) {
+          S[mt][nt] = mfma32(u4{h0, h1, m0, m1}, u4{vq[nt].x, vq[nt].y, vq[nt].x, vq[nt].y}, S[mt][nt]);
+          S[mt][nt] = mfma32(rest, u4{vq[nt].x, vq[nt].y, 0, 0}, S[mt][nt]);
+        }
+      }
+    } else {
+      if (!STATE) {
+        f4 pt = {0, 0, 0, 0};
 #pragma unroll
         for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) x = mfma4(S[mt][nt][e], qr[e].get(mt), x);
+          for (int e = 0; e < 4; e++) pt = mfma4(kr[e].get(mt), qr[e].get(mt), pt);
+        scores(pt);
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++) {
+          f4 x = {0, 0, 0, 0};
+#pragma unroll
+          for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x = mfma4(S[mt][nt][e], qr[e].get(mt), x);
+          entering(x);
+#pragma unroll
+          for (int e = 0; e < 4; e++) x = mfma4(vc[e].get(nt), pt[e], x);
+#pragma unroll
+          for (int e = 0; e < 4; e++) o[e][nt] = x[e];
+        }
+        put(n, low, o);
+      }
+      decay();
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float y = x[e] * fi;
-          x[e] = from_state ? y : 0.0f;
+          const float kw = key(mt, e);
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma4(kw, vc[e].get(nt), S[mt][nt]);
         }
-#pragma unroll
-        for (int e = 0; e < 4; e++) x = mfma4(vc[e].get(nt), pt[e], x);
-#pragma unroll
-        for (int e = 0; e < 4; e++) o[e][nt] = x[e];
-      }
-      /* o[e][nt]: channel VT (4 g + e) + nt of token idx */
-      put(n, low, o);
     }
-
-    const bool keep = brk == 0;
-#pragma unroll
-    for (int mt = 0; mt < KT; mt++)
-#pragma unroll
-      for (int nt = 0; nt < VT; nt++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const float x = S[mt][nt][e] * gn;
-          S[mt][nt][e] = keep ? x : 0.0f;
-        }
-#pragma unroll
-    for (int mt = 0; mt < KT; mt++)
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const bool ok = (brk >> (4 * g + e + 1)) == 0;
-        const float x = kc[e].get(mt) * wk[e], kw = ok ? x : 0.0f;
-#pragma unroll
-        for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma4(kw, vc[e].get(nt), S[mt][nt]);
-      }
+    if (STATE) through = keep ? through * gn : 0.0f;
     p += n;
     if (single) single--;
   }
 
   float* s_out = nullptr;
-  if (STATE) s_out = w.ws + (bh * nsplit + split + 1) * elems;
+  if (STATE) {
+    s_out = w.ws + (bh * nsplit + split + 1) * elems;
+    if (slab == 0 && lane == 0) w.wf[bh * nsplit + split + 1] = through;
+  }
   else if (split == nsplit - 1 && w.s_out) s_out = w.s_out + bh * elems;
   if (s_out) {
     /* the state in front of a start that the first token carries gets no gradient */
@@ -498,36 +614,38 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 }
 
 /* States that enter each split: ws[s] holds split s - 1's own sum (k_attn_walk, STATE) and becomes
-   X_s = gamma^(tokens of split s - 1) X_{s-1} + ws[s], X_0 = s_in; the decay is 0 across an episode start. */
-__global__ __launch_bounds__(256) void k_attn_join(WalkArgs a) {
-  const Walk& w = a.w[blockIdx.z];
+   X_s = wf[s] X_{s-1} + ws[s], X_0 = s_in.  A thread owns VW elements and runs along the splits, whose sums it
+   loads JOIN at a time (nothing but the chain of multiply-adds depends on the split in front). */
+#define JOIN 16
+template <int VW> __global__ __launch_bounds__(64) void k_attn_join(WalkArgs a) {
+  const Walk w = a.w[blockIdx.z];
   const long long bh = blockIdx.y;
-  const int b = (int)(bh / a.h), h = (int)(bh % a.h);
-  const long long elems = (long long)a.kdim * a.vdim;
-  const float l = a.log_decay[h];
-  int len = a.t;
-  if (a.lengths) {
-    len = a.lengths[b];
-    len = len < 0 ? 0 : len > a.t ? a.t : len;
-  }
-  const int e = blockIdx.x * 256 + threadIdx.x;
-  float* ws = w.ws + bh * a.nsplit * elems;
-  float x = 0.0f;
-  if (e < elems && w.s_in) x = w.s_in[bh * elems + e];
-  for (int s = 0;; s++) {
-    if (e < elems) ws[s * elems + e] = x;
-    if (s == a.nsplit - 1) break;
-    int lo = s * a.split_len, hi = lo + a.split_len;
-    hi = hi < len ? hi : len;
-    lo = lo < hi ? lo : hi;
-    bool brk = false;
-    if (a.starts) {
-      const unsigned char* st = a.starts + b * a.starts_sb;
-      for (int p = lo + (int)threadIdx.x; p < hi; p += 256)
-        if (!(w.reversed && p == 0)) brk |= st[(w.reversed ? len - p : p) * a.starts_st] != 0;
-      brk = __syncthreads_or(brk);
+  const int elems = a.kdim * a.vdim, nsplit = a.nsplit;
+  const int e = (blockIdx.x * 64 + threadIdx.x) * VW;
+  if (e >= elems) return;
+  struct alignas(4 * VW) Pack { float x[VW]; };
+  float* ws = w.ws + bh * nsplit * elems + e;
+  const float* wf = w.wf + bh * nsplit;
+  Pack x = {};
+  if (w.s_in) x = *reinterpret_cast<const Pack*>(w.s_in + bh * elems + e);
+  for (int s0 = 0; s0 < nsplit; s0 += JOIN) {
+    Pack u[JOIN];
+    float f[JOIN];
+#pragma unroll
+    for (int i = 0; i < JOIN; i++) {
+      const int s = s0 + 1 + i < nsplit ? s0 + 1 + i : nsplit - 1;
+      u[i] = *reinterpret_cast<const Pack*>(ws + (long long)s * elems);
+      f[i] = wf[s];
     }
-    if (e < elems) x = (brk ? 0.0f : x * pw(l, hi - lo)) + ws[(s + 1) * elems + e];
+#pragma unroll
+    for (int i = 0; i < JOIN; i++) {
+      if (s0 + i < nsplit) *reinterpret_cast<Pack*>(ws + (long long)(s0 + i) * elems) = x;
+#pragma unroll
+      for (int c = 0; c < VW; c++) {
+        const float y = f[i] * x.x[c];
+        x.x[c] = (f[i] == 0.0f ? 0.0f : y) + u[i].x[c];
+      }
+    }
   }
 }
 
@@ -727,7 +845,7 @@ static Plan plan_of(int b, int t, int h, int kdim, int vdim, int walks) {
 }
 
 static size_t walk_bytes(const Plan& p, long long b, int h, int kdim, int vdim) {
-  return p.nsplit > 1 ? (size_t)b * h * p.nsplit * kdim * vdim * sizeof(float) : 0;
+  return p.nsplit > 1 ? (size_t)b * h * p.nsplit * (kdim * vdim + 1) * sizeof(float) : 0;
 }
 
 /* groups of kt channels can be moved whole: all there or none, on their boundary */
@@ -741,7 +859,11 @@ template <class T, int KT, int VT, bool VEC> static int walk_launch(const WalkAr
   if (a.nsplit > 1) {
     hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, true>), dim3((unsigned)((streams * (a.nsplit - 1) + 3) / 4)), dim3(256), 0, s, a);
     PL_CHK(hipGetLastError());
-    hipLaunchKernelGGL(k_attn_join, dim3((a.kdim * a.vdim + 255) / 256, (unsigned)(a.b * a.h), (unsigned)a.nw), dim3(256), 0, s, a);
+    const int elems = a.kdim * a.vdim;
+    if (elems % 4 == 0 && a.state_vec)
+      hipLaunchKernelGGL((k_attn_join<4>), dim3((elems + 255) / 256, (unsigned)(a.b * a.h), (unsigned)a.nw), dim3(64), 0, s, a);
+    else
+      hipLaunchKernelGGL((k_attn_join<1>), dim3((elems + 63) / 64, (unsigned)(a.b * a.h), (unsigned)a.nw), dim3(64), 0, s, a);
     PL_CHK(hipGetLastError());
   }
   hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false>), dim3((unsigned)((streams * a.nsplit + 3) / 4)), dim3(256), 0, s, a);
@@ -758,9 +880,9 @@ template <class T, int KT, int VT> static int walk_vec(WalkArgs& a, hipStream_t 
   for (int i = 0; i < a.nw; i++) {
     const Walk& w = a.w[i];
     if (w.q.st > far || w.k.st > far || w.v.st > far || w.o.st > far) a.chunk = 1;
-    const int by = 4 * (w.state_t ? KT : VT) < 16 ? 4 * (w.state_t ? KT : VT) : 16;
-    if ((w.state_t ? a.kdim % KT : a.vdim % VT) || (uintptr_t)w.s_in % by || (uintptr_t)w.s_out % by || (uintptr_t)w.ws % by)
+    if ((w.state_t ? a.kdim % KT : a.vdim % VT) || (uintptr_t)w.s_in % 16 || (uintptr_t)w.s_out % 16 || (uintptr_t)w.ws % 16)
       a.state_vec = 0;
+    a.w[i].wf = w.ws ? w.ws + (long long)a.b * a.h * a.nsplit * a.kdim * a.vdim : nullptr;
   }
   for (int i = 0; i < a.nw; i++)
     vec = vec && aligned(a.w[i].q, sizeof(T), KT, a.kdim) && aligned(a.w[i].k, sizeof(T), KT, a.kdim) &&
