@@ -181,28 +181,50 @@ def test_dropout_refuses():
             ops.keyed_dropout(*a, **kw)
 
 
+class TokensC(ctypes.Structure):
+    _fields_ = [("p", ctypes.c_void_p), ("sb", ctypes.c_longlong), ("st", ctypes.c_longlong),
+                ("sh", ctypes.c_longlong)]
+
+
+class AttnC(ctypes.Structure):
+    _fields_ = [("b", ctypes.c_int), ("t", ctypes.c_int), ("heads", ctypes.c_int), ("kv_heads", ctypes.c_int),
+                ("dk", ctypes.c_int), ("dv", ctypes.c_int), ("dtype", ctypes.c_int), ("scale", ctypes.c_float),
+                ("q", TokensC), ("k", TokensC), ("v", TokensC), ("log_decay", ctypes.c_void_p),
+                ("s0", ctypes.c_void_p), ("starts", ctypes.c_void_p), ("starts_sb", ctypes.c_longlong),
+                ("starts_st", ctypes.c_longlong), ("lengths", ctypes.c_void_p)]
+
+
 def test_c_entries_refuse_before_any_launch():
     """every refusal of the C entries comes from the host (no GPU here); empty calls succeed"""
-    L = ops._lib()
+    from ur3e_amd import runtime as rt
+    L = rt.load_library()
     EINVAL = -1
+    vp, sz, ll, ip = ctypes.c_void_p, ctypes.c_size_t, ctypes.c_longlong, ctypes.c_int
+    L.ur3e_attn_workspace.argtypes = [vp, ip, vp]
+    L.ur3e_attn_forward.argtypes = [vp, vp, vp, vp, sz, vp]
+    L.ur3e_attn_backward.argtypes = [vp] * 8 + [sz, vp]
+    L.ur3e_attn_step.argtypes = [vp] * 5
+    L.ur3e_keyed_dropout.argtypes = [ip, ll, ip, vp, ll, vp, ll, vp, ll, vp, ctypes.c_ulonglong, ctypes.c_uint, ip, vp]
 
     def attn(**kw):
-        a = ops.AttnC()
+        a = AttnC()
         a.b, a.t, a.heads, a.kv_heads, a.dk, a.dv, a.dtype, a.scale = 1, 4, 2, 1, 8, 8, 0, 1.0
-        a.q = a.k = a.v = ops.TokensC(4096, 64, 16, 8)
+        a.q = a.k = a.v = TokensC(4096, 64, 16, 8)
         a.log_decay = 4096
         for n, x in kw.items():
             setattr(a, n, x)
         return a
-    tok = ops.TokensC(4096, 64, 16, 8)
-    null = ops.TokensC(None, 64, 16, 8)
+    tok = TokensC(4096, 64, 16, 8)
+    null = TokensC(None, 64, 16, 8)
 
     def fwd(a, out=tok, ws=None, n=0):
         return L.ur3e_attn_forward(ctypes.byref(a) if a else None, ctypes.byref(out) if out else None, None, ws, n, None)
     for a in (None, attn(dtype=3), attn(dtype=-1), attn(b=-1), attn(t=-1), attn(heads=0), attn(kv_heads=0),
               attn(heads=3, kv_heads=2), attn(dk=0), attn(dk=129), attn(dv=0), attn(dv=129), attn(log_decay=None),
-              attn(q=null), attn(k=null), attn(v=null), attn(b=1 << 22)):
+              attn(q=null), attn(k=null), attn(v=null), attn(b=1 << 22),
+              attn(q=TokensC(4096, 64, -16, 8)), attn(starts_st=-1)):
         assert fwd(a) == EINVAL and L.ur3e_last_error()
+    assert fwd(attn(), TokensC(4096, 64, -16, 8)) == EINVAL
     assert fwd(attn(), None) == EINVAL and fwd(attn(), null) == EINVAL
     assert fwd(attn(b=0)) == 0
     n = ctypes.c_size_t()

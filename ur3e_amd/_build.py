@@ -13,6 +13,7 @@ HERE = os.path.dirname(os.path.abspath(__file__))
 SRC = os.path.join(HERE, "csrc", "ur3e_batch.hip")
 SRC_VN = os.path.join(HERE, "csrc", "ur3e_vecnorm.hip")
 SRC_PL = os.path.join(HERE, "csrc", "ur3e_policy.hip")  # the operators of ur3e_amd/rl/ops.py
+SRC_PL_TORCH = os.path.join(HERE, "csrc", "ur3e_policy_torch.cpp")  # their torch binding, a library of its own
 SRC_MJCF = os.path.join(HERE, "csrc", "ur3e_mjcf.cpp")  # host only: the MJCF / YAML entry points
 SRC_GATHER = os.path.join(HERE, "csrc", "ur3e_gather.cpp")  # host only: the RCCL gather entry point
 DEPS = [SRC, SRC_VN, SRC_PL, SRC_MJCF, SRC_GATHER, os.path.join(HERE, "..", "include", "ur3e_vecnorm.h"),
@@ -176,6 +177,37 @@ def _objects(defs, tag, force, verbose):
     return objs, jobs
 
 
+# the policy operators' torch binding: host code against this interpreter's torch, linked to the product library
+# beside it
+TORCH_LIB = os.path.join(HERE, "_lib", "ur3e_policy_torch.so")
+
+
+def _torch_cmd():
+    import sysconfig
+
+    import torch
+    from torch.utils import cpp_extension as ce
+    lib = ce.library_paths()[0]
+    return (["g++", "-O2", "-std=c++17", "-fPIC", "-shared", "-D__HIP_PLATFORM_AMD__=1", "-DUSE_ROCM=1",
+             "-DTORCH_EXTENSION_NAME=ur3e_policy_torch",
+             f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}"]
+            + [f"-I{p}" for p in ce.include_paths()] + [f"-I{sysconfig.get_paths()['include']}", "-I/opt/rocm/include"]
+            + ["-MD", "-MF", os.path.join(OBJ, "ur3e_policy_torch.d"), SRC_PL_TORCH, "-o", TORCH_LIB,
+               f"-L{os.path.dirname(LIB)}", "-lur3e_amd", "-Wl,-rpath,$ORIGIN", f"-L{lib}", "-ltorch_python", "-ltorch",
+               "-ltorch_cpu", "-ltorch_hip", "-lc10", "-lc10_hip"])
+
+
+def _build_torch(force, verbose):
+    deps = _depfile_deps(os.path.join(OBJ, "ur3e_policy_torch.d"))
+    if force or _newer(TORCH_LIB, [SRC_PL_TORCH] + (deps if deps is not None else HEADERS)):
+        cmd = _torch_cmd()
+        if verbose:
+            print(" ".join(cmd))
+        t0 = time.time()
+        subprocess.run(cmd, check=True)
+        os.utime(TORCH_LIB, (t0, t0))
+
+
 def build(force: bool = False, verbose: bool = False, trace: bool = False) -> str:
     """Build the product library (and, with trace=True, the trace variant) when a source is newer.
     Objects compile in parallel; a library relinks when one of its objects changed."""
@@ -204,6 +236,7 @@ def build(force: bool = False, verbose: bool = False, trace: bool = False) -> st
             if verbose:
                 print(" ".join(cmd))
             subprocess.run(cmd, check=True)
+    _build_torch(force, verbose)
     return LIB
 
 
