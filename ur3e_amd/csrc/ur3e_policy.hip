@@ -107,6 +107,7 @@ struct WalkArgs {
   Walk w[3];
   int nw; /* walks of this launch, all of the same tile shape */
   int b, t, h, kdim, vdim, slabs, nsplit, split_len;
+  int near; /* consecutive workgroups that share a sequence's tensors */
   int chunk;     /* 16, or 1 where tokens lie too far apart for 30-bit offsets inside a chunk */
   int state_vec; /* states may be moved KT or VT floats at a time */
   const float* log_decay;
@@ -252,12 +253,14 @@ template <int VT, bool VEC> __device__ __forceinline__ u2 pack_col(const Raw<Bf1
 
 /* KT, VT: tiles of 16 key channels and of 16 value channels per wave.  STATE: only the state at the end of
    each split (from zero), for sequences that several waves share. */
-template <class T, int KT, int VT, bool VEC, bool STATE>
-__global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
+template <class T, int KT, int VT, bool VEC, bool STATE, bool PREFETCH>
+__global__ __launch_bounds__(256, PREFETCH && (sizeof(T) == 4 || KT == 8) ? 1 : 2) void k_attn_walk(WalkArgs a) {
   constexpr int ES = (int)sizeof(T);
   const int lane = threadIdx.x & 63, idx = lane & 15, g = lane >> 4;
-  /* the wave's task in scalar registers, and with it every address base and loop bound */
-  const unsigned task = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  /* Workgroups go round the 8 XCDs in turn; the `near` of them that share a sequence's tensors and states stay on
+     one, behind its L2.  The wave's task is in scalar registers, and with it every address base and loop bound. */
+  const unsigned slot = blockIdx.x >> 3, group = (slot / a.near * 8 + (blockIdx.x & 7)) * a.near + slot % a.near;
+  const unsigned task = group * (blockDim.x >> 6) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
   const int nsp = STATE ? a.nsplit - 1 : a.nsplit;
   unsigned r = task;
   const int slab = (int)(r % a.slabs); r /= a.slabs;
@@ -297,12 +300,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   }
   const unsigned kidx = at(KT * idx * ES, KT * idx < kdim, FAR_D), vidx = at(VT * idx * ES, VT * idx < vleft, FAR_D);
   /* ... and of its tokens, for chunks of n: the lowest token of the chunk is the base */
-  unsigned qrow, krow, orow, kcol[4], vcol[4];
+  unsigned qrow, krow, kcol[4], vcol[4];
   auto place = [&](int n) {
     const unsigned back = n - 1 - idx, rel = rev ? back : idx;
     qrow = at(rel * (unsigned)qst, idx < n, FAR_T);
     krow = at(rel * (unsigned)kst, idx < n, FAR_T);
-    orow = at(rel * (unsigned)ost, idx < n, FAR_T);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const int j = 4 * g + e;
@@ -311,8 +313,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       vcol[e] = at(rc * (unsigned)vst, j < n, FAR_T) + vidx;
     }
   };
-  auto put = [&](int n, long long low, const float (&o)[4][VT]) {
+  auto put = [&](unsigned rel, int n, long long low, const float (&o)[4][VT]) {
     const Rsrc ro = rsrc_of(out + low * ost);
+    const unsigned orow = at(rel * (unsigned)ost, idx < n, FAR_T);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const unsigned off = orow + od[e];
@@ -327,8 +330,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
     const float zero[4][VT] = {};
     for (int t = len > lo ? len : lo; t < end; t += chunk) {
       const int n = end - t < chunk ? end - t : chunk;
-      orow = at(idx * (unsigned)ost, idx < n, FAR_T);
-      put(n, t, zero);
+      put(idx, n, t, zero);
     }
   }
 
@@ -395,13 +397,49 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 
   float through = 1.0f; /* STATE: what the split multiplies an entering state by */
   int single = 0;       /* tokens left to take one by one */
-  int placed = 0;
-  for (int p = lo; p < hi;) {
-    int n = hi - p < chunk ? hi - p : chunk;
-    if (single) n = 1;
+  int placed = 0, scaled = 0; /* the chunk sizes that the offsets and the factors stand for */
+  struct Chunk {
+    Raw<T, KT, VEC> kr[4], qr[4], kc[4];
+    Raw<T, VT, VEC> vc[4];
+    unsigned start;
+  };
+  auto load = [&](Chunk& c, int p, int n) {
     if (n != placed) {
       placed = n;
       place(n);
+    }
+    const long long low = rev ? len - p - n : p;
+    const Rsrc rk = rsrc_of(k + low * kst), rv = rsrc_of(v + low * vst);
+    if (!STATE) {
+      const Rsrc rq = rsrc_of(q + low * qst);
+#pragma unroll
+      for (int e = 0; e < 4; e++) {
+        const int left = kdim - KT * (4 * g + e);
+        c.kr[e].load(rk, krow + kd[e], left);
+        c.qr[e].load(rq, qrow + kd[e], left);
+      }
+    }
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      c.vc[e].load(rv, vcol[e], vleft - VT * idx);
+      c.kc[e].load(rk, kcol[e], kdim - KT * idx);
+    }
+    c.start = 0;
+    if (starts) {
+      /* position x of a reversed walk is token len - 1 - x, behind the start that token len - x may carry */
+      const Rsrc rs = rsrc_of(starts + (rev ? low + 1 : low) * starts_st);
+      const bool there = (idx < n) & ((p + idx != 0) | !rev);
+      const unsigned back = n - 1 - idx, rel = rev ? back : idx;
+      c.start = __builtin_amdgcn_raw_buffer_load_b8(rs, at(rel * (unsigned)starts_st, there, FAR_T), 0, 0);
+    }
+  };
+  auto size = [&](int p) { return single ? 1 : hi - p < chunk ? hi - p : chunk; };
+
+  int p = lo, n = 0;
+  /* one chunk; false: it holds a value that is not finite and has to be taken token by token */
+  auto work = [&](const Chunk& c) {
+    if (n != scaled) {
+      scaled = n;
       gn = pw(l, n);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
@@ -410,40 +448,17 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       }
     }
     const long long low = rev ? len - p - n : p;
-    const Rsrc rk = rsrc_of(k + low * kst), rv = rsrc_of(v + low * vst);
-    Raw<T, KT, VEC> kr[4], qr[4], kc[4];
-    Raw<T, VT, VEC> vc[4];
-    if (!STATE) {
-      const Rsrc rq = rsrc_of(q + low * qst);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int left = kdim - KT * (4 * g + e);
-        kr[e].load(rk, krow + kd[e], left);
-        qr[e].load(rq, qrow + kd[e], left);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      vc[e].load(rv, vcol[e], vleft - VT * idx);
-      kc[e].load(rk, kcol[e], kdim - KT * idx);
-    }
+    const auto &kr = c.kr, &qr = c.qr, &kc = c.kc;
+    const auto& vc = c.vc;
     /* bit i: an episode starts between positions i - 1 and i */
-    unsigned brk = 0;
-    if (starts) {
-      /* position x of a reversed walk is token len - 1 - x, behind the start that token len - x may carry */
-      const Rsrc rs = rsrc_of(starts + (rev ? low + 1 : low) * starts_st);
-      const bool there = (idx < n) & ((p + idx != 0) | !rev);
-      const unsigned back = n - 1 - idx, rel = rev ? back : idx;
-      const unsigned f = __builtin_amdgcn_raw_buffer_load_b8(rs, at(rel * (unsigned)starts_st, there, FAR_T), 0, 0);
-      brk = (unsigned)(__ballot(f != 0) & 0xffffu);
-    }
+    const unsigned brk = starts ? (unsigned)(__ballot(c.start != 0) & 0xffffu) : 0u;
 
     /* a value that is not finite must not meet the zeros of the mask (0 * inf): its chunk is taken token by
        token, where every product belongs to the token */
     unsigned bad = 0;
 #pragma unroll
     for (int e = 0; e < 4; e++) bad |= not_finite(vc[e]);
-    if (n > 1 && __any(bad != 0)) { single = n; continue; }
+    if (n > 1 && __any(bad != 0)) return false;
 
     const unsigned upto = (2u << idx) - 1u; /* breaks at or in front of this lane's position */
     const bool from_state = (brk & upto) == 0, keep = brk == 0;
@@ -512,7 +527,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; e++) o[e][nt] = x[e];
         }
-        put(n, low, o);
+        put(rev ? n - 1 - idx : idx, n, low, o);
       }
       decay();
 #pragma unroll
@@ -547,7 +562,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; e++) o[e][nt] = x[e];
         }
-        put(n, low, o);
+        put(rev ? n - 1 - idx : idx, n, low, o);
       }
       decay();
 #pragma unroll
@@ -560,8 +575,44 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         }
     }
     if (STATE) through = keep ? through * gn : 0.0f;
-    p += n;
-    if (single) single--;
+    return true;
+  };
+  if constexpr (PREFETCH) {
+    /* the chunk behind is on its way while one is worked on */
+    Chunk c;
+    bool here = false;
+    while (p < hi) {
+      if (!here) {
+        n = size(p);
+        load(c, p, n);
+      }
+      Chunk next;
+      const bool more = p + n < hi && !single;
+      const int n_next = more ? size(p + n) : 0;
+      if (more) load(next, p + n, n_next);
+      if (!work(c)) {
+        single = n;
+        here = false;
+        continue;
+      }
+      p += n;
+      if (single) single--;
+      here = more;
+      n = n_next;
+      c = next;
+    }
+  } else {
+    while (p < hi) {
+      Chunk c;
+      n = size(p);
+      load(c, p, n);
+      if (!work(c)) {
+        single = n;
+        continue;
+      }
+      p += n;
+      if (single) single--;
+    }
   }
 
   float* s_out = nullptr;
@@ -614,57 +665,67 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 }
 
 /* States that enter each split: ws[s] holds split s - 1's own sum (k_attn_walk, STATE) and becomes
-   X_s = wf[s] X_{s-1} + ws[s], X_0 = s_in.  A thread owns VW elements and runs along the splits, whose sums it
-   loads JOIN at a time (nothing but the chain of multiply-adds depends on the split in front). */
-#define JOIN 16
-template <int VW> __global__ __launch_bounds__(64) void k_attn_join(WalkArgs a) {
+   X_s = wf[s] X_{s-1} + ws[s], X_0 = s_in.  A thread owns one element and runs along the splits; nothing but
+   the chain of multiply-adds depends on the split in front, so the sums of JOIN splits are loaded at a time, the
+   next ones while one lot is chained. */
+#define JOIN 32
+__global__ __launch_bounds__(64) void k_attn_join(WalkArgs a) {
   const Walk w = a.w[blockIdx.z];
   const long long bh = blockIdx.y;
   const int elems = a.kdim * a.vdim, nsplit = a.nsplit;
-  const int e = (blockIdx.x * 64 + threadIdx.x) * VW;
+  const int e = blockIdx.x * 64 + threadIdx.x;
   if (e >= elems) return;
-  struct alignas(4 * VW) Pack { float x[VW]; };
   float* ws = w.ws + bh * nsplit * elems + e;
   const float* wf = w.wf + bh * nsplit;
-  Pack x = {};
-  if (w.s_in) x = *reinterpret_cast<const Pack*>(w.s_in + bh * elems + e);
-  for (int s0 = 0; s0 < nsplit; s0 += JOIN) {
-    Pack u[JOIN];
-    float f[JOIN];
+  struct Lot { float u[JOIN], f[JOIN]; };
+  auto load = [&](Lot& l, int s0) {
 #pragma unroll
     for (int i = 0; i < JOIN; i++) {
       const int s = s0 + 1 + i < nsplit ? s0 + 1 + i : nsplit - 1;
-      u[i] = *reinterpret_cast<const Pack*>(ws + (long long)s * elems);
-      f[i] = wf[s];
+      l.u[i] = ws[(long long)s * elems];
+      l.f[i] = wf[s];
     }
+  };
+  Lot l;
+  load(l, 0);
+  float x = w.s_in ? w.s_in[bh * elems + e] : 0.0f;
+  for (int s0 = 0; s0 < nsplit; s0 += JOIN) {
+    Lot next;
+    if (s0 + JOIN < nsplit) load(next, s0 + JOIN);
 #pragma unroll
     for (int i = 0; i < JOIN; i++) {
-      if (s0 + i < nsplit) *reinterpret_cast<Pack*>(ws + (long long)(s0 + i) * elems) = x;
-#pragma unroll
-      for (int c = 0; c < VW; c++) {
-        const float y = f[i] * x.x[c];
-        x.x[c] = (f[i] == 0.0f ? 0.0f : y) + u[i].x[c];
-      }
+      if (s0 + i < nsplit) ws[(long long)(s0 + i) * elems] = x;
+      const float y = l.f[i] * x;
+      x = (l.f[i] == 0.0f ? 0.0f : y) + l.u[i];
     }
+    l = next;
   }
 }
 
-/* sums of the per-query-head gradients over the heads that share a key / value head */
-template <class T>
-__global__ __launch_bounds__(256) void k_attn_group_sum(const float* __restrict__ src, T* __restrict__ dst, int b, int t,
-                                                        int h, int hk, int d, long long sb, long long st, long long sh) {
-  const long long n = (long long)b * t * hk * d;
-  for (long long i = (long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (long long)gridDim.x * 256) {
-    const int c = (int)(i % d);
-    long long r = i / d;
-    const int kh = (int)(r % hk); r /= hk;
-    const int tt = (int)(r % t);
-    const int bb = (int)(r / t);
-    const int grp = h / hk;
-    const float* s = src + (((long long)bb * t + tt) * h + kh * grp) * d + c;
-    float x = 0.0f;
-    for (int k = 0; k < grp; k++) x += s[(long long)k * d];
-    dst[bb * sb + tt * st + kh * sh + c] = from_f<T>(x);
+/* sums of the per-query-head gradients over the heads that share a key / value head: [b][t][h][d] floats to
+   [b][t][hk][d], VW channels a thread */
+template <class T, int VW>
+__global__ __launch_bounds__(256) void k_attn_group_sum(const float* __restrict__ src, T* __restrict__ dst, unsigned t,
+                                                        unsigned hk, unsigned grp, unsigned groups, unsigned n, long long sb,
+                                                        long long st, long long sh) {
+  struct alignas(4 * VW) Pack { float x[VW]; };
+  for (unsigned long long i0 = (unsigned long long)blockIdx.x * 256; i0 < n; i0 += (unsigned long long)gridDim.x * 256) {
+    const unsigned i = (unsigned)i0 + threadIdx.x;
+    if (i >= n) return;
+    unsigned r = i / groups;
+    const unsigned c = (i - r * groups) * VW, kh = r % hk;
+    r /= hk;
+    const unsigned tt = r % t, bb = r / t;
+    const float* s = src + ((long long)r * hk + kh) * grp * (groups * VW) + c;
+    float x[VW] = {};
+    for (unsigned k = 0; k < grp; k++) {
+      const Pack y = *reinterpret_cast<const Pack*>(s + (long long)k * groups * VW);
+#pragma unroll
+      for (int e = 0; e < VW; e++) x[e] += y.x[e];
+    }
+    T* o = dst + bb * sb + tt * st + kh * sh + c;
+#pragma unroll
+    for (int e = 0; e < VW; e++) o[e] = from_f<T>(x[e]);
   }
 }
 
@@ -816,36 +877,48 @@ static int attn_check(const ur3e_attn_t* a) {
 
 static int pow2_tiles(int d) { return d <= 16 ? 1 : d <= 32 ? 2 : d <= 64 ? 4 : 8; }
 
-struct Plan {
-  int kt, vt, slabs, nsplit, split_len;
+struct Tiles {
+  int kt, vt, slabs;
 };
-
-/* Tiles: the state of a wave is kdim x 16 vt floats, at most 64 registers a lane, so vt is at most 2 at 128 key
-   channels.  Splits: ~2 waves a SIMD (2,048) fill the card. */
-static Plan plan_of(int b, int t, int h, int kdim, int vdim, int walks) {
-  Plan p;
+/* the state of a wave is kdim x 16 vt floats, at most 64 registers a lane, so vt is at most 2 at 128 key channels */
+static Tiles tiles_of(int kdim, int vdim) {
+  Tiles p;
   p.kt = pow2_tiles(kdim);
   p.vt = pow2_tiles(vdim);
   const int most = p.kt == 8 ? 2 : 4;
   if (p.vt > most) p.vt = most;
   p.slabs = (vdim + 16 * p.vt - 1) / (16 * p.vt);
-  const long long waves = (long long)b * h * p.slabs * walks;
-  p.nsplit = 1;
-  p.split_len = t > 0 ? t : 1;
-  if (waves < 1024 && t >= 256) {
-    long long want = (2048 + waves - 1) / (waves > 0 ? waves : 1);
-    long long most_splits = t / 128;
-    if (want > most_splits) want = most_splits;
-    if (want > 1) {
-      p.split_len = (int)(((t + want - 1) / want + 15) / 16 * 16);
-      p.nsplit = (t + p.split_len - 1) / p.split_len;
-    }
+  return p;
+}
+
+struct Splits {
+  int n, len;
+};
+/* How many waves share a sequence.  ~2 waves a SIMD (2,048) fill the card; a split costs a chain of 16-token
+   chunks, and its state one more link of the chain of the join, so the shortest worth having grows with the
+   square root of the length. */
+static Splits splits_of(const ur3e_attn_t* a, int walks) {
+  const long long waves = (long long)a->b * a->heads * tiles_of(a->dk, a->dv).slabs * walks;
+  Splits p = {1, a->t > 0 ? a->t : 1};
+  if (waves < 1024 && a->t >= 64) {
+    const long long want = (2048 + waves - 1) / waves;
+    int least = 32;
+    while ((long long)least * least * 4 < a->t) least += 16;
+    const int len = (int)(((a->t + want - 1) / want + 15) / 16 * 16);
+    p.len = len > least ? len : least;
+    p.n = (a->t + p.len - 1) / p.len;
   }
   return p;
 }
 
-static size_t walk_bytes(const Plan& p, long long b, int h, int kdim, int vdim) {
-  return p.nsplit > 1 ? (size_t)b * h * p.nsplit * (kdim * vdim + 1) * sizeof(float) : 0;
+/* the states that enter the splits, and the factors between them */
+static size_t split_bytes(const ur3e_attn_t* a, const Splits& p) {
+  return p.n > 1 ? (size_t)a->b * a->heads * p.n * (a->dk * a->dv + 1) * sizeof(float) : 0;
+}
+static void split_use(const ur3e_attn_t* a, const Splits& p, void* ws, Walk& w) {
+  if (p.n < 2) return;
+  w.ws = (float*)ws;
+  w.wf = w.ws + (long long)a->b * a->heads * p.n * a->dk * a->dv;
 }
 
 /* groups of kt channels can be moved whole: all there or none, on their boundary */
@@ -854,23 +927,31 @@ static bool aligned(const Tok& t, int e, int kt, int d) {
   return d % kt == 0 && (uintptr_t)t.p % by == 0 && t.sb * e % by == 0 && t.st * e % by == 0 && t.sh * e % by == 0;
 }
 
-template <class T, int KT, int VT, bool VEC> static int walk_launch(const WalkArgs& a, hipStream_t s) {
+/* what a launch does: the states at the ends of the splits and their join, or the outputs */
+enum Phase { STATES, OUTPUTS };
+
+template <class T, int KT, int VT, bool VEC> static int walk_launch(WalkArgs& a, Phase phase, hipStream_t s) {
   const long long streams = (long long)a.b * a.h * a.nw * a.slabs;
-  if (a.nsplit > 1) {
-    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, true>), dim3((unsigned)((streams * (a.nsplit - 1) + 3) / 4)), dim3(256), 0, s, a);
+  /* the waves that share a sequence's tensors in one workgroup, where they are at most four */
+  const int share = a.nw * a.slabs, waves = share <= 4 ? share : 4;
+  a.near = (share + waves - 1) / waves;
+  const long long tasks = streams * (phase == STATES ? a.nsplit - 1 : a.nsplit), per = 8LL * a.near * waves;
+  const dim3 grid((unsigned)((tasks + per - 1) / per * 8 * a.near)), block(64 * waves);
+  if (phase == STATES) {
+    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, true, true>), grid, block, 0, s, a);
     PL_CHK(hipGetLastError());
-    const int elems = a.kdim * a.vdim;
-    if (elems % 4 == 0 && a.state_vec)
-      hipLaunchKernelGGL((k_attn_join<4>), dim3((elems + 255) / 256, (unsigned)(a.b * a.h), (unsigned)a.nw), dim3(64), 0, s, a);
-    else
-      hipLaunchKernelGGL((k_attn_join<1>), dim3((elems + 63) / 64, (unsigned)(a.b * a.h), (unsigned)a.nw), dim3(64), 0, s, a);
-    PL_CHK(hipGetLastError());
+    hipLaunchKernelGGL(k_attn_join, dim3((a.kdim * a.vdim + 63) / 64, (unsigned)(a.b * a.h), (unsigned)a.nw), dim3(64), 0, s, a);
+  } else if (a.nsplit > 1 || (sizeof(T) == 2 && KT < 8 && a.t > 16)) {
+    /* the next chunk's loads run ahead where a wave has a SIMD to itself (split sequences) or the registers for two
+       chunks leave room for two waves; else the second wave hides them */
+    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false, true>), grid, block, 0, s, a);
+  } else {
+    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false, false>), grid, block, 0, s, a);
   }
-  hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false>), dim3((unsigned)((streams * a.nsplit + 3) / 4)), dim3(256), 0, s, a);
   PL_CHK(hipGetLastError());
   return UR3E_OK;
 }
-template <class T, int KT, int VT> static int walk_vec(WalkArgs& a, hipStream_t s) {
+template <class T, int KT, int VT> static int walk_vec(WalkArgs& a, Phase phase, hipStream_t s) {
   bool vec = true;
   a.state_vec = 1;
   a.chunk = 16;
@@ -882,53 +963,53 @@ template <class T, int KT, int VT> static int walk_vec(WalkArgs& a, hipStream_t 
     if (w.q.st > far || w.k.st > far || w.v.st > far || w.o.st > far) a.chunk = 1;
     if ((w.state_t ? a.kdim % KT : a.vdim % VT) || (uintptr_t)w.s_in % 16 || (uintptr_t)w.s_out % 16 || (uintptr_t)w.ws % 16)
       a.state_vec = 0;
-    a.w[i].wf = w.ws ? w.ws + (long long)a.b * a.h * a.nsplit * a.kdim * a.vdim : nullptr;
+    vec = vec && aligned(w.k, sizeof(T), KT, a.kdim) && aligned(w.v, sizeof(T), VT, a.vdim);
+    if (phase == OUTPUTS)
+      vec = vec && aligned(w.q, sizeof(T), KT, a.kdim) && aligned(w.o, w.out_f32 ? 4 : (int)sizeof(T), VT, a.vdim);
   }
-  for (int i = 0; i < a.nw; i++)
-    vec = vec && aligned(a.w[i].q, sizeof(T), KT, a.kdim) && aligned(a.w[i].k, sizeof(T), KT, a.kdim) &&
-          aligned(a.w[i].v, sizeof(T), VT, a.vdim) && aligned(a.w[i].o, a.w[i].out_f32 ? 4 : (int)sizeof(T), VT, a.vdim);
-  return vec ? walk_launch<T, KT, VT, true>(a, s) : walk_launch<T, KT, VT, false>(a, s);
+  return vec ? walk_launch<T, KT, VT, true>(a, phase, s) : walk_launch<T, KT, VT, false>(a, phase, s);
 }
-template <class T, int KT> static int walk_vt(WalkArgs& a, int vt, hipStream_t s) {
-  if (vt == 1) return walk_vec<T, KT, 1>(a, s);
-  if (vt == 2) return walk_vec<T, KT, 2>(a, s);
-  if constexpr (KT < 8) return walk_vec<T, KT, 4>(a, s);
-  return ur3e_internal_fail(UR3E_EINVAL, "attention: no such tile");
+template <class T, int KT> static int walk_vt(WalkArgs& a, int vt, Phase phase, hipStream_t s) {
+  if (vt == 1) return walk_vec<T, KT, 1>(a, phase, s);
+  if (vt == 2) return walk_vec<T, KT, 2>(a, phase, s);
+  if constexpr (KT < 8) return walk_vec<T, KT, 4>(a, phase, s);
+  return bad_arg("attention: no such tile");
 }
-template <class T> static int walk_kt(WalkArgs& a, const Plan& p, hipStream_t s) {
+template <class T> static int walk_kt(WalkArgs& a, const Tiles& p, Phase phase, hipStream_t s) {
   switch (p.kt) {
-    case 1: return walk_vt<T, 1>(a, p.vt, s);
-    case 2: return walk_vt<T, 2>(a, p.vt, s);
-    case 4: return walk_vt<T, 4>(a, p.vt, s);
-    default: return walk_vt<T, 8>(a, p.vt, s);
+    case 1: return walk_vt<T, 1>(a, p.vt, phase, s);
+    case 2: return walk_vt<T, 2>(a, p.vt, phase, s);
+    case 4: return walk_vt<T, 4>(a, p.vt, phase, s);
+    default: return walk_vt<T, 8>(a, p.vt, phase, s);
   }
 }
-static int walk_run(int dtype, WalkArgs& a, const Plan& p, hipStream_t s) {
-  if (dtype == UR3E_F32) return walk_kt<float>(a, p, s);
-  if (dtype == UR3E_BF16) return walk_kt<Bf16>(a, p, s);
-  return walk_kt<F16>(a, p, s);
+static int walk_run(int dtype, WalkArgs& a, Phase phase, hipStream_t s) {
+  const Tiles p = tiles_of(a.kdim, a.vdim);
+  a.slabs = p.slabs;
+  if (dtype == UR3E_F32) return walk_kt<float>(a, p, phase, s);
+  if (dtype == UR3E_BF16) return walk_kt<Bf16>(a, p, phase, s);
+  return walk_kt<F16>(a, p, phase, s);
 }
 
 static Tok tok_of(const ur3e_tokens_t& x, int hdiv) { return Tok{x.p, x.sb, x.st, x.sh, hdiv}; }
 
-static WalkArgs args_of(const ur3e_attn_t* a, int kdim, int vdim, const Plan& p) {
+static WalkArgs args_of(const ur3e_attn_t* a, int kdim, int vdim, const Splits& p) {
   WalkArgs w = {};
   w.b = a->b; w.t = a->t; w.h = a->heads; w.kdim = kdim; w.vdim = vdim;
-  w.slabs = p.slabs; w.nsplit = p.nsplit; w.split_len = p.split_len;
+  w.nsplit = p.n; w.split_len = p.len;
   w.log_decay = a->log_decay;
   w.starts = a->starts; w.starts_sb = a->starts_sb; w.starts_st = a->starts_st;
   w.lengths = a->lengths;
   return w;
 }
 
-static size_t up16(size_t x) { return (x + 255) / 256 * 256; }
+static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 static size_t attn_bytes(const ur3e_attn_t* a, int backward) {
-  if (!backward) return walk_bytes(plan_of(a->b, a->t, a->heads, a->dk, a->dv, 1), a->b, a->heads, a->dk, a->dv);
-  const int same = pow2_tiles(a->dk) == pow2_tiles(a->dv) && a->dk == a->dv;
-  const Plan p1 = plan_of(a->b, a->t, a->heads, a->dv, a->dk, same ? 3 : 2), p2 = same ? p1 : plan_of(a->b, a->t, a->heads, a->dk, a->dv, 1);
-  size_t n = 2 * up16(walk_bytes(p1, a->b, a->heads, a->dv, a->dk)) + up16(walk_bytes(p2, a->b, a->heads, a->dk, a->dv));
-  if (a->heads != a->kv_heads) n += up16((size_t)a->b * a->t * a->heads * a->dk * 4) + up16((size_t)a->b * a->t * a->heads * a->dv * 4);
+  if (a->b == 0) return 0;
+  if (!backward) return split_bytes(a, splits_of(a, 1));
+  size_t n = 2 * up256(split_bytes(a, splits_of(a, 3)));
+  if (a->heads != a->kv_heads) n += up256((size_t)a->b * a->t * a->heads * a->dk * 4) + up256((size_t)a->b * a->t * a->heads * a->dv * 4);
   return n;
 }
 
@@ -948,15 +1029,31 @@ extern "C" int ur3e_attn_forward(const ur3e_attn_t* a, const ur3e_tokens_t* out,
   if (!out || (a->t > 0 && !out->p)) return bad_arg("attention: null out");
   if (out->st < 0) return bad_arg("attention: token strides must not be negative");
   if (workspace_bytes < attn_bytes(a, 0) || (attn_bytes(a, 0) && !workspace)) return bad_arg("attention: workspace too small");
-  const Plan p = plan_of(a->b, a->t, a->heads, a->dk, a->dv, 1);
+  const Splits p = splits_of(a, 1);
   WalkArgs w = args_of(a, a->dk, a->dv, p);
   const int grp = a->heads / a->kv_heads;
   w.nw = 1;
   Walk& f = w.w[0];
   f.q = tok_of(a->q, 1); f.k = tok_of(a->k, grp); f.v = tok_of(a->v, grp); f.o = tok_of(*out, 1);
-  f.s_in = a->s0; f.s_out = s_out; f.ws = (float*)workspace;
+  f.s_in = a->s0; f.s_out = s_out;
   f.in_scale = f.p_scale = a->scale; f.w_scale = 1.0f;
-  return walk_run(a->dtype, w, p, (hipStream_t)stream);
+  split_use(a, p, workspace, f);
+  if (p.n > 1) {
+    rc = walk_run(a->dtype, w, STATES, (hipStream_t)stream);
+    if (rc) return rc;
+  }
+  return walk_run(a->dtype, w, OUTPUTS, (hipStream_t)stream);
+}
+
+template <class T> static void group_sum(const ur3e_attn_t* a, const float* src, const ur3e_tokens_t& d, int c, hipStream_t s) {
+  const int vw = c % 4 == 0 ? 4 : 1;
+  const long long n = (long long)a->b * a->t * a->kv_heads * (c / vw), blocks = (n + 255) / 256;
+  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
+  const unsigned grp = a->heads / a->kv_heads;
+  if (vw == 4)
+    hipLaunchKernelGGL((k_attn_group_sum<T, 4>), grid, dim3(256), 0, s, src, (T*)d.p, (unsigned)a->t, (unsigned)a->kv_heads, grp, (unsigned)(c / 4), (unsigned)n, d.sb, d.st, d.sh);
+  else
+    hipLaunchKernelGGL((k_attn_group_sum<T, 1>), grid, dim3(256), 0, s, src, (T*)d.p, (unsigned)a->t, (unsigned)a->kv_heads, grp, (unsigned)c, (unsigned)n, d.sb, d.st, d.sh);
 }
 
 extern "C" int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dout, const float* ds_out,
@@ -966,62 +1063,71 @@ extern "C" int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dou
   if (rc) return rc;
   if (a->b == 0) return UR3E_OK;
   if (!dout || !dq || !dk || !dv) return bad_arg("attention: null gradient");
+  if (a->heads != a->kv_heads && (long long)a->b * a->t * a->kv_heads * (a->dk > a->dv ? a->dk : a->dv) > 0xffffff00LL)
+    return bad_arg("attention: too many tokens for shared heads");
   if (a->t > 0 && (!dout->p || !dq->p || !dk->p || !dv->p)) return bad_arg("attention: null gradient");
   if (dout->st < 0 || dq->st < 0 || dk->st < 0 || dv->st < 0) return bad_arg("attention: token strides must not be negative");
   if (workspace_bytes < attn_bytes(a, 1) || (attn_bytes(a, 1) && !workspace)) return bad_arg("attention: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   const int grp = a->heads / a->kv_heads;
-  const bool same = a->dk == a->dv;
-  const Plan p1 = plan_of(a->b, a->t, a->heads, a->dv, a->dk, same ? 3 : 2), p2 = same ? p1 : plan_of(a->b, a->t, a->heads, a->dk, a->dv, 1);
+  const Splits p = splits_of(a, 3);
   char* ws = (char*)workspace;
-  const size_t n1 = up16(walk_bytes(p1, a->b, a->heads, a->dv, a->dk)), n2 = up16(walk_bytes(p2, a->b, a->heads, a->dk, a->dv));
+  const size_t n = up256(split_bytes(a, p));
   float *fk = nullptr, *fv = nullptr;
   if (grp > 1) {
-    fk = (float*)(ws + 2 * n1 + n2);
-    fv = (float*)(ws + 2 * n1 + n2 + up16((size_t)a->b * a->t * a->heads * a->dk * 4));
+    fk = (float*)(ws + 2 * n);
+    fv = (float*)(ws + 2 * n + up256((size_t)a->b * a->t * a->heads * a->dk * 4));
   }
   const Tok tq = tok_of(a->q, 1), tk = tok_of(a->k, grp), tv = tok_of(a->v, grp), tdo = tok_of(*dout, 1);
-  auto wide = [&](const float* p, int d) { return Tok{p, (long long)a->t * a->heads * d, (long long)a->heads * d, d, 1}; };
-  Walk q = {}, k = {}, v = {};
+  auto wide = [&](const float* x, int d) { return Tok{x, (long long)a->t * a->heads * d, (long long)a->heads * d, d, 1}; };
+  Walk f = {}, q = {}, k = {}, v = {};
   /* dq = walk(do, v, k) on S^T */
   q.q = tdo; q.k = tv; q.v = tk; q.o = tok_of(*dq, 1);
   q.state_t = 1;
-  q.s_in = a->s0; q.ws = (float*)ws;
+  q.s_in = a->s0;
   q.in_scale = q.p_scale = a->scale; q.w_scale = 1.0f;
-  /* dk = reversed walk(v, do, q) on G^T */
-  k.q = tv; k.k = tdo; k.v = tq; k.o = grp > 1 ? wide(fk, a->dk) : tok_of(*dk, 1);
-  k.out_f32 = grp > 1;
-  k.state_t = 1;
-  k.s_in = ds_out; k.ws = (float*)(ws + n1);
-  k.reversed = 1;
-  k.in_scale = 1.0f; k.p_scale = k.w_scale = a->scale;
+  split_use(a, p, ws, q);
   /* dv = reversed walk(k, q, do) on G */
   v.q = tk; v.k = tq; v.v = tdo; v.o = grp > 1 ? wide(fv, a->dv) : tok_of(*dv, 1);
   v.out_f32 = grp > 1;
-  v.s_in = ds_out; v.s_out = ds0; v.ws = (float*)(ws + 2 * n1);
+  v.s_in = ds_out; v.s_out = ds0;
   v.reversed = 1;
   v.in_scale = 1.0f; v.p_scale = v.w_scale = a->scale;
-  WalkArgs w = args_of(a, a->dv, a->dk, p1);
-  w.w[0] = q; w.w[1] = k;
-  w.nw = 2;
-  if (same) { w.w[2] = v; w.nw = 3; }
-  rc = walk_run(a->dtype, w, p1, s);
+  split_use(a, p, ws + n, v);
+  /* dk = reversed walk(v, do, q) on G^T */
+  k = v;
+  k.q = tv; k.k = tdo; k.v = tq; k.o = grp > 1 ? wide(fk, a->dk) : tok_of(*dk, 1);
+  k.state_t = 1;
+  k.s_out = nullptr;
+  if (p.n > 1) {
+    /* the states of the splits: S of the forward walk, and G, which dk and dv share */
+    f.k = tk; f.v = tv;
+    f.s_in = a->s0;
+    f.w_scale = 1.0f;
+    split_use(a, p, ws, f);
+    WalkArgs w = args_of(a, a->dk, a->dv, p);
+    w.w[0] = f; w.w[1] = v;
+    w.nw = 2;
+    rc = walk_run(a->dtype, w, STATES, s);
+    if (rc) return rc;
+  }
+  WalkArgs w = args_of(a, a->dv, a->dk, p);
+  w.w[0] = q; w.w[1] = k; w.w[2] = v;
+  w.nw = a->dk == a->dv ? 3 : 2;
+  rc = walk_run(a->dtype, w, OUTPUTS, s);
   if (rc) return rc;
-  if (!same) {
-    WalkArgs x = args_of(a, a->dk, a->dv, p2);
+  if (w.nw == 2) {
+    WalkArgs x = args_of(a, a->dk, a->dv, p);
     x.w[0] = v;
     x.nw = 1;
-    rc = walk_run(a->dtype, x, p2, s);
+    rc = walk_run(a->dtype, x, OUTPUTS, s);
     if (rc) return rc;
   }
   if (grp > 1 && a->t > 0) {
-    const long long m = (long long)a->b * a->t * a->kv_heads;
     auto sum = [&](const float* src, const ur3e_tokens_t& d, int c) {
-      const long long blocks = (m * c + 255) / 256;
-      const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
-      if (a->dtype == UR3E_F32) hipLaunchKernelGGL(k_attn_group_sum<float>, grid, dim3(256), 0, s, src, (float*)d.p, a->b, a->t, a->heads, a->kv_heads, c, d.sb, d.st, d.sh);
-      else if (a->dtype == UR3E_BF16) hipLaunchKernelGGL(k_attn_group_sum<Bf16>, grid, dim3(256), 0, s, src, (Bf16*)d.p, a->b, a->t, a->heads, a->kv_heads, c, d.sb, d.st, d.sh);
-      else hipLaunchKernelGGL(k_attn_group_sum<F16>, grid, dim3(256), 0, s, src, (F16*)d.p, a->b, a->t, a->heads, a->kv_heads, c, d.sb, d.st, d.sh);
+      if (a->dtype == UR3E_F32) group_sum<float>(a, src, d, c, s);
+      else if (a->dtype == UR3E_BF16) group_sum<Bf16>(a, src, d, c, s);
+      else group_sum<F16>(a, src, d, c, s);
       return hipGetLastError();
     };
     PL_CHK(sum(fk, *dk, a->dk));
