@@ -129,8 +129,8 @@ __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_a
 #define FAR_D 0x40000000u
 typedef __amdgpu_buffer_rsrc_t Rsrc;
 __device__ __forceinline__ unsigned at(unsigned off, bool there, unsigned far) { return there ? off : far; }
-__device__ __forceinline__ Rsrc rsrc_of(const void* p) {
-  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, (int)FAR_D, 0x00027000);
+__device__ __forceinline__ Rsrc rsrc_of(const void* p, bool there = true) {
+  return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, there ? (int)FAR_D : 0, 0x00027000);
 }
 
 /* N consecutive elements as dwords; VEC: aligned to min(16, N * sizeof(T)) bytes and all there or none, else
@@ -175,9 +175,13 @@ template <class T, int N, bool VEC> __device__ __forceinline__ void store_n(Rsrc
     constexpr int B = N * (int)sizeof(T);
     unsigned d[(B + 3) / 4] = {};
 #pragma unroll
-    for (int i = 0; i < N; i++) {
+    for (int i = 0; i < N; i += sizeof(T) == 4 ? 1 : 2) {
       if constexpr (sizeof(T) == 4) d[i] = __builtin_bit_cast(unsigned, x[i]);
-      else d[i / 2] |= (unsigned)__builtin_bit_cast(unsigned short, from_f<T>(x[i])) << (16 * (i & 1));
+      else if constexpr (N == 1) d[0] = __builtin_bit_cast(unsigned short, from_f<T>(x[0]));
+      else {
+        struct Two { T a, b; };
+        d[i / 2] = __builtin_bit_cast(unsigned, Two{from_f<T>(x[i]), from_f<T>(x[i + 1])});
+      }
     }
     if constexpr (B == 2) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)d[0], r, off, 0, 0);
     else if constexpr (B == 4) __builtin_amdgcn_raw_buffer_store_b32(d[0], r, off, 0, 0);
@@ -253,9 +257,10 @@ template <int VT, bool VEC> __device__ __forceinline__ u2 pack_col(const Raw<Bf1
 
 /* KT, VT: tiles of 16 key channels and of 16 value channels per wave.  STATE: only the state at the end of
    each split (from zero), for sequences that several waves share. */
-template <class T, int KT, int VT, bool VEC, bool STATE, bool PREFETCH>
-__global__ __launch_bounds__(256, PREFETCH && (sizeof(T) == 4 || KT == 8) ? 1 : 2) void k_attn_walk(WalkArgs a) {
-  constexpr int ES = (int)sizeof(T);
+template <class T, int KT, int VT, bool VEC, bool STATE, int H>
+__global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
+  constexpr int ES = (int)sizeof(T), C = 16 * H;
+  static_assert(H == 1 || __is_same(T, Bf16), "two tiles of tokens: bfloat16 only");
   const int lane = threadIdx.x & 63, idx = lane & 15, g = lane >> 4;
   /* Workgroups go round the 8 XCDs in turn; the `near` of them that share a sequence's tensors and states stay on
      one, behind its L2.  The wave's task is in scalar registers, and with it every address base and loop bound. */
@@ -299,7 +304,7 @@ __global__ __launch_bounds__(256, PREFETCH && (sizeof(T) == 4 || KT == 8) ? 1 : 
     od[e] = at(dv * os, dv < vleft, FAR_D);
   }
   const unsigned kidx = at(KT * idx * ES, KT * idx < kdim, FAR_D), vidx = at(VT * idx * ES, VT * idx < vleft, FAR_D);
-  /* ... and of its tokens, for chunks of n: the lowest token of the chunk is the base */
+  /* ... and of its tokens, for tiles of n: the lowest token of the tile is the base */
   unsigned qrow, krow, kcol[4], vcol[4];
   auto place = [&](int n) {
     const unsigned back = n - 1 - idx, rel = rev ? back : idx;
@@ -313,9 +318,8 @@ __global__ __launch_bounds__(256, PREFETCH && (sizeof(T) == 4 || KT == 8) ? 1 : 
       vcol[e] = at(rc * (unsigned)vst, j < n, FAR_T) + vidx;
     }
   };
-  auto put = [&](unsigned rel, int n, long long low, const float (&o)[4][VT]) {
-    const Rsrc ro = rsrc_of(out + low * ost);
-    const unsigned orow = at(rel * (unsigned)ost, idx < n, FAR_T);
+  auto put = [&](Rsrc ro, unsigned rel, bool there, const float (&o)[4][VT]) {
+    const unsigned orow = at(rel * (unsigned)ost, there, FAR_T);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
       const unsigned off = orow + od[e];
@@ -328,9 +332,10 @@ __global__ __launch_bounds__(256, PREFETCH && (sizeof(T) == 4 || KT == 8) ? 1 : 
   /* padding: zeros, in forward order whatever the walk */
   if (!STATE) {
     const float zero[4][VT] = {};
-    for (int t = len > lo ? len : lo; t < end; t += chunk) {
-      const int n = end - t < chunk ? end - t : chunk;
-      put(idx, n, t, zero);
+    const int tile = chunk < 16 ? chunk : 16;
+    for (int t = len > lo ? len : lo; t < end; t += tile) {
+      const int n = end - t < tile ? end - t : tile;
+      put(rsrc_of(out + t * ost), idx, idx < n, zero);
     }
   }
 
@@ -386,159 +391,233 @@ __global__ __launch_bounds__(256, PREFETCH && (sizeof(T) == 4 || KT == 8) ? 1 : 
   }
 
   const int e0 = rev ? 0 : 1; /* the entering state has decayed by one step at position 0, or by none yet */
-  float dm[4], wk[4];
+  float dm[H][4], wk[H][4], fi[H]; /* dm[x]: from a key to a query x tiles behind it */
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const int j = 4 * g + e;
-    dm[e] = idx >= j ? w.p_scale * pw(l, idx - j) : 0.0f;
+  for (int f = 0; f < H; f++) {
+#pragma unroll
+    for (int e = 0; e < 4; e++) {
+      const int d = 16 * f + idx - (4 * g + e);
+      dm[f][e] = d >= 0 ? w.p_scale * pw(l, d) : 0.0f;
+    }
+    fi[f] = w.in_scale * pw(l, 16 * f + idx + e0);
   }
-  const float fi = w.in_scale * pw(l, idx + e0);
   float gn = 1.0f;
 
   float through = 1.0f; /* STATE: what the split multiplies an entering state by */
   int single = 0;       /* tokens left to take one by one */
   int placed = 0, scaled = 0; /* the chunk sizes that the offsets and the factors stand for */
+  int p = lo, n = 0;
+  /* the lowest token of tile f of the chunk */
+  auto low_of = [&](int n, int f) -> long long {
+    const int n0 = n < 16 ? n : 16;
+    return rev ? len - p - n0 - 16 * f : p + 16 * f;
+  };
   struct Chunk {
-    Raw<T, KT, VEC> kr[4], qr[4], kc[4];
-    Raw<T, VT, VEC> vc[4];
+    Raw<T, KT, VEC> kr[H][4], qr[H][4], kc[H][4];
+    Raw<T, VT, VEC> vc[H][4];
     unsigned start;
   };
   auto load = [&](Chunk& c, int p, int n) {
-    if (n != placed) {
-      placed = n;
-      place(n);
-    }
-    const long long low = rev ? len - p - n : p;
-    const Rsrc rk = rsrc_of(k + low * kst), rv = rsrc_of(v + low * vst);
-    if (!STATE) {
-      const Rsrc rq = rsrc_of(q + low * qst);
-#pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int left = kdim - KT * (4 * g + e);
-        c.kr[e].load(rk, krow + kd[e], left);
-        c.qr[e].load(rq, qrow + kd[e], left);
-      }
-    }
-#pragma unroll
-    for (int e = 0; e < 4; e++) {
-      c.vc[e].load(rv, vcol[e], vleft - VT * idx);
-      c.kc[e].load(rk, kcol[e], kdim - KT * idx);
+    const int n0 = n < 16 ? n : 16;
+    if (n0 != placed) {
+      placed = n0;
+      place(n0);
     }
     c.start = 0;
     if (starts) {
       /* position x of a reversed walk is token len - 1 - x, behind the start that token len - x may carry */
-      const Rsrc rs = rsrc_of(starts + (rev ? low + 1 : low) * starts_st);
-      const bool there = (idx < n) & ((p + idx != 0) | !rev);
-      const unsigned back = n - 1 - idx, rel = rev ? back : idx;
+      const Rsrc rs = rsrc_of(starts + (rev ? len - p - n + 1 : p) * starts_st);
+      const int i = lane & (C - 1);
+      const bool there = (i < n) & ((p + i != 0) | !rev);
+      const unsigned back = n - 1 - i, rel = rev ? back : i;
       c.start = __builtin_amdgcn_raw_buffer_load_b8(rs, at(rel * (unsigned)starts_st, there, FAR_T), 0, 0);
     }
+#pragma unroll
+    for (int f = 0; f < H; f++) {
+      const bool there = 16 * f < n; /* the tile behind is whole or missing */
+      const long long low = low_of(n, f);
+      const Rsrc rk = rsrc_of(k + low * kst, there), rv = rsrc_of(v + low * vst, there), rq = rsrc_of(q + low * qst, there);
+#pragma unroll
+      for (int e = 0; e < 4; e++) c.vc[f][e].load(rv, vcol[e], vleft - VT * idx);
+      if (!STATE) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int left = kdim - KT * (4 * g + e);
+          c.kr[f][e].load(rk, krow + kd[e], left);
+          c.qr[f][e].load(rq, qrow + kd[e], left);
+        }
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) c.kc[f][e].load(rk, kcol[e], kdim - KT * idx);
+    }
   };
-  auto size = [&](int p) { return single ? 1 : hi - p < chunk ? hi - p : chunk; };
-
-  int p = lo, n = 0;
   /* one chunk; false: it holds a value that is not finite and has to be taken token by token */
-  auto work = [&](const Chunk& c) {
+  auto work = [&](Chunk& c) {
     if (n != scaled) {
       scaled = n;
       gn = pw(l, n);
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int j = 4 * g + e;
-        wk[e] = j < n ? w.w_scale * pw(l, n - 1 - j + (1 - e0)) : 0.0f;
-      }
+      for (int f = 0; f < H; f++)
+#pragma unroll
+        for (int e = 0; e < 4; e++) {
+          const int j = 16 * f + 4 * g + e;
+          wk[f][e] = j < n ? w.w_scale * pw(l, n - 1 - j + (1 - e0)) : 0.0f;
+        }
     }
-    const long long low = rev ? len - p - n : p;
-    const auto &kr = c.kr, &qr = c.qr, &kc = c.kc;
-    const auto& vc = c.vc;
-    /* bit i: an episode starts between positions i - 1 and i */
-    const unsigned brk = starts ? (unsigned)(__ballot(c.start != 0) & 0xffffu) : 0u;
-
     /* a value that is not finite must not meet the zeros of the mask (0 * inf): its chunk is taken token by
        token, where every product belongs to the token */
     unsigned bad = 0;
 #pragma unroll
-    for (int e = 0; e < 4; e++) bad |= not_finite(vc[e]);
+    for (int f = 0; f < H; f++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) bad |= not_finite(c.vc[f][e]);
     if (n > 1 && __any(bad != 0)) return false;
 
-    const unsigned upto = (2u << idx) - 1u; /* breaks at or in front of this lane's position */
-    const bool from_state = (brk & upto) == 0, keep = brk == 0;
-    auto scores = [&](f4& pt) { /* the scores of token idx with keys 4 g + e, masked and decayed */
+    /* bit i: an episode starts between positions i - 1 and i.  Most chunks have none, and skip what a start cuts. */
+    const unsigned brk = starts ? (unsigned)__ballot(c.start != 0) & (unsigned)((1ull << C) - 1) : 0u;
+    const bool cut = brk != 0;
+    auto upto = [&](int f) { return (2u << (16 * f + idx)) - 1u; }; /* breaks at or in front of a query */
+    /* the scores of query tile fi with key tile fj: masked and decayed (pt[e]: query idx, key 4 g + e) */
+    auto scores = [&](f4& pt, int fq, int fk) {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
-        const int j = 4 * g + e;
-        const float x = pt[e] * dm[e];
-        const bool ok = (idx >= j) & ((brk & upto & ~((2u << j) - 1u)) == 0);
+        const float x = pt[e] * dm[fq - fk][e];
+        const bool ok = (fq != fk) | (idx >= 4 * g + e);
         pt[e] = ok ? x : 0.0f;
       }
-    };
-    auto entering = [&](f4& x) { /* the read-out of the entering state for token idx */
+      if (cut) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const float y = x[e] * fi;
-        x[e] = from_state ? y : 0.0f;
+        for (int e = 0; e < 4; e++) pt[e] = (brk & upto(fq) & ~((2u << (16 * fk + 4 * g + e)) - 1u)) == 0 ? pt[e] : 0.0f;
+      }
+    };
+    /* the read-out of the entering state */
+    auto entering = [&](f4& x, int f) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) x[e] *= fi[f];
+      if (cut) {
+#pragma unroll
+        for (int e = 0; e < 4; e++) x[e] = (brk & upto(f)) == 0 ? x[e] : 0.0f;
       }
     };
     auto decay = [&] {
+      if (cut) {
 #pragma unroll
-      for (int mt = 0; mt < KT; mt++)
+        for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-        for (int nt = 0; nt < VT; nt++)
+          for (int nt = 0; nt < VT; nt++) S[mt][nt] = f4{0, 0, 0, 0};
+        /* keys in front of the last start do not enter the state */
+#pragma unroll
+        for (int f = 0; f < H; f++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const float x = S[mt][nt][e] * gn;
-            S[mt][nt][e] = keep ? x : 0.0f;
+            const int j = 16 * f + 4 * g + e;
+            const bool ok = (brk & ~((2u << j) - 1u)) == 0;
+#pragma unroll
+            for (int i = 0; i < Raw<T, KT, VEC>::D; i++) c.kc[f][e].d[i] = ok ? c.kc[f][e].d[i] : 0;
           }
+      } else {
+#pragma unroll
+        for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) S[mt][nt][e] *= gn;
+      }
     };
-    auto key = [&](int mt, int e) { /* k of token 4 g + e as it enters the state behind the chunk */
-      const float x = kc[e].get(mt) * wk[e];
-      return (brk >> (4 * g + e + 1)) == 0 ? x : 0.0f;
+    auto key = [&](int f, int mt, int e) { return c.kc[f][e].get(mt) * wk[f][e]; }; /* as it enters the state */
+    auto put_tile = [&](int f, const float (&o)[4][VT]) {
+      const int n0 = n < 16 ? n : 16;
+      put(rsrc_of(out + low_of(n, f) * ost, 16 * f < n), rev ? n0 - 1 - idx : idx, idx < n0, o);
     };
-    float o[4][VT]; /* o[e][nt]: channel VT (4 g + e) + nt of token idx */
     if constexpr (__is_same(T, Bf16)) {
-      u2 vq[VT];
+      u2 vq[H][VT];
 #pragma unroll
-      for (int nt = 0; nt < VT; nt++) vq[nt] = pack_col<VT, VEC>(vc, nt);
+      for (int f = 0; f < H; f++)
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++) vq[f][nt] = pack_col<VT, VEC>(c.vc[f], nt);
       if (!STATE) {
-        u2 kq[KT], qq[KT];
-        pack_row<KT, VEC>(kr, kq);
-        pack_row<KT, VEC>(qr, qq);
-        f4 pt = {0, 0, 0, 0};
-        if constexpr (KT == 1) pt = mfma32(u4{kq[0].x, kq[0].y, 0, 0}, u4{qq[0].x, qq[0].y, 0, 0}, pt);
+        u2 kq[H][KT], qq[H][KT];
 #pragma unroll
-        for (int i = 0; i + 1 < KT; i += 2)
-          pt = mfma32(u4{kq[i].x, kq[i].y, kq[i + 1].x, kq[i + 1].y}, u4{qq[i].x, qq[i].y, qq[i + 1].x, qq[i + 1].y}, pt);
-        scores(pt);
-        float p0 = pt[0], p1 = pt[1], p2 = pt[2], p3 = pt[3];
-        const unsigned h0 = split_bf16(p0, p1), h1 = split_bf16(p2, p3);
-        const u4 ph = {h0, h1, pack_bf16(p0, p1), pack_bf16(p2, p3)};
+        for (int f = 0; f < H; f++) {
+          pack_row<KT, VEC>(c.kr[f], kq[f]);
+          pack_row<KT, VEC>(c.qr[f], qq[f]);
+        }
+        u2 ph[H][H], pl[H][H]; /* [query tile][key tile]: leading part and rest */
+#pragma unroll
+        for (int fq = 0; fq < H; fq++)
+#pragma unroll
+          for (int fk = 0; fk <= fq; fk++) {
+            f4 pt = {0, 0, 0, 0};
+            const auto &x = kq[fk], &y = qq[fq];
+            if constexpr (KT == 1) pt = mfma32(u4{x[0].x, x[0].y, 0, 0}, u4{y[0].x, y[0].y, 0, 0}, pt);
+#pragma unroll
+            for (int i = 0; i + 1 < KT; i += 2)
+              pt = mfma32(u4{x[i].x, x[i].y, x[i + 1].x, x[i + 1].y}, u4{y[i].x, y[i].y, y[i + 1].x, y[i + 1].y}, pt);
+            scores(pt, fq, fk);
+            float p0 = pt[0], p1 = pt[1], p2 = pt[2], p3 = pt[3];
+            ph[fq][fk].x = split_bf16(p0, p1);
+            ph[fq][fk].y = split_bf16(p2, p3);
+            pl[fq][fk] = u2{pack_bf16(p0, p1), pack_bf16(p2, p3)};
+          }
+        float o[H][4][VT]; /* o[f][e][nt]: channel VT (4 g + e) + nt of token 16 f + idx */
 #pragma unroll
         for (int nt = 0; nt < VT; nt++) {
-          f4 x = {0, 0, 0, 0};
+          f4 x[H];
+#pragma unroll
+          for (int f = 0; f < H; f++) x[f] = f4{0, 0, 0, 0};
 #pragma unroll
           for (int i = 0; i < KT; i++) {
-            /* the state's elements of the four channels in qq[i] */
+            /* the state's elements of the four channels in qq[.][i] */
             float s0 = S[4 * i % KT][nt][4 * i / KT], s1 = S[(4 * i + 1) % KT][nt][(4 * i + 1) / KT],
                   s2 = S[(4 * i + 2) % KT][nt][(4 * i + 2) / KT], s3 = S[(4 * i + 3) % KT][nt][(4 * i + 3) / KT];
             const unsigned a0 = split_bf16(s0, s1), a1 = split_bf16(s2, s3);
-            x = mfma32(u4{a0, a1, pack_bf16(s0, s1), pack_bf16(s2, s3)}, u4{qq[i].x, qq[i].y, qq[i].x, qq[i].y}, x);
-          }
-          entering(x);
-          x = mfma32(u4{vq[nt].x, vq[nt].y, vq[nt].x, vq[nt].y}, ph, x);
+            const u4 sa = {a0, a1, pack_bf16(s0, s1), pack_bf16(s2, s3)};
 #pragma unroll
-          for (int e = 0; e < 4; e++) o[e][nt] = x[e];
+            for (int f = 0; f < H; f++) x[f] = mfma32(sa, u4{qq[f][i].x, qq[f][i].y, qq[f][i].x, qq[f][i].y}, x[f]);
+          }
+#pragma unroll
+          for (int f = 0; f < H; f++) {
+            entering(x[f], f);
+            if (f == 0) {
+              const u2 y = vq[0][nt], z = ph[0][0], zl = pl[0][0];
+              x[f] = mfma32(u4{y.x, y.y, y.x, y.y}, u4{z.x, z.y, zl.x, zl.y}, x[f]);
+            } else {
+              const u4 y = {vq[0][nt].x, vq[0][nt].y, vq[f][nt].x, vq[f][nt].y};
+              x[f] = mfma32(y, u4{ph[f][0].x, ph[f][0].y, ph[f][f].x, ph[f][f].y}, x[f]);
+              x[f] = mfma32(y, u4{pl[f][0].x, pl[f][0].y, pl[f][f].x, pl[f][f].y}, x[f]);
+            }
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[f][e][nt] = x[f][e];
+          }
         }
-        put(rev ? n - 1 - idx : idx, n, low, o);
+#pragma unroll
+        for (int f = 0; f < H; f++) put_tile(f, o[f]);
       }
       decay();
 #pragma unroll
       for (int mt = 0; mt < KT; mt++) {
-        float k0 = key(mt, 0), k1 = key(mt, 1), k2 = key(mt, 2), k3 = key(mt, 3);
-        const unsigned h0 = split_bf16(k0, k1), h1 = split_bf16(k2, k3), m0 = split_bf16(k0, k1), m1 = split_bf16(k2, k3);
-        const u4 rest = {pack_bf16(k0, k1), pack_bf16(k2, k3), 0, 0};
+        u2 kh[H], km[H], kl[H];
+#pragma unroll
+        for (int f = 0; f < H; f++) {
+          float k0 = key(f, mt, 0), k1 = key(f, mt, 1), k2 = key(f, mt, 2), k3 = key(f, mt, 3);
+          kh[f].x = split_bf16(k0, k1);
+          kh[f].y = split_bf16(k2, k3);
+          km[f].x = split_bf16(k0, k1);
+          km[f].y = split_bf16(k2, k3);
+          kl[f] = u2{pack_bf16(k0, k1), pack_bf16(k2, k3)};
+        }
 #pragma unroll
         for (int nt = 0; nt < VT; nt++) {
-          S[mt][nt] = mfma32(u4{h0, h1, m0, m1}, u4{vq[nt].x, vq[nt].y, vq[nt].x, vq[nt].y}, S[mt][nt]);
-          S[mt][nt] = mfma32(rest, u4{vq[nt].x, vq[nt].y, 0, 0}, S[mt][nt]);
+          const u2 x = vq[0][nt], y = vq[H - 1][nt];
+          if constexpr (H == 1) {
+            S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, km[0].x, km[0].y}, u4{x.x, x.y, x.x, x.y}, S[mt][nt]);
+            S[mt][nt] = mfma32(u4{kl[0].x, kl[0].y, 0, 0}, u4{x.x, x.y, 0, 0}, S[mt][nt]);
+          } else {
+            const u4 z = {x.x, x.y, y.x, y.y};
+            S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, kh[1].x, kh[1].y}, z, S[mt][nt]);
+            S[mt][nt] = mfma32(u4{km[0].x, km[0].y, km[1].x, km[1].y}, z, S[mt][nt]);
+            S[mt][nt] = mfma32(u4{kl[0].x, kl[0].y, kl[1].x, kl[1].y}, z, S[mt][nt]);
+          }
         }
       }
     } else {
@@ -547,72 +626,49 @@ __global__ __launch_bounds__(256, PREFETCH && (sizeof(T) == 4 || KT == 8) ? 1 : 
 #pragma unroll
         for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) pt = mfma4(kr[e].get(mt), qr[e].get(mt), pt);
-        scores(pt);
+          for (int e = 0; e < 4; e++) pt = mfma4(c.kr[0][e].get(mt), c.qr[0][e].get(mt), pt);
+        scores(pt, 0, 0);
+        float o[4][VT];
 #pragma unroll
         for (int nt = 0; nt < VT; nt++) {
           f4 x = {0, 0, 0, 0};
 #pragma unroll
           for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) x = mfma4(S[mt][nt][e], qr[e].get(mt), x);
-          entering(x);
+            for (int e = 0; e < 4; e++) x = mfma4(S[mt][nt][e], c.qr[0][e].get(mt), x);
+          entering(x, 0);
 #pragma unroll
-          for (int e = 0; e < 4; e++) x = mfma4(vc[e].get(nt), pt[e], x);
+          for (int e = 0; e < 4; e++) x = mfma4(c.vc[0][e].get(nt), pt[e], x);
 #pragma unroll
           for (int e = 0; e < 4; e++) o[e][nt] = x[e];
         }
-        put(rev ? n - 1 - idx : idx, n, low, o);
+        put_tile(0, o);
       }
       decay();
 #pragma unroll
       for (int mt = 0; mt < KT; mt++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          const float kw = key(mt, e);
+          const float kw = key(0, mt, e);
 #pragma unroll
-          for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma4(kw, vc[e].get(nt), S[mt][nt]);
+          for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma4(kw, c.vc[0][e].get(nt), S[mt][nt]);
         }
     }
-    if (STATE) through = keep ? through * gn : 0.0f;
+    if (STATE) through = cut ? 0.0f : through * gn;
     return true;
   };
-  if constexpr (PREFETCH) {
-    /* the chunk behind is on its way while one is worked on */
+  while (p < hi) {
     Chunk c;
-    bool here = false;
-    while (p < hi) {
-      if (!here) {
-        n = size(p);
-        load(c, p, n);
-      }
-      Chunk next;
-      const bool more = p + n < hi && !single;
-      const int n_next = more ? size(p + n) : 0;
-      if (more) load(next, p + n, n_next);
-      if (!work(c)) {
-        single = n;
-        here = false;
-        continue;
-      }
-      p += n;
-      if (single) single--;
-      here = more;
-      n = n_next;
-      c = next;
+    /* whole chunks, then tiles */
+    const int left = hi - p;
+    n = single || chunk == 1 ? 1 : left >= C ? C : left < 16 ? left : 16;
+    load(c, p, n);
+    if (!work(c)) {
+      single = n;
+      continue;
     }
-  } else {
-    while (p < hi) {
-      Chunk c;
-      n = size(p);
-      load(c, p, n);
-      if (!work(c)) {
-        single = n;
-        continue;
-      }
-      p += n;
-      if (single) single--;
-    }
+    p += n;
+    if (single) single--;
   }
 
   float* s_out = nullptr;
@@ -937,16 +993,16 @@ template <class T, int KT, int VT, bool VEC> static int walk_launch(WalkArgs& a,
   a.near = (share + waves - 1) / waves;
   const long long tasks = streams * (phase == STATES ? a.nsplit - 1 : a.nsplit), per = 8LL * a.near * waves;
   const dim3 grid((unsigned)((tasks + per - 1) / per * 8 * a.near)), block(64 * waves);
+  /* bfloat16 sequences of more than one tile of tokens go two tiles at a time */
+  constexpr int H = __is_same(T, Bf16) ? 2 : 1;
   if (phase == STATES) {
-    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, true, true>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, true, H>), grid, block, 0, s, a);
     PL_CHK(hipGetLastError());
     hipLaunchKernelGGL(k_attn_join, dim3((a.kdim * a.vdim + 63) / 64, (unsigned)(a.b * a.h), (unsigned)a.nw), dim3(64), 0, s, a);
-  } else if (a.nsplit > 1 || (sizeof(T) == 2 && KT < 8 && a.t > 16)) {
-    /* the next chunk's loads run ahead where a wave has a SIMD to itself (split sequences) or the registers for two
-       chunks leave room for two waves; else the second wave hides them */
-    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false, true>), grid, block, 0, s, a);
+  } else if (H == 2 && (a.nsplit > 1 || a.t > 16)) {
+    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false, H>), grid, block, 0, s, a);
   } else {
-    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false, false>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false, 1>), grid, block, 0, s, a);
   }
   PL_CHK(hipGetLastError());
   return UR3E_OK;
@@ -955,7 +1011,7 @@ template <class T, int KT, int VT> static int walk_vec(WalkArgs& a, Phase phase,
   bool vec = true;
   a.state_vec = 1;
   a.chunk = 16;
-  /* 16 tokens within the 30-bit offsets of a chunk, else token by token */
+  /* a tile's tokens (a chunk's starts) within its 30-bit offsets, else token by token */
   const long long far = ((1LL << 30) - 1024) / 64;
   if (a.starts_st > far) a.chunk = 1;
   for (int i = 0; i < a.nw; i++) {
