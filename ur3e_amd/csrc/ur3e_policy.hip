@@ -407,6 +407,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   int single = 0;       /* tokens left to take one by one */
   int placed = 0, scaled = 0; /* the chunk sizes that the offsets and the factors stand for */
   int p = lo, n = 0;
+  /* whether anything reads the state behind the chunk */
+  const bool kept = STATE || (split == nsplit - 1 && w.s_out);
+  auto carried = [&](int n) { return kept || p + n < hi; };
   /* the lowest token of tile f of the chunk */
   auto low_of = [&](int n, int f) -> long long {
     const int n0 = n < 16 ? n : 16;
@@ -447,8 +450,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           c.qr[f][e].load(rq, qrow + kd[e], left);
         }
       }
+      if (STATE || carried(n)) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) c.kc[f][e].load(rk, kcol[e], kdim - KT * idx);
+        for (int e = 0; e < 4; e++) c.kc[f][e].load(rk, kcol[e], kdim - KT * idx);
+      }
     }
   };
   /* one chunk; false: it holds a value that is not finite and has to be taken token by token */
@@ -593,6 +598,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
         for (int f = 0; f < H; f++) put_tile(f, o[f]);
       }
+      if (!carried(n)) return true;
       decay();
 #pragma unroll
       for (int mt = 0; mt < KT; mt++) {
@@ -644,6 +650,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         }
         put_tile(0, o);
       }
+      if (!carried(n)) return true;
       decay();
 #pragma unroll
       for (int mt = 0; mt < KT; mt++)
@@ -721,38 +728,43 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 }
 
 /* States that enter each split: ws[s] holds split s - 1's own sum (k_attn_walk, STATE) and becomes
-   X_s = wf[s] X_{s-1} + ws[s], X_0 = s_in.  A thread owns one element and runs along the splits; nothing but
-   the chain of multiply-adds depends on the split in front, so the sums of JOIN splits are loaded at a time, the
-   next ones while one lot is chained. */
-#define JOIN 32
-__global__ __launch_bounds__(64) void k_attn_join(WalkArgs a) {
+   X_s = wf[s] X_{s-1} + ws[s], X_0 = s_in.  A thread owns VW elements and runs along the splits; nothing but
+   the chain of multiply-adds depends on the split in front, so the sums of LOT splits are loaded at a time, the next
+   ones while one lot is chained.  Few long sequences wait for the chain: one element a thread, long lots.  Many
+   short ones wait for their turn on the card: four elements a thread. */
+template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(WalkArgs a) {
   const Walk w = a.w[blockIdx.z];
   const long long bh = blockIdx.y;
   const int elems = a.kdim * a.vdim, nsplit = a.nsplit;
-  const int e = blockIdx.x * 64 + threadIdx.x;
+  const int e = (blockIdx.x * 64 + threadIdx.x) * VW;
   if (e >= elems) return;
+  struct alignas(4 * VW) Pack { float x[VW]; };
   float* ws = w.ws + bh * nsplit * elems + e;
   const float* wf = w.wf + bh * nsplit;
-  struct Lot { float u[JOIN], f[JOIN]; };
+  struct Lot { Pack u[LOT]; float f[LOT]; };
   auto load = [&](Lot& l, int s0) {
 #pragma unroll
-    for (int i = 0; i < JOIN; i++) {
+    for (int i = 0; i < LOT; i++) {
       const int s = s0 + 1 + i < nsplit ? s0 + 1 + i : nsplit - 1;
-      l.u[i] = ws[(long long)s * elems];
+      l.u[i] = *reinterpret_cast<const Pack*>(ws + (long long)s * elems);
       l.f[i] = wf[s];
     }
   };
   Lot l;
   load(l, 0);
-  float x = w.s_in ? w.s_in[bh * elems + e] : 0.0f;
-  for (int s0 = 0; s0 < nsplit; s0 += JOIN) {
+  Pack x = {};
+  if (w.s_in) x = *reinterpret_cast<const Pack*>(w.s_in + bh * elems + e);
+  for (int s0 = 0; s0 < nsplit; s0 += LOT) {
     Lot next;
-    if (s0 + JOIN < nsplit) load(next, s0 + JOIN);
+    if (s0 + LOT < nsplit) load(next, s0 + LOT);
 #pragma unroll
-    for (int i = 0; i < JOIN; i++) {
-      if (s0 + i < nsplit) ws[(long long)(s0 + i) * elems] = x;
-      const float y = l.f[i] * x;
-      x = (l.f[i] == 0.0f ? 0.0f : y) + l.u[i];
+    for (int i = 0; i < LOT; i++) {
+      if (s0 + i < nsplit) *reinterpret_cast<Pack*>(ws + (long long)(s0 + i) * elems) = x;
+#pragma unroll
+      for (int c = 0; c < VW; c++) {
+        const float y = l.f[i] * x.x[c];
+        x.x[c] = (l.f[i] == 0.0f ? 0.0f : y) + l.u[i].x[c];
+      }
     }
     l = next;
   }
@@ -950,14 +962,20 @@ static Tiles tiles_of(int kdim, int vdim) {
 struct Splits {
   int n, len;
 };
-/* How many waves share a sequence.  ~2 waves a SIMD (2,048) fill the card; a split costs a chain of 16-token
-   chunks, and its state one more link of the chain of the join, so the shortest worth having grows with the
-   square root of the length. */
-static Splits splits_of(const ur3e_attn_t* a, int walks) {
-  const long long waves = (long long)a->b * a->heads * tiles_of(a->dk, a->dv).slabs * walks;
+/* How many waves share a sequence, from the waves of the smallest launch.  Two waves a SIMD (2,048) fill the card,
+   and what does not fit beside them waits for a second round, so as many splits as still fit.  A split costs a
+   chain of chunks, and its state one more link of the chain of the join, so the shortest worth having grows with
+   the square root of the length. */
+static Splits splits_of(const ur3e_attn_t* a, int backward) {
+  long long waves = (long long)a->b * a->heads * tiles_of(a->dk, a->dv).slabs;
+  if (backward && a->dk == a->dv) waves *= 3;
+  if (backward && a->dk != a->dv) {
+    const long long other = 2LL * a->b * a->heads * tiles_of(a->dv, a->dk).slabs;
+    if (other < waves) waves = other;
+  }
   Splits p = {1, a->t > 0 ? a->t : 1};
-  if (waves < 1024 && a->t >= 64) {
-    const long long want = (2048 + waves - 1) / waves;
+  const long long want = 2048 / waves;
+  if (want > 1 && a->t >= 64) {
     int least = 32;
     while ((long long)least * least * 4 < a->t) least += 16;
     const int len = (int)(((a->t + want - 1) / want + 15) / 16 * 16);
@@ -998,7 +1016,12 @@ template <class T, int KT, int VT, bool VEC> static int walk_launch(WalkArgs& a,
   if (phase == STATES) {
     hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, true, H>), grid, block, 0, s, a);
     PL_CHK(hipGetLastError());
-    hipLaunchKernelGGL(k_attn_join, dim3((a.kdim * a.vdim + 63) / 64, (unsigned)(a.b * a.h), (unsigned)a.nw), dim3(64), 0, s, a);
+    const int elems = a.kdim * a.vdim;
+    const unsigned bh = (unsigned)(a.b * a.h), nw = (unsigned)a.nw;
+    if (a.state_vec && elems % 4 == 0 && (long long)bh * nw * elems >= 64 * 4096)
+      hipLaunchKernelGGL((k_attn_join<4, 8>), dim3((elems + 255) / 256, bh, nw), dim3(64), 0, s, a);
+    else
+      hipLaunchKernelGGL((k_attn_join<1, 32>), dim3((elems + 63) / 64, bh, nw), dim3(64), 0, s, a);
   } else if (H == 2 && (a.nsplit > 1 || a.t > 16)) {
     hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false, H>), grid, block, 0, s, a);
   } else {
@@ -1063,8 +1086,8 @@ static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
 static size_t attn_bytes(const ur3e_attn_t* a, int backward) {
   if (a->b == 0) return 0;
-  if (!backward) return split_bytes(a, splits_of(a, 1));
-  size_t n = 2 * up256(split_bytes(a, splits_of(a, 3)));
+  if (!backward) return split_bytes(a, splits_of(a, 0));
+  size_t n = 2 * up256(split_bytes(a, splits_of(a, 1)));
   if (a->heads != a->kv_heads) n += up256((size_t)a->b * a->t * a->heads * a->dk * 4) + up256((size_t)a->b * a->t * a->heads * a->dv * 4);
   return n;
 }
@@ -1085,7 +1108,7 @@ extern "C" int ur3e_attn_forward(const ur3e_attn_t* a, const ur3e_tokens_t* out,
   if (!out || (a->t > 0 && !out->p)) return bad_arg("attention: null out");
   if (out->st < 0) return bad_arg("attention: token strides must not be negative");
   if (workspace_bytes < attn_bytes(a, 0) || (attn_bytes(a, 0) && !workspace)) return bad_arg("attention: workspace too small");
-  const Splits p = splits_of(a, 1);
+  const Splits p = splits_of(a, 0);
   WalkArgs w = args_of(a, a->dk, a->dv, p);
   const int grp = a->heads / a->kv_heads;
   w.nw = 1;
@@ -1126,7 +1149,7 @@ extern "C" int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dou
   if (workspace_bytes < attn_bytes(a, 1) || (attn_bytes(a, 1) && !workspace)) return bad_arg("attention: workspace too small");
   hipStream_t s = (hipStream_t)stream;
   const int grp = a->heads / a->kv_heads;
-  const Splits p = splits_of(a, 3);
+  const Splits p = splits_of(a, 1);
   char* ws = (char*)workspace;
   const size_t n = up256(split_bytes(a, p));
   float *fk = nullptr, *fv = nullptr;
