@@ -201,15 +201,26 @@ template <class T, int N, bool VEC> __device__ __forceinline__ void store_n(Rsrc
   }
 }
 
-/* whether one of the elements is an infinity or a NaN: its exponent carries into the sign's place */
-template <class T, int N, bool VEC> __device__ __forceinline__ unsigned not_finite(const Raw<T, N, VEC>& x) {
-  constexpr unsigned abs = sizeof(T) == 4 ? 0x7fffffffu : 0x7fff7fffu;
-  constexpr unsigned one = sizeof(T) == 4 ? 0x00800000u : __is_same(T, Bf16) ? 0x00800080u : 0x04000400u;
-  unsigned r = 0;
-#pragma unroll
-  for (int i = 0; i < Raw<T, N, VEC>::D; i++) r |= (x.d[i] & abs) + one;
-  return r & ~abs;
-}
+/* The largest magnitude met so far, as the bits of an unsigned integer (two 16-bit ones), and whether it is an
+   infinity or a NaN. */
+template <class T> struct Peak {
+  typedef unsigned short us2 __attribute__((ext_vector_type(2)));
+  unsigned m = 0;
+  __device__ __forceinline__ void add(unsigned d) {
+    if constexpr (sizeof(T) == 4) {
+      const unsigned x = d & 0x7fffffffu;
+      m = x > m ? x : m;
+    } else {
+      const unsigned x = d & 0x7fff7fffu;
+      m = __builtin_bit_cast(unsigned, __builtin_elementwise_max(__builtin_bit_cast(us2, x), __builtin_bit_cast(us2, m)));
+    }
+  }
+  __device__ __forceinline__ bool not_finite() const {
+    if constexpr (sizeof(T) == 4) return m >= 0x7f800000u;
+    constexpr unsigned inf = __is_same(T, Bf16) ? 0x7f80u : 0x7c00u;
+    return (m >= inf << 16) | ((m & 0xffffu) >= inf);
+  }
+};
 
 /* bfloat16 fragments, two elements to a dword.  A 32-bit operand enters the matrix instructions as the sum of
    its leading parts of 8 bits each: two (error 2^-17) for scores and state, whose results are rounded to 2^-9
@@ -305,13 +316,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   }
   const unsigned kidx = at(KT * idx * ES, KT * idx < kdim, FAR_D), vidx = at(VT * idx * ES, VT * idx < vleft, FAR_D);
   /* ... and of its tokens, for tiles of n: the lowest token of the tile is the base */
-  unsigned qrow, krow, kcol[4], vcol[4];
+  unsigned qrow[4], krow[4], kcol[4], vcol[4];
   auto place = [&](int n) {
     const unsigned back = n - 1 - idx, rel = rev ? back : idx;
-    qrow = at(rel * (unsigned)qst, idx < n, FAR_T);
-    krow = at(rel * (unsigned)kst, idx < n, FAR_T);
 #pragma unroll
     for (int e = 0; e < 4; e++) {
+      qrow[e] = at(rel * (unsigned)qst, idx < n, FAR_T) + kd[e];
+      krow[e] = at(rel * (unsigned)kst, idx < n, FAR_T) + kd[e];
       const int j = 4 * g + e;
       const unsigned backj = n - 1 - j, rc = rev ? backj : j;
       kcol[e] = at(rc * (unsigned)kst, j < n, FAR_T) + kidx;
@@ -401,6 +412,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
     }
     fi[f] = w.in_scale * pw(l, 16 * f + idx + e0);
   }
+  unsigned causal[4];
+#pragma unroll
+  for (int e = 0; e < 4; e++) causal[e] = idx >= 4 * g + e ? 0xffffffffu : 0u;
   float gn = 1.0f;
 
   float through = 1.0f; /* STATE: what the split multiplies an entering state by */
@@ -410,6 +424,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   /* whether anything reads the state behind the chunk */
   const bool kept = STATE || (split == nsplit - 1 && w.s_out);
   auto carried = [&](int n) { return kept || p + n < hi; };
+  /* a state that leaves as floats is summed to their precision; one that only feeds 16-bit outputs, from keys
+     in two parts */
+  const bool fine = w.s_out != nullptr;
   /* the lowest token of tile f of the chunk */
   auto low_of = [&](int n, int f) -> long long {
     const int n0 = n < 16 ? n : 16;
@@ -446,8 +463,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           const int left = kdim - KT * (4 * g + e);
-          c.kr[f][e].load(rk, krow + kd[e], left);
-          c.qr[f][e].load(rq, qrow + kd[e], left);
+          c.kr[f][e].load(rk, krow[e], left);
+          c.qr[f][e].load(rq, qrow[e], left);
         }
       }
       if (STATE || carried(n)) {
@@ -471,12 +488,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
     }
     /* a value that is not finite must not meet the zeros of the mask (0 * inf): its chunk is taken token by
        token, where every product belongs to the token */
-    unsigned bad = 0;
+    Peak<T> peak;
 #pragma unroll
     for (int f = 0; f < H; f++)
 #pragma unroll
-      for (int e = 0; e < 4; e++) bad |= not_finite(c.vc[f][e]);
-    if (n > 1 && __any(bad != 0)) return false;
+      for (int e = 0; e < 4; e++)
+#pragma unroll
+        for (int i = 0; i < Raw<T, VT, VEC>::D; i++) peak.add(c.vc[f][e].d[i]);
+    if (n > 1 && __any(peak.not_finite())) return false;
 
     /* bit i: an episode starts between positions i - 1 and i.  Most chunks have none, and skip what a start cuts. */
     const unsigned brk = starts ? (unsigned)__ballot(c.start != 0) & (unsigned)((1ull << C) - 1) : 0u;
@@ -487,8 +506,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const float x = pt[e] * dm[fq - fk][e];
-        const bool ok = (fq != fk) | (idx >= 4 * g + e);
-        pt[e] = ok ? x : 0.0f;
+        /* a mask of bits, not a select: a select by VCC takes six times an AND here */
+        pt[e] = fq != fk ? x : __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & causal[e]);
       }
       if (cut) {
 #pragma unroll
@@ -602,27 +621,40 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       decay();
 #pragma unroll
       for (int mt = 0; mt < KT; mt++) {
-        u2 kh[H], km[H], kl[H];
+        float kx[H][4];
+        u2 kh[H], km[H];
 #pragma unroll
         for (int f = 0; f < H; f++) {
-          float k0 = key(f, mt, 0), k1 = key(f, mt, 1), k2 = key(f, mt, 2), k3 = key(f, mt, 3);
-          kh[f].x = split_bf16(k0, k1);
-          kh[f].y = split_bf16(k2, k3);
-          km[f].x = split_bf16(k0, k1);
-          km[f].y = split_bf16(k2, k3);
-          kl[f] = u2{pack_bf16(k0, k1), pack_bf16(k2, k3)};
+#pragma unroll
+          for (int e = 0; e < 4; e++) kx[f][e] = key(f, mt, e);
+          kh[f].x = split_bf16(kx[f][0], kx[f][1]);
+          kh[f].y = split_bf16(kx[f][2], kx[f][3]);
+          km[f] = u2{pack_bf16(kx[f][0], kx[f][1]), pack_bf16(kx[f][2], kx[f][3])};
         }
 #pragma unroll
         for (int nt = 0; nt < VT; nt++) {
           const u2 x = vq[0][nt], y = vq[H - 1][nt];
           if constexpr (H == 1) {
             S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, km[0].x, km[0].y}, u4{x.x, x.y, x.x, x.y}, S[mt][nt]);
-            S[mt][nt] = mfma32(u4{kl[0].x, kl[0].y, 0, 0}, u4{x.x, x.y, 0, 0}, S[mt][nt]);
           } else {
             const u4 z = {x.x, x.y, y.x, y.y};
             S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, kh[1].x, kh[1].y}, z, S[mt][nt]);
             S[mt][nt] = mfma32(u4{km[0].x, km[0].y, km[1].x, km[1].y}, z, S[mt][nt]);
-            S[mt][nt] = mfma32(u4{kl[0].x, kl[0].y, kl[1].x, kl[1].y}, z, S[mt][nt]);
+          }
+        }
+        if (fine) {
+          u2 kl[H];
+#pragma unroll
+          for (int f = 0; f < H; f++) {
+            (void)split_bf16(kx[f][0], kx[f][1]);
+            (void)split_bf16(kx[f][2], kx[f][3]);
+            kl[f] = u2{pack_bf16(kx[f][0], kx[f][1]), pack_bf16(kx[f][2], kx[f][3])};
+          }
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++) {
+            const u2 x = vq[0][nt], y = vq[H - 1][nt];
+            const u4 z = {x.x, x.y, H == 1 ? 0 : y.x, H == 1 ? 0 : y.y};
+            S[mt][nt] = mfma32(u4{kl[0].x, kl[0].y, H == 1 ? 0 : kl[H - 1].x, H == 1 ? 0 : kl[H - 1].y}, z, S[mt][nt]);
           }
         }
       }
