@@ -566,56 +566,70 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           pack_row<KT, VEC>(c.kr[f], kq[f]);
           pack_row<KT, VEC>(c.qr[f], qq[f]);
         }
-        u2 ph[H][H], pl[H][H]; /* [query tile][key tile]: leading part and rest */
+        /* Instructions that add to the same accumulators stand apart by those of the other tiles. */
+        f4 pt[H][H]; /* [query tile][key tile] */
 #pragma unroll
-        for (int fq = 0; fq < H; fq++)
+        for (int i = 0; i < (KT + 1) / 2; i++)
 #pragma unroll
-          for (int fk = 0; fk <= fq; fk++) {
-            f4 pt = {0, 0, 0, 0};
-            const auto &x = kq[fk], &y = qq[fq];
-            if constexpr (KT == 1) pt = mfma32(u4{x[0].x, x[0].y, 0, 0}, u4{y[0].x, y[0].y, 0, 0}, pt);
+          for (int fq = 0; fq < H; fq++)
 #pragma unroll
-            for (int i = 0; i + 1 < KT; i += 2)
-              pt = mfma32(u4{x[i].x, x[i].y, x[i + 1].x, x[i + 1].y}, u4{y[i].x, y[i].y, y[i + 1].x, y[i + 1].y}, pt);
-            scores(pt, fq, fk);
-            float p0 = pt[0], p1 = pt[1], p2 = pt[2], p3 = pt[3];
-            ph[fq][fk].x = split_bf16(p0, p1);
-            ph[fq][fk].y = split_bf16(p2, p3);
-            pl[fq][fk] = u2{pack_bf16(p0, p1), pack_bf16(p2, p3)};
-          }
-        float o[H][4][VT]; /* o[f][e][nt]: channel VT (4 g + e) + nt of token 16 f + idx */
+            for (int fk = 0; fk <= fq; fk++) {
+              const auto &x = kq[fk], &y = qq[fq];
+              const f4 z = i ? pt[fq][fk] : f4{0, 0, 0, 0};
+              if constexpr (KT == 1) pt[fq][fk] = mfma32(u4{x[0].x, x[0].y, 0, 0}, u4{y[0].x, y[0].y, 0, 0}, z);
+              else
+                pt[fq][fk] = mfma32(u4{x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y},
+                                    u4{y[2 * i].x, y[2 * i].y, y[2 * i + 1].x, y[2 * i + 1].y}, z);
+            }
+        f4 x[H][VT];
 #pragma unroll
-        for (int nt = 0; nt < VT; nt++) {
-          f4 x[H];
+        for (int i = 0; i < KT; i++)
 #pragma unroll
-          for (int f = 0; f < H; f++) x[f] = f4{0, 0, 0, 0};
-#pragma unroll
-          for (int i = 0; i < KT; i++) {
+          for (int nt = 0; nt < VT; nt++) {
             /* the state's elements of the four channels in qq[.][i] */
             float s0 = S[4 * i % KT][nt][4 * i / KT], s1 = S[(4 * i + 1) % KT][nt][(4 * i + 1) / KT],
                   s2 = S[(4 * i + 2) % KT][nt][(4 * i + 2) / KT], s3 = S[(4 * i + 3) % KT][nt][(4 * i + 3) / KT];
             const unsigned a0 = split_bf16(s0, s1), a1 = split_bf16(s2, s3);
             const u4 sa = {a0, a1, pack_bf16(s0, s1), pack_bf16(s2, s3)};
 #pragma unroll
-            for (int f = 0; f < H; f++) x[f] = mfma32(sa, u4{qq[f][i].x, qq[f][i].y, qq[f][i].x, qq[f][i].y}, x[f]);
+            for (int f = 0; f < H; f++)
+              x[f][nt] = mfma32(sa, u4{qq[f][i].x, qq[f][i].y, qq[f][i].x, qq[f][i].y}, i ? x[f][nt] : f4{0, 0, 0, 0});
+          }
+        u2 ph[H][H], pl[H][H]; /* leading part and rest */
+#pragma unroll
+        for (int fq = 0; fq < H; fq++)
+#pragma unroll
+          for (int fk = 0; fk <= fq; fk++) {
+            scores(pt[fq][fk], fq, fk);
+            float p0 = pt[fq][fk][0], p1 = pt[fq][fk][1], p2 = pt[fq][fk][2], p3 = pt[fq][fk][3];
+            ph[fq][fk].x = split_bf16(p0, p1);
+            ph[fq][fk].y = split_bf16(p2, p3);
+            pl[fq][fk] = u2{pack_bf16(p0, p1), pack_bf16(p2, p3)};
           }
 #pragma unroll
-          for (int f = 0; f < H; f++) {
-            entering(x[f], f);
-            if (f == 0) {
-              const u2 y = vq[0][nt], z = ph[0][0], zl = pl[0][0];
-              x[f] = mfma32(u4{y.x, y.y, y.x, y.y}, u4{z.x, z.y, zl.x, zl.y}, x[f]);
-            } else {
-              const u4 y = {vq[0][nt].x, vq[0][nt].y, vq[f][nt].x, vq[f][nt].y};
-              x[f] = mfma32(y, u4{ph[f][0].x, ph[f][0].y, ph[f][f].x, ph[f][f].y}, x[f]);
-              x[f] = mfma32(y, u4{pl[f][0].x, pl[f][0].y, pl[f][f].x, pl[f][f].y}, x[f]);
-            }
+        for (int f = 0; f < H; f++)
 #pragma unroll
-            for (int e = 0; e < 4; e++) o[f][e][nt] = x[f][e];
+          for (int nt = 0; nt < VT; nt++) {
+            entering(x[f][nt], f);
+            const u2 y = vq[0][nt], yf = vq[f][nt], z = ph[f][0], zl = pl[f][0], zf = ph[f][f];
+            if (f == 0) x[f][nt] = mfma32(u4{y.x, y.y, y.x, y.y}, u4{z.x, z.y, zl.x, zl.y}, x[f][nt]);
+            else x[f][nt] = mfma32(u4{y.x, y.y, yf.x, yf.y}, u4{z.x, z.y, zf.x, zf.y}, x[f][nt]);
           }
+#pragma unroll
+        for (int f = 1; f < H; f++)
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++)
+            x[f][nt] = mfma32(u4{vq[0][nt].x, vq[0][nt].y, vq[f][nt].x, vq[f][nt].y},
+                              u4{pl[f][0].x, pl[f][0].y, pl[f][f].x, pl[f][f].y}, x[f][nt]);
+#pragma unroll
+        for (int f = 0; f < H; f++) {
+          float o[4][VT]; /* o[e][nt]: channel VT (4 g + e) + nt of token 16 f + idx */
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) o[e][nt] = x[f][nt][e];
+          put_tile(f, o);
         }
-#pragma unroll
-        for (int f = 0; f < H; f++) put_tile(f, o[f]);
       }
       if (!carried(n)) return true;
       decay();
@@ -637,10 +651,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           if constexpr (H == 1) {
             S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, km[0].x, km[0].y}, u4{x.x, x.y, x.x, x.y}, S[mt][nt]);
           } else {
-            const u4 z = {x.x, x.y, y.x, y.y};
-            S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, kh[1].x, kh[1].y}, z, S[mt][nt]);
-            S[mt][nt] = mfma32(u4{km[0].x, km[0].y, km[1].x, km[1].y}, z, S[mt][nt]);
+            S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, kh[1].x, kh[1].y}, u4{x.x, x.y, y.x, y.y}, S[mt][nt]);
           }
+        }
+        if constexpr (H == 2) {
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++)
+            S[mt][nt] = mfma32(u4{km[0].x, km[0].y, km[1].x, km[1].y},
+                               u4{vq[0][nt].x, vq[0][nt].y, vq[1][nt].x, vq[1][nt].y}, S[mt][nt]);
         }
         if (fine) {
           u2 kl[H];
@@ -660,26 +678,35 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       }
     } else {
       if (!STATE) {
-        f4 pt = {0, 0, 0, 0};
+        f4 part[4] = {};
 #pragma unroll
         for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) pt = mfma4(c.kr[0][e].get(mt), c.qr[0][e].get(mt), pt);
+          for (int e = 0; e < 4; e++) part[e] = mfma4(c.kr[0][e].get(mt), c.qr[0][e].get(mt), part[e]);
+        f4 x[VT];
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++) x[nt] = f4{0, 0, 0, 0};
+#pragma unroll
+        for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++)
+#pragma unroll
+            for (int nt = 0; nt < VT; nt++) x[nt] = mfma4(S[mt][nt][e], c.qr[0][e].get(mt), x[nt]);
+        f4 pt;
+#pragma unroll
+        for (int e = 0; e < 4; e++) pt[e] = (part[0][e] + part[1][e]) + (part[2][e] + part[3][e]);
         scores(pt, 0, 0);
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++) entering(x[nt], 0);
         float o[4][VT];
 #pragma unroll
-        for (int nt = 0; nt < VT; nt++) {
-          f4 x = {0, 0, 0, 0};
+        for (int e = 0; e < 4; e++)
 #pragma unroll
-          for (int mt = 0; mt < KT; mt++)
+          for (int nt = 0; nt < VT; nt++) x[nt] = mfma4(c.vc[0][e].get(nt), pt[e], x[nt]);
 #pragma unroll
-            for (int e = 0; e < 4; e++) x = mfma4(S[mt][nt][e], c.qr[0][e].get(mt), x);
-          entering(x, 0);
+        for (int nt = 0; nt < VT; nt++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) x = mfma4(c.vc[0][e].get(nt), pt[e], x);
-#pragma unroll
-          for (int e = 0; e < 4; e++) o[e][nt] = x[e];
-        }
+          for (int e = 0; e < 4; e++) o[e][nt] = x[nt][e];
         put_tile(0, o);
       }
       if (!carried(n)) return true;
