@@ -229,13 +229,6 @@ __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
   typedef __bf16 b2 __attribute__((ext_vector_type(2)));
   return __builtin_bit_cast(unsigned, b2{(__bf16)lo, (__bf16)hi});
 }
-/* hi = the packed leading parts of x0, x1; x0, x1 become the rest */
-__device__ __forceinline__ unsigned split_bf16(float& x0, float& x1) {
-  const unsigned hi = pack_bf16(x0, x1);
-  x0 -= __builtin_bit_cast(float, hi << 16);
-  x1 -= __builtin_bit_cast(float, hi & 0xffff0000u);
-  return hi;
-}
 /* the K = 32 shape throughout, half empty where four elements are all there is: a K = 16 instruction right behind
    a K = 32 one on the same accumulators read them before the first had written (the compiler had put one wait
    state between the two; measured at one tile, where nothing else stands between them) */
@@ -243,27 +236,51 @@ __device__ __forceinline__ f4 mfma32(u4 a, u4 b, f4 c) {
   typedef __bf16 b8 __attribute__((ext_vector_type(8)));
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
-/* the 4 KT elements of a lane's row form, four to a u2: element KT e + mt of group e, tile mt */
-template <int KT, bool VEC> __device__ __forceinline__ void pack_row(const Raw<Bf16, KT, VEC> (&x)[4], u2 (&y)[KT]) {
-  unsigned d[2 * KT];
-  if constexpr (VEC && KT > 1) {
+/* The packed leading parts of four elements that lie as an accumulator does (rows 4 g + e of column idx); x
+   becomes the rest, x - hi, a product with the negative unit matrix: one instruction of the matrix pipe
+   in place of eight of the vector pipe, which is the busier one.  Exact: every sum has one product.  An infinity
+   or a NaN spreads to the rest of its column, whose elements all feed the same result. */
+__device__ __forceinline__ u2 split4(f4& x, u2 minus_one) {
+  const u2 hi = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
+  x = mfma32(u4{minus_one.x, minus_one.y, 0, 0}, u4{hi.x, hi.y, 0, 0}, x);
+  return hi;
+}
+__device__ __forceinline__ u2 pack4(f4 x) { return u2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])}; }
+
+/* Which channels position 4 g + e of N tiles stands for: N consecutive ones from here on.  Groups e lie so that the
+   four lanes of a token read 64 consecutive bytes of its row with each load (C groups of a lane at once, up to
+   16 bytes): half the cache lines a load of 32 bytes a lane would touch. */
+template <class T, int N> struct Place {
+  static constexpr int U = N * (int)sizeof(T), C = U >= 16 ? 1 : U >= 4 ? 16 / U : 4, R = 4 / C;
+  static __device__ __forceinline__ int of(int g, int e) { return N * (e / C * 4 * C + g * C + e % C); }
+};
+/* the row form of a token: channels of(g, 0 .. 3) + 0 .. N - 1 */
+template <class T, int N, bool VEC> struct Row {
+  typedef Place<T, N> P;
+  Raw<T, N * P::C, VEC> x[P::R];
+  __device__ __forceinline__ void load(Rsrc r, const unsigned (&off)[P::R], int g, int dim) {
 #pragma unroll
-    for (int i = 0; i < 2 * KT; i++) d[i] = x[i / (KT / 2)].d[i % (KT / 2)];
-  } else {
-#pragma unroll
-    for (int i = 0; i < 2 * KT; i++) d[i] = x[2 * i / KT].d[2 * i % KT] | x[(2 * i + 1) / KT].d[(2 * i + 1) % KT] << 16;
+    for (int i = 0; i < P::R; i++) x[i].load(r, off[i], dim - P::of(g, i * P::C));
   }
-#pragma unroll
-  for (int i = 0; i < KT; i++) y[i] = u2{d[2 * i], d[2 * i + 1]};
+  __device__ __forceinline__ float get(int e, int mt) const { return x[e / P::C].get(e % P::C * N + mt); }
+};
+/* elements i of x and j of y as two halves */
+template <class X> __device__ __forceinline__ unsigned halves(const X& x, int i, const X& y, int j, bool vec) {
+  if (!vec) return x.d[i] | y.d[j] << 16;
+  if (&x == &y && i + 1 == j && i % 2 == 0) return x.d[i / 2];
+  const unsigned sel = (i & 1 ? 0x0302u : 0x0100u) | (j & 1 ? 0x07060000u : 0x05040000u);
+  return __builtin_amdgcn_perm(y.d[j / 2], x.d[i / 2], sel);
 }
 /* the four tokens of tile nt in the column form */
 template <int VT, bool VEC> __device__ __forceinline__ u2 pack_col(const Raw<Bf16, VT, VEC> (&x)[4], int nt) {
-  if constexpr (VEC && VT > 1) {
-    const unsigned sel = nt & 1 ? 0x07060302u : 0x05040100u; /* the high or the low halves of two dwords */
-    return u2{__builtin_amdgcn_perm(x[1].d[nt / 2], x[0].d[nt / 2], sel), __builtin_amdgcn_perm(x[3].d[nt / 2], x[2].d[nt / 2], sel)};
-  } else {
-    return u2{x[0].d[nt] | x[1].d[nt] << 16, x[2].d[nt] | x[3].d[nt] << 16};
-  }
+  return u2{halves(x[0], nt, x[1], nt, VEC), halves(x[2], nt, x[3], nt, VEC)};
+}
+/* the row form by tiles: e = 0 .. 3 of tile mt, as the rows of an accumulator lie */
+template <int KT, bool VEC> __device__ __forceinline__ void pack_row(const Row<Bf16, KT, VEC>& r, u2 (&y)[KT]) {
+  constexpr int C = Place<Bf16, KT>::C;
+#pragma unroll
+  for (int mt = 0; mt < KT; mt++)
+    y[mt] = u2{halves(r.x[0], mt, r.x[1 / C], 1 % C * KT + mt, VEC), halves(r.x[2 / C], 2 % C * KT + mt, r.x[3 / C], 3 % C * KT + mt, VEC)};
 }
 
 /* KT, VT: tiles of 16 key channels and of 16 value channels per wave.  STATE: only the state at the end of
@@ -306,37 +323,50 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   const long long qst = ES * w.q.st, kst = ES * w.k.st, vst = ES * w.v.st, ost = os * w.o.st;
   const unsigned char* starts = a.starts ? a.starts + b * a.starts_sb : nullptr;
 
-  /* byte offsets of a lane's channels: row form (group e of KT or VT channels at tile width x (4 g + e)) ... */
-  unsigned kd[4], od[4];
+  /* byte offsets of a lane's channels, in the row form and in the column form ... */
+  typedef Place<T, KT> PK;
+  typedef Place<T, VT> PV;
+  unsigned kd[PK::R], od[PV::R];
 #pragma unroll
-  for (int e = 0; e < 4; e++) {
-    const int dk = KT * (4 * g + e), dv = VT * (4 * g + e);
-    kd[e] = at(dk * ES, dk < kdim, FAR_D);
-    od[e] = at(dv * os, dv < vleft, FAR_D);
-  }
-  const unsigned kidx = at(KT * idx * ES, KT * idx < kdim, FAR_D), vidx = at(VT * idx * ES, VT * idx < vleft, FAR_D);
+  for (int i = 0; i < PK::R; i++) kd[i] = at(PK::of(g, i * PK::C) * ES, PK::of(g, i * PK::C) < kdim, FAR_D);
+#pragma unroll
+  for (int i = 0; i < PV::R; i++) od[i] = at(PV::of(g, i * PV::C) * ES, PV::of(g, i * PV::C) < vleft, FAR_D);
+  const int kmine = PK::of(idx >> 2, idx & 3), vmine = PV::of(idx >> 2, idx & 3);
+  const unsigned kidx = at(kmine * ES, kmine < kdim, FAR_D), vidx = at(vmine * ES, vmine < vleft, FAR_D);
   /* ... and of its tokens, for tiles of n: the lowest token of the tile is the base */
-  unsigned qrow[4], krow[4], kcol[4], vcol[4];
+  unsigned qrow[PK::R], krow[PK::R], kcol[4], vcol[4];
   auto place = [&](int n) {
     const unsigned back = n - 1 - idx, rel = rev ? back : idx;
 #pragma unroll
+    for (int i = 0; i < PK::R; i++) {
+      qrow[i] = at(rel * (unsigned)qst, idx < n, FAR_T) + kd[i];
+      krow[i] = at(rel * (unsigned)kst, idx < n, FAR_T) + kd[i];
+    }
+#pragma unroll
     for (int e = 0; e < 4; e++) {
-      qrow[e] = at(rel * (unsigned)qst, idx < n, FAR_T) + kd[e];
-      krow[e] = at(rel * (unsigned)kst, idx < n, FAR_T) + kd[e];
       const int j = 4 * g + e;
       const unsigned backj = n - 1 - j, rc = rev ? backj : j;
       kcol[e] = at(rc * (unsigned)kst, j < n, FAR_T) + kidx;
       vcol[e] = at(rc * (unsigned)vst, j < n, FAR_T) + vidx;
     }
   };
+  /* o[e][nt]: channel of(g, e) + nt of this lane's token */
   auto put = [&](Rsrc ro, unsigned rel, bool there, const float (&o)[4][VT]) {
     const unsigned orow = at(rel * (unsigned)ost, there, FAR_T);
+    if (w.out_f32) {
 #pragma unroll
-    for (int e = 0; e < 4; e++) {
-      const unsigned off = orow + od[e];
-      const int left = vleft - VT * (4 * g + e);
-      if (w.out_f32) store_n<float, VT, VEC>(ro, off, left, o[e]);
-      else store_n<T, VT, VEC>(ro, off, left, o[e]);
+      for (int e = 0; e < 4; e++) {
+        const int d = PV::of(g, e);
+        store_n<float, VT, VEC>(ro, orow + at(4 * d, d < vleft, FAR_D), vleft - d, o[e]);
+      }
+    } else {
+#pragma unroll
+      for (int i = 0; i < PV::R; i++) {
+        float x[VT * PV::C];
+#pragma unroll
+        for (int j = 0; j < VT * PV::C; j++) x[j] = o[i * PV::C + j / VT][j % VT];
+        store_n<T, VT * PV::C, VEC>(ro, orow + od[i], vleft - PV::of(g, i * PV::C), x);
+      }
     }
   };
 
@@ -355,7 +385,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   f4 S[KT][VT];
   const float* s_in = STATE ? nullptr : nsplit > 1 ? w.ws + (bh * nsplit + split) * elems
                                                      : w.s_in ? w.s_in + bh * elems : nullptr;
-  /* S[mt][nt][e]: key channel KT (4 g + e) + mt, value channel v0 + VT idx + nt */
+  /* S[mt][nt][e]: key channel of(g, e) + mt, value channel v0 + of(idx >> 2, idx & 3) + nt */
   const unsigned srow = 4 * (w.state_t ? 1 : vdim), scol = 4 * (w.state_t ? kdim : 1);
   auto state_off = [&](int dk, int dv) {
     return at(dk * srow, dk < kdim, FAR_T) + at((v0 + dv) * scol, dv < vleft, FAR_D);
@@ -368,7 +398,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           Raw<float, VT, true> x;
-          x.load(rs, state_off(KT * (4 * g + e) + mt, VT * idx), VT);
+          x.load(rs, state_off(PK::of(g, e) + mt, vmine), VT);
 #pragma unroll
           for (int nt = 0; nt < VT; nt++) S[mt][nt][e] = x.get(nt);
         }
@@ -378,7 +408,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
         for (int e = 0; e < 4; e++) {
           Raw<float, KT, true> x;
-          x.load(rs, state_off(KT * (4 * g + e), VT * idx + nt), KT);
+          x.load(rs, state_off(PK::of(g, e), vmine + nt), KT);
 #pragma unroll
           for (int mt = 0; mt < KT; mt++) S[mt][nt][e] = x.get(mt);
         }
@@ -390,7 +420,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             Raw<float, 1, true> x;
-            x.load(rs, state_off(KT * (4 * g + e) + mt, VT * idx + nt), 1);
+            x.load(rs, state_off(PK::of(g, e) + mt, vmine + nt), 1);
             S[mt][nt][e] = x.get(0);
           }
     }
@@ -412,6 +442,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
     }
     fi[f] = w.in_scale * pw(l, 16 * f + idx + e0);
   }
+  const unsigned unit = idx >> 2 != g ? 0u : idx & 1 ? 0xbf800000u : 0xbf80u;
+  const u2 minus_one = {idx & 2 ? 0u : unit, idx & 2 ? unit : 0u}; /* this lane's part of the negative unit matrix */
   unsigned causal[4];
 #pragma unroll
   for (int e = 0; e < 4; e++) causal[e] = idx >= 4 * g + e ? 0xffffffffu : 0u;
@@ -433,7 +465,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
     return rev ? len - p - n0 - 16 * f : p + 16 * f;
   };
   struct Chunk {
-    Raw<T, KT, VEC> kr[H][4], qr[H][4], kc[H][4];
+    Row<T, KT, VEC> kr[H], qr[H];
+    Raw<T, KT, VEC> kc[H][4];
     Raw<T, VT, VEC> vc[H][4];
     unsigned start;
   };
@@ -458,18 +491,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       const long long low = low_of(n, f);
       const Rsrc rk = rsrc_of(k + low * kst, there), rv = rsrc_of(v + low * vst, there), rq = rsrc_of(q + low * qst, there);
 #pragma unroll
-      for (int e = 0; e < 4; e++) c.vc[f][e].load(rv, vcol[e], vleft - VT * idx);
+      for (int e = 0; e < 4; e++) c.vc[f][e].load(rv, vcol[e], vleft - vmine);
       if (!STATE) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int left = kdim - KT * (4 * g + e);
-          c.kr[f][e].load(rk, krow[e], left);
-          c.qr[f][e].load(rq, qrow[e], left);
-        }
+        c.kr[f].load(rk, krow, g, kdim);
+        c.qr[f].load(rq, qrow, g, kdim);
       }
       if (STATE || carried(n)) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) c.kc[f][e].load(rk, kcol[e], kdim - KT * idx);
+        for (int e = 0; e < 4; e++) c.kc[f][e].load(rk, kcol[e], kdim - kmine);
       }
     }
   };
@@ -583,17 +612,15 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
             }
         f4 x[H][VT];
 #pragma unroll
-        for (int i = 0; i < KT; i++)
+        for (int mt = 0; mt < KT; mt++)
 #pragma unroll
           for (int nt = 0; nt < VT; nt++) {
-            /* the state's elements of the four channels in qq[.][i] */
-            float s0 = S[4 * i % KT][nt][4 * i / KT], s1 = S[(4 * i + 1) % KT][nt][(4 * i + 1) / KT],
-                  s2 = S[(4 * i + 2) % KT][nt][(4 * i + 2) / KT], s3 = S[(4 * i + 3) % KT][nt][(4 * i + 3) / KT];
-            const unsigned a0 = split_bf16(s0, s1), a1 = split_bf16(s2, s3);
-            const u4 sa = {a0, a1, pack_bf16(s0, s1), pack_bf16(s2, s3)};
+            f4 rest = S[mt][nt];
+            const u2 hi = split4(rest, minus_one), lo = pack4(rest);
 #pragma unroll
             for (int f = 0; f < H; f++)
-              x[f][nt] = mfma32(sa, u4{qq[f][i].x, qq[f][i].y, qq[f][i].x, qq[f][i].y}, i ? x[f][nt] : f4{0, 0, 0, 0});
+              x[f][nt] = mfma32(u4{hi.x, hi.y, lo.x, lo.y}, u4{qq[f][mt].x, qq[f][mt].y, qq[f][mt].x, qq[f][mt].y},
+                                mt ? x[f][nt] : f4{0, 0, 0, 0});
           }
         u2 ph[H][H], pl[H][H]; /* leading part and rest */
 #pragma unroll
@@ -601,10 +628,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
           for (int fk = 0; fk <= fq; fk++) {
             scores(pt[fq][fk], fq, fk);
-            float p0 = pt[fq][fk][0], p1 = pt[fq][fk][1], p2 = pt[fq][fk][2], p3 = pt[fq][fk][3];
-            ph[fq][fk].x = split_bf16(p0, p1);
-            ph[fq][fk].y = split_bf16(p2, p3);
-            pl[fq][fk] = u2{pack_bf16(p0, p1), pack_bf16(p2, p3)};
+            ph[fq][fk] = split4(pt[fq][fk], minus_one);
+            pl[fq][fk] = pack4(pt[fq][fk]);
           }
 #pragma unroll
         for (int f = 0; f < H; f++)
@@ -623,7 +648,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
                               u4{pl[f][0].x, pl[f][0].y, pl[f][f].x, pl[f][f].y}, x[f][nt]);
 #pragma unroll
         for (int f = 0; f < H; f++) {
-          float o[4][VT]; /* o[e][nt]: channel VT (4 g + e) + nt of token 16 f + idx */
+          float o[4][VT];
 #pragma unroll
           for (int nt = 0; nt < VT; nt++)
 #pragma unroll
@@ -635,15 +660,14 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       decay();
 #pragma unroll
       for (int mt = 0; mt < KT; mt++) {
-        float kx[H][4];
+        f4 kx[H];
         u2 kh[H], km[H];
 #pragma unroll
         for (int f = 0; f < H; f++) {
 #pragma unroll
           for (int e = 0; e < 4; e++) kx[f][e] = key(f, mt, e);
-          kh[f].x = split_bf16(kx[f][0], kx[f][1]);
-          kh[f].y = split_bf16(kx[f][2], kx[f][3]);
-          km[f] = u2{pack_bf16(kx[f][0], kx[f][1]), pack_bf16(kx[f][2], kx[f][3])};
+          kh[f] = split4(kx[f], minus_one);
+          km[f] = pack4(kx[f]);
         }
 #pragma unroll
         for (int nt = 0; nt < VT; nt++) {
@@ -664,9 +688,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           u2 kl[H];
 #pragma unroll
           for (int f = 0; f < H; f++) {
-            (void)split_bf16(kx[f][0], kx[f][1]);
-            (void)split_bf16(kx[f][2], kx[f][3]);
-            kl[f] = u2{pack_bf16(kx[f][0], kx[f][1]), pack_bf16(kx[f][2], kx[f][3])};
+            (void)split4(kx[f], minus_one);
+            kl[f] = pack4(kx[f]);
           }
 #pragma unroll
           for (int nt = 0; nt < VT; nt++) {
@@ -682,7 +705,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
         for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) part[e] = mfma4(c.kr[0][e].get(mt), c.qr[0][e].get(mt), part[e]);
+          for (int e = 0; e < 4; e++) part[e] = mfma4(c.kr[0].get(e, mt), c.qr[0].get(e, mt), part[e]);
         f4 x[VT];
 #pragma unroll
         for (int nt = 0; nt < VT; nt++) x[nt] = f4{0, 0, 0, 0};
@@ -691,7 +714,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; e++)
 #pragma unroll
-            for (int nt = 0; nt < VT; nt++) x[nt] = mfma4(S[mt][nt][e], c.qr[0][e].get(mt), x[nt]);
+            for (int nt = 0; nt < VT; nt++) x[nt] = mfma4(S[mt][nt][e], c.qr[0].get(e, mt), x[nt]);
         f4 pt;
 #pragma unroll
         for (int e = 0; e < 4; e++) pt[e] = (part[0][e] + part[1][e]) + (part[2][e] + part[3][e]);
@@ -760,7 +783,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           float x[VT];
 #pragma unroll
           for (int nt = 0; nt < VT; nt++) x[nt] = S[mt][nt][e];
-          store_n<float, VT, true>(rs, state_off(KT * (4 * g + e) + mt, VT * idx), VT, x);
+          store_n<float, VT, true>(rs, state_off(PK::of(g, e) + mt, vmine), VT, x);
         }
     } else if (a.state_vec) {
 #pragma unroll
@@ -770,7 +793,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           float x[KT];
 #pragma unroll
           for (int mt = 0; mt < KT; mt++) x[mt] = S[mt][nt][e];
-          store_n<float, KT, true>(rs, state_off(KT * (4 * g + e), VT * idx + nt), KT, x);
+          store_n<float, KT, true>(rs, state_off(PK::of(g, e), vmine + nt), KT, x);
         }
     } else {
 #pragma unroll
@@ -780,7 +803,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
           for (int e = 0; e < 4; e++) {
             const float x = S[mt][nt][e];
-            store_n<float, 1, true>(rs, state_off(KT * (4 * g + e) + mt, VT * idx + nt), 1, &x);
+            store_n<float, 1, true>(rs, state_off(PK::of(g, e) + mt, vmine + nt), 1, &x);
           }
     }
   }
@@ -1054,10 +1077,10 @@ static void split_use(const ur3e_attn_t* a, const Splits& p, void* ws, Walk& w) 
   w.wf = w.ws + (long long)a->b * a->heads * p.n * a->dk * a->dv;
 }
 
-/* groups of kt channels can be moved whole: all there or none, on their boundary */
-static bool aligned(const Tok& t, int e, int kt, int d) {
-  const int by = kt * e < 16 ? kt * e : 16;
-  return d % kt == 0 && (uintptr_t)t.p % by == 0 && t.sb * e % by == 0 && t.st * e % by == 0 && t.sh * e % by == 0;
+/* n tiles of channels can be moved whole: all of a lane's load there or none of it, and on its boundary */
+static bool aligned(const Tok& t, int e, int n, int d) {
+  const int by = 4 * n * e < 16 ? 4 * n * e : 16, unit = n * e > by ? n : by / e;
+  return d % unit == 0 && (uintptr_t)t.p % by == 0 && t.sb * e % by == 0 && t.st * e % by == 0 && t.sh * e % by == 0;
 }
 
 /* what a launch does: the states at the ends of the splits and their join, or the outputs */
@@ -1103,7 +1126,7 @@ template <class T, int KT, int VT> static int walk_vec(WalkArgs& a, Phase phase,
       a.state_vec = 0;
     vec = vec && aligned(w.k, sizeof(T), KT, a.kdim) && aligned(w.v, sizeof(T), VT, a.vdim);
     if (phase == OUTPUTS)
-      vec = vec && aligned(w.q, sizeof(T), KT, a.kdim) && aligned(w.o, w.out_f32 ? 4 : (int)sizeof(T), VT, a.vdim);
+      vec = vec && aligned(w.q, sizeof(T), KT, a.kdim) && (w.out_f32 || aligned(w.o, sizeof(T), VT, a.vdim));
   }
   return vec ? walk_launch<T, KT, VT, true>(a, phase, s) : walk_launch<T, KT, VT, false>(a, phase, s);
 }
