@@ -128,6 +128,12 @@ __device__ __forceinline__ f4 mfma4(float a, float b, f4 c) { return __builtin_a
 #define FAR_T 0x80000000u
 #define FAR_D 0x40000000u
 typedef __amdgpu_buffer_rsrc_t Rsrc;
+/* The value, opaque from here on: what a rare branch derives from it is computed there, not kept in registers
+   through the loop around the branch. */
+__device__ __forceinline__ int fresh(int x) {
+  asm volatile("" : "+v"(x));
+  return x;
+}
 __device__ __forceinline__ unsigned at(unsigned off, bool there, unsigned far) { return there ? off : far; }
 __device__ __forceinline__ Rsrc rsrc_of(const void* p, bool there = true) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, there ? (int)FAR_D : 0, 0x00027000);
@@ -284,8 +290,9 @@ template <int KT, bool VEC> __device__ __forceinline__ void pack_row(const Row<B
 }
 
 /* KT, VT: tiles of 16 key channels and of 16 value channels per wave.  STATE: only the state at the end of
-   each split (from zero), for sequences that several waves share. */
-template <class T, int KT, int VT, bool VEC, bool STATE, int H>
+   each split (from zero), for sequences that several waves share.  FINE (bfloat16): a state leaves as floats and is
+   summed to their precision, from keys in three parts; where it only feeds 16-bit outputs, from keys in two. */
+template <class T, int KT, int VT, bool VEC, bool STATE, int H, bool FINE>
 __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   constexpr int ES = (int)sizeof(T), C = 16 * H;
   static_assert(H == 1 || __is_same(T, Bf16), "two tiles of tokens: bfloat16 only");
@@ -326,21 +333,19 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   /* byte offsets of a lane's channels, in the row form and in the column form ... */
   typedef Place<T, KT> PK;
   typedef Place<T, VT> PV;
-  unsigned kd[PK::R], od[PV::R];
-#pragma unroll
-  for (int i = 0; i < PK::R; i++) kd[i] = at(PK::of(g, i * PK::C) * ES, PK::of(g, i * PK::C) < kdim, FAR_D);
-#pragma unroll
-  for (int i = 0; i < PV::R; i++) od[i] = at(PV::of(g, i * PV::C) * ES, PV::of(g, i * PV::C) < vleft, FAR_D);
   const int kmine = PK::of(idx >> 2, idx & 3), vmine = PV::of(idx >> 2, idx & 3);
-  const unsigned kidx = at(kmine * ES, kmine < kdim, FAR_D), vidx = at(vmine * ES, vmine < vleft, FAR_D);
   /* ... and of its tokens, for tiles of n: the lowest token of the tile is the base */
   unsigned qrow[PK::R], krow[PK::R], kcol[4], vcol[4];
   auto place = [&](int n) {
+    const int idx = fresh(lane & 15), g = fresh(lane >> 4), kmine = PK::of(idx >> 2, idx & 3), vmine = PV::of(idx >> 2, idx & 3);
     const unsigned back = n - 1 - idx, rel = rev ? back : idx;
+    const unsigned kidx = at(kmine * ES, kmine < kdim, FAR_D), vidx = at(vmine * ES, vmine < vleft, FAR_D);
 #pragma unroll
     for (int i = 0; i < PK::R; i++) {
-      qrow[i] = at(rel * (unsigned)qst, idx < n, FAR_T) + kd[i];
-      krow[i] = at(rel * (unsigned)kst, idx < n, FAR_T) + kd[i];
+      const int d = PK::of(g, i * PK::C);
+      const unsigned kd = at(d * ES, d < kdim, FAR_D);
+      qrow[i] = at(rel * (unsigned)qst, idx < n, FAR_T) + kd;
+      krow[i] = at(rel * (unsigned)kst, idx < n, FAR_T) + kd;
     }
 #pragma unroll
     for (int e = 0; e < 4; e++) {
@@ -365,7 +370,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         float x[VT * PV::C];
 #pragma unroll
         for (int j = 0; j < VT * PV::C; j++) x[j] = o[i * PV::C + j / VT][j % VT];
-        store_n<T, VT * PV::C, VEC>(ro, orow + od[i], vleft - PV::of(g, i * PV::C), x);
+        const int d = PV::of(g, i * PV::C);
+        store_n<T, VT * PV::C, VEC>(ro, orow + at(d * ES, d < vleft, FAR_D), vleft - d, x);
       }
     }
   };
@@ -432,7 +438,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   }
 
   const int e0 = rev ? 0 : 1; /* the entering state has decayed by one step at position 0, or by none yet */
-  float dm[H][4], wk[H][4], fi[H]; /* dm[x]: from a key to a query x tiles behind it */
+  float dm[H][4], wk[4]; /* dm[x]: from a key to a query x tiles behind it; wk: from a key of the last tile to the end */
 #pragma unroll
   for (int f = 0; f < H; f++) {
 #pragma unroll
@@ -440,13 +446,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       const int d = 16 * f + idx - (4 * g + e);
       dm[f][e] = d >= 0 ? w.p_scale * pw(l, d) : 0.0f;
     }
-    fi[f] = w.in_scale * pw(l, 16 * f + idx + e0);
   }
+  const float fi = w.in_scale * pw(l, idx + e0), g16 = pw(l, 16);
   const unsigned unit = idx >> 2 != g ? 0u : idx & 1 ? 0xbf800000u : 0xbf80u;
   const u2 minus_one = {idx & 2 ? 0u : unit, idx & 2 ? unit : 0u}; /* this lane's part of the negative unit matrix */
-  unsigned causal[4];
-#pragma unroll
-  for (int e = 0; e < 4; e++) causal[e] = idx >= 4 * g + e ? 0xffffffffu : 0u;
   float gn = 1.0f;
 
   float through = 1.0f; /* STATE: what the split multiplies an entering state by */
@@ -456,9 +459,6 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   /* whether anything reads the state behind the chunk */
   const bool kept = STATE || (split == nsplit - 1 && w.s_out);
   auto carried = [&](int n) { return kept || p + n < hi; };
-  /* a state that leaves as floats is summed to their precision; one that only feeds 16-bit outputs, from keys
-     in two parts */
-  const bool fine = w.s_out != nullptr;
   /* the lowest token of tile f of the chunk */
   auto low_of = [&](int n, int f) -> long long {
     const int n0 = n < 16 ? n : 16;
@@ -470,16 +470,24 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
     Raw<T, VT, VEC> vc[H][4];
     unsigned start;
   };
+  /* The keys' column form is the state's, which is done last: where registers are short it is read behind the
+     scores, from the cache lines that the row form brought. */
+  constexpr bool LATE = H == 2;
+  auto load_columns = [&](Chunk& c, Rsrc rk, int f) {
+    if (STATE || carried(n)) {
+#pragma unroll
+      for (int e = 0; e < 4; e++) c.kc[f][e].load(rk, kcol[e], kdim - kmine);
+    }
+  };
   auto load = [&](Chunk& c, int p, int n) {
     const int n0 = n < 16 ? n : 16;
     if (n0 != placed) {
       placed = n0;
       place(n0);
     }
-    c.start = 0;
-    if (starts) {
+    {
       /* position x of a reversed walk is token len - 1 - x, behind the start that token len - x may carry */
-      const Rsrc rs = rsrc_of(starts + (rev ? len - p - n + 1 : p) * starts_st);
+      const Rsrc rs = rsrc_of(starts + (rev ? len - p - n + 1 : p) * starts_st, starts != nullptr);
       const int i = lane & (C - 1);
       const bool there = (i < n) & ((p + i != 0) | !rev);
       const unsigned back = n - 1 - i, rel = rev ? back : i;
@@ -496,10 +504,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         c.kr[f].load(rk, krow, g, kdim);
         c.qr[f].load(rq, qrow, g, kdim);
       }
-      if (STATE || carried(n)) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) c.kc[f][e].load(rk, kcol[e], kdim - kmine);
-      }
+      if (STATE || !LATE) load_columns(c, rk, f);
     }
   };
   /* one chunk; false: it holds a value that is not finite and has to be taken token by token */
@@ -507,13 +512,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
     if (n != scaled) {
       scaled = n;
       gn = pw(l, n);
+      const int n0 = n > 16 ? 16 : n, j0 = fresh(4 * g);
 #pragma unroll
-      for (int f = 0; f < H; f++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          const int j = 16 * f + 4 * g + e;
-          wk[f][e] = j < n ? w.w_scale * pw(l, n - 1 - j + (1 - e0)) : 0.0f;
-        }
+      for (int e = 0; e < 4; e++) {
+        const int j = j0 + e;
+        wk[e] = j < n0 ? w.w_scale * pw(l, n0 - 1 - j + (1 - e0)) : 0.0f;
+      }
     }
     /* a value that is not finite must not meet the zeros of the mask (0 * inf): its chunk is taken token by
        token, where every product belongs to the token */
@@ -527,30 +531,27 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
     if (n > 1 && __any(peak.not_finite())) return false;
 
     /* bit i: an episode starts between positions i - 1 and i.  Most chunks have none, and skip what a start cuts. */
-    const unsigned brk = starts ? (unsigned)__ballot(c.start != 0) & (unsigned)((1ull << C) - 1) : 0u;
+    const unsigned brk = (unsigned)__ballot(c.start != 0) & (unsigned)((1ull << C) - 1);
     const bool cut = brk != 0;
-    auto upto = [&](int f) { return (2u << (16 * f + idx)) - 1u; }; /* breaks at or in front of a query */
-    /* the scores of query tile fi with key tile fj: masked and decayed (pt[e]: query idx, key 4 g + e) */
+    auto upto = [&](int f) { return (2u << (16 * f + fresh(idx))) - 1u; }; /* breaks at or in front of a query */
+    /* the scores of query tile fq with key tile fk: decayed, later keys masked (pt[e]: query idx, key 4 g + e) */
     auto scores = [&](f4& pt, int fq, int fk) {
 #pragma unroll
       for (int e = 0; e < 4; e++) {
         const float x = pt[e] * dm[fq - fk][e];
-        /* a mask of bits, not a select: a select by VCC takes six times an AND here */
-        pt[e] = fq != fk ? x : __builtin_bit_cast(float, __builtin_bit_cast(unsigned, x) & causal[e]);
-      }
-      if (cut) {
-#pragma unroll
-        for (int e = 0; e < 4; e++) pt[e] = (brk & upto(fq) & ~((2u << (16 * fk + 4 * g + e)) - 1u)) == 0 ? pt[e] : 0.0f;
+        /* the sign of the distance as a mask of bits, not a select: a select by VCC takes six times an AND here */
+        const int later = (idx - 4 * g - e) >> 31;
+        pt[e] = fq != fk ? x : __builtin_bit_cast(float, __builtin_bit_cast(int, x) & ~later);
       }
     };
-    /* the read-out of the entering state */
-    auto entering = [&](f4& x, int f) {
+    /* a start between key and query, or in front of the query: no score, nothing from the entering state */
+    auto cut_scores = [&](f4& pt, int fq, int fk) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) x[e] *= fi[f];
-      if (cut) {
+      for (int e = 0; e < 4; e++) pt[e] = (brk & upto(fq) & ~((2u << (16 * fk + fresh(4 * g) + e)) - 1u)) == 0 ? pt[e] : 0.0f;
+    };
+    auto cut_entering = [&](f4& x, int f) {
 #pragma unroll
-        for (int e = 0; e < 4; e++) x[e] = (brk & upto(f)) == 0 ? x[e] : 0.0f;
-      }
+      for (int e = 0; e < 4; e++) x[e] = (brk & upto(f)) == 0 ? x[e] : 0.0f;
     };
     auto decay = [&] {
       if (cut) {
@@ -563,7 +564,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         for (int f = 0; f < H; f++)
 #pragma unroll
           for (int e = 0; e < 4; e++) {
-            const int j = 16 * f + 4 * g + e;
+            const int j = 16 * f + fresh(4 * g) + e;
             const bool ok = (brk & ~((2u << j) - 1u)) == 0;
 #pragma unroll
             for (int i = 0; i < Raw<T, KT, VEC>::D; i++) c.kc[f][e].d[i] = ok ? c.kc[f][e].d[i] : 0;
@@ -577,7 +578,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
             for (int e = 0; e < 4; e++) S[mt][nt][e] *= gn;
       }
     };
-    auto key = [&](int f, int mt, int e) { return c.kc[f][e].get(mt) * wk[f][e]; }; /* as it enters the state */
+    const float ahead = H == 2 && n > 16 ? g16 : 1.0f; /* tile 0, where another one follows */
+    auto key = [&](int f, int mt, int e) { /* as it enters the state */
+      return c.kc[f][e].get(mt) * (f == H - 1 ? wk[e] : wk[e] * ahead);
+    };
     auto put_tile = [&](int f, const float (&o)[4][VT]) {
       const int n0 = n < 16 ? n : 16;
       put(rsrc_of(out + low_of(n, f) * ost, 16 * f < n), rev ? n0 - 1 - idx : idx, idx < n0, o);
@@ -612,7 +616,8 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
             }
         f4 x[H][VT];
 #pragma unroll
-        for (int mt = 0; mt < KT; mt++)
+        for (int mt = 0; mt < KT; mt++) {
+          
 #pragma unroll
           for (int nt = 0; nt < VT; nt++) {
             f4 rest = S[mt][nt];
@@ -622,12 +627,33 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
               x[f][nt] = mfma32(u4{hi.x, hi.y, lo.x, lo.y}, u4{qq[f][mt].x, qq[f][mt].y, qq[f][mt].x, qq[f][mt].y},
                                 mt ? x[f][nt] : f4{0, 0, 0, 0});
           }
+        }
+        
+#pragma unroll
+        for (int f = 0; f < H; f++) {
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++) x[f][nt] *= f ? fi * g16 : fi;
+#pragma unroll
+          for (int fk = 0; fk <= f; fk++) scores(pt[f][fk], f, fk);
+        }
+        if constexpr (LATE) {
+#pragma unroll
+          for (int f = 0; f < H; f++) load_columns(c, rsrc_of(k + low_of(n, f) * kst, 16 * f < n), f);
+        }
+        if (cut) {
+#pragma unroll
+          for (int f = 0; f < H; f++) {
+#pragma unroll
+            for (int nt = 0; nt < VT; nt++) cut_entering(x[f][nt], f);
+#pragma unroll
+            for (int fk = 0; fk <= f; fk++) cut_scores(pt[f][fk], f, fk);
+          }
+        }
         u2 ph[H][H], pl[H][H]; /* leading part and rest */
 #pragma unroll
         for (int fq = 0; fq < H; fq++)
 #pragma unroll
           for (int fk = 0; fk <= fq; fk++) {
-            scores(pt[fq][fk], fq, fk);
             ph[fq][fk] = split4(pt[fq][fk], minus_one);
             pl[fq][fk] = pack4(pt[fq][fk]);
           }
@@ -635,7 +661,6 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         for (int f = 0; f < H; f++)
 #pragma unroll
           for (int nt = 0; nt < VT; nt++) {
-            entering(x[f][nt], f);
             const u2 y = vq[0][nt], yf = vq[f][nt], z = ph[f][0], zl = pl[f][0], zf = ph[f][f];
             if (f == 0) x[f][nt] = mfma32(u4{y.x, y.y, y.x, y.y}, u4{z.x, z.y, zl.x, zl.y}, x[f][nt]);
             else x[f][nt] = mfma32(u4{y.x, y.y, yf.x, yf.y}, u4{z.x, z.y, zf.x, zf.y}, x[f][nt]);
@@ -646,6 +671,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           for (int nt = 0; nt < VT; nt++)
             x[f][nt] = mfma32(u4{vq[0][nt].x, vq[0][nt].y, vq[f][nt].x, vq[f][nt].y},
                               u4{pl[f][0].x, pl[f][0].y, pl[f][f].x, pl[f][f].y}, x[f][nt]);
+        
 #pragma unroll
         for (int f = 0; f < H; f++) {
           float o[4][VT];
@@ -660,6 +686,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       decay();
 #pragma unroll
       for (int mt = 0; mt < KT; mt++) {
+        
         f4 kx[H];
         u2 kh[H], km[H];
 #pragma unroll
@@ -684,7 +711,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
             S[mt][nt] = mfma32(u4{km[0].x, km[0].y, km[1].x, km[1].y},
                                u4{vq[0][nt].x, vq[0][nt].y, vq[1][nt].x, vq[1][nt].y}, S[mt][nt]);
         }
-        if (fine) {
+        if constexpr (FINE) {
           u2 kl[H];
 #pragma unroll
           for (int f = 0; f < H; f++) {
@@ -720,7 +747,12 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         for (int e = 0; e < 4; e++) pt[e] = (part[0][e] + part[1][e]) + (part[2][e] + part[3][e]);
         scores(pt, 0, 0);
 #pragma unroll
-        for (int nt = 0; nt < VT; nt++) entering(x[nt], 0);
+        for (int nt = 0; nt < VT; nt++) x[nt] *= fi;
+        if (cut) {
+          cut_scores(pt, 0, 0);
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++) cut_entering(x[nt], 0);
+        }
         float o[4][VT];
 #pragma unroll
         for (int e = 0; e < 4; e++)
@@ -1086,6 +1118,20 @@ static bool aligned(const Tok& t, int e, int n, int d) {
 /* what a launch does: the states at the ends of the splits and their join, or the outputs */
 enum Phase { STATES, OUTPUTS };
 
+template <class T, int KT, int VT, bool VEC, bool STATE>
+static void walk_kernel(const WalkArgs& a, bool fine, dim3 grid, dim3 block, hipStream_t s) {
+  if constexpr (__is_same(T, Bf16)) {
+    /* two tiles of tokens at a time where there is more than one */
+    if (a.t > 16) {
+      if (fine) hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, STATE, 2, true>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, STATE, 2, false>), grid, block, 0, s, a);
+      return;
+    }
+  }
+  /* (splits, and with them STATE, are for longer sequences) */
+  if constexpr (!STATE || !__is_same(T, Bf16))
+    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, STATE, 1, true>), grid, block, 0, s, a);
+}
 template <class T, int KT, int VT, bool VEC> static int walk_launch(WalkArgs& a, Phase phase, hipStream_t s) {
   const long long streams = (long long)a.b * a.h * a.nw * a.slabs;
   /* the waves that share a sequence's tensors in one workgroup, where they are at most four */
@@ -1093,10 +1139,10 @@ template <class T, int KT, int VT, bool VEC> static int walk_launch(WalkArgs& a,
   a.near = (share + waves - 1) / waves;
   const long long tasks = streams * (phase == STATES ? a.nsplit - 1 : a.nsplit), per = 8LL * a.near * waves;
   const dim3 grid((unsigned)((tasks + per - 1) / per * 8 * a.near)), block(64 * waves);
-  /* bfloat16 sequences of more than one tile of tokens go two tiles at a time */
-  constexpr int H = __is_same(T, Bf16) ? 2 : 1;
+  bool fine = false;
+  for (int i = 0; i < a.nw; i++) fine = fine || a.w[i].s_out;
   if (phase == STATES) {
-    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, true, H>), grid, block, 0, s, a);
+    walk_kernel<T, KT, VT, VEC, true>(a, fine, grid, block, s);
     PL_CHK(hipGetLastError());
     const int elems = a.kdim * a.vdim;
     const unsigned bh = (unsigned)(a.b * a.h), nw = (unsigned)a.nw;
@@ -1104,10 +1150,8 @@ template <class T, int KT, int VT, bool VEC> static int walk_launch(WalkArgs& a,
       hipLaunchKernelGGL((k_attn_join<4, 8>), dim3((elems + 255) / 256, bh, nw), dim3(64), 0, s, a);
     else
       hipLaunchKernelGGL((k_attn_join<1, 32>), dim3((elems + 63) / 64, bh, nw), dim3(64), 0, s, a);
-  } else if (H == 2 && (a.nsplit > 1 || a.t > 16)) {
-    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false, H>), grid, block, 0, s, a);
   } else {
-    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, false, 1>), grid, block, 0, s, a);
+    walk_kernel<T, KT, VT, VEC, false>(a, fine, grid, block, s);
   }
   PL_CHK(hipGetLastError());
   return UR3E_OK;
