@@ -53,12 +53,13 @@ int ur3e_attn_forward(const ur3e_attn_t* a, const ur3e_tokens_t* out, float* s_o
                       size_t workspace_bytes, void* stream);
 
 /* Gradients of a forward call with the same `a`: dout [b][t][heads][dv] and ds_out (null: 0) in; dq, dk, dv
-   (shaped as q, k, v; dk and dv summed over the query heads that share them) and ds0 (or null) out. */
+   (shaped as q, k, v; dk and dv summed over the query heads that share them) and ds0 (or null) out.
+   workspace: ur3e_attn_workspace(a, 1) bytes. */
 int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dout, const float* ds_out,
                        const ur3e_tokens_t* dq, const ur3e_tokens_t* dk, const ur3e_tokens_t* dv, float* ds0,
                        void* workspace, size_t workspace_bytes, void* stream);
 
-/* bytes of workspace the two calls above need */
+/* bytes of workspace that the forward (backward = 0) or the backward call needs */
 int ur3e_attn_workspace(const ur3e_attn_t* a, int backward, size_t* bytes);
 
 /* One token (a->t must be 1): state_in -> state_out (the same buffer, two that do not overlap, or

@@ -95,7 +95,7 @@ struct Tok {
 struct Walk {
   Tok q, k, v, o;           /* o.p is written */
   const float* s_in;        /* [b][h][dk * dv] or null */
-  float* s_out;             /* or null */
+  float* s_out;             /* or null (always where state_t) */
   float* ws;                /* nsplit > 1: [b][h][split][kdim * vdim], split s holds the state that enters it, */
   float* wf;                /* and [b][h][split], what split s - 1 multiplies the state by */
   int state_t;              /* a [dk][dv] state is this walk's transposed: kdim = dv */
@@ -109,7 +109,6 @@ struct WalkArgs {
   int b, t, h, kdim, vdim, slabs, nsplit, split_len;
   int near; /* consecutive workgroups that share a sequence's tensors */
   int chunk;     /* 16, or 1 where tokens lie too far apart for 30-bit offsets inside a chunk */
-  int state_vec; /* states may be moved KT or VT floats at a time */
   const float* log_decay;
   const unsigned char* starts;
   long long starts_sb, starts_st;
@@ -139,71 +138,56 @@ __device__ __forceinline__ Rsrc rsrc_of(const void* p, bool there = true) {
   return __builtin_amdgcn_make_buffer_rsrc(const_cast<void*>(p), (short)0, there ? (int)FAR_D : 0, 0x00027000);
 }
 
-/* N consecutive elements as dwords; VEC: aligned to min(16, N * sizeof(T)) bytes and all there or none, else
-   one element to a dword, `left` of them there */
-template <class T, int N, bool VEC> struct Raw {
-  static constexpr int B = N * (int)sizeof(T);
-  static constexpr int D = VEC ? (B + 3) / 4 : N;
+/* N consecutive elements as dwords, on any boundary of an element */
+template <class T, int N> struct Raw {
+  static constexpr int B = N * (int)sizeof(T), D = (B + 3) / 4;
   unsigned d[D];
-  __device__ __forceinline__ void load(Rsrc r, unsigned off, int left) {
-    if constexpr (VEC) {
-      if constexpr (B == 2) d[0] = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
-      else if constexpr (B == 4) d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
-      else if constexpr (B == 8) {
-        const u2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
-        d[0] = x.x; d[1] = x.y;
-      } else {
-#pragma unroll
-        for (int i = 0; i < B / 16; i++) {
-          const u4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * i, 0, 0);
-          d[4 * i] = x.x; d[4 * i + 1] = x.y; d[4 * i + 2] = x.z; d[4 * i + 3] = x.w;
-        }
-      }
+  __device__ __forceinline__ void load(Rsrc r, unsigned off) {
+    if constexpr (B == 2) d[0] = __builtin_amdgcn_raw_buffer_load_b16(r, off, 0, 0);
+    else if constexpr (B == 4) d[0] = __builtin_amdgcn_raw_buffer_load_b32(r, off, 0, 0);
+    else if constexpr (B == 8) {
+      const u2 x = __builtin_amdgcn_raw_buffer_load_b64(r, off, 0, 0);
+      d[0] = x.x; d[1] = x.y;
     } else {
 #pragma unroll
-      for (int i = 0; i < N; i++) {
-        const unsigned o = at(off + i * (int)sizeof(T), i < left, FAR_T);
-        if constexpr (sizeof(T) == 2) d[i] = __builtin_amdgcn_raw_buffer_load_b16(r, o, 0, 0);
-        else d[i] = __builtin_amdgcn_raw_buffer_load_b32(r, o, 0, 0);
+      for (int i = 0; i < B / 16; i++) {
+        const u4 x = __builtin_amdgcn_raw_buffer_load_b128(r, off + 16 * i, 0, 0);
+        d[4 * i] = x.x; d[4 * i + 1] = x.y; d[4 * i + 2] = x.z; d[4 * i + 3] = x.w;
       }
+    }
+  }
+  /* zeros for the first n elements (n <= 0: none) */
+  __device__ __forceinline__ void clear(int n) {
+#pragma unroll
+    for (int i = 0; i < D; i++) {
+      if constexpr (sizeof(T) == 4) d[i] = i < n ? 0 : d[i];
+      else d[i] &= 2 * i + 1 < n ? 0u : 2 * i < n ? 0xffff0000u : 0xffffffffu;
     }
   }
   __device__ __forceinline__ float get(int i) const {
     if constexpr (sizeof(T) == 4) return __builtin_bit_cast(float, d[i]);
-    else {
-      const unsigned short h = VEC ? (unsigned short)(d[i / 2] >> (16 * (i & 1))) : (unsigned short)d[i];
-      return to_f(__builtin_bit_cast(T, h));
-    }
+    else return to_f(__builtin_bit_cast(T, (unsigned short)(d[i / 2] >> (16 * (i & 1)))));
   }
 };
-template <class T, int N, bool VEC> __device__ __forceinline__ void store_n(Rsrc r, unsigned off, int left, const float* x) {
-  if constexpr (VEC) {
-    constexpr int B = N * (int)sizeof(T);
-    unsigned d[(B + 3) / 4] = {};
+template <class T, int N> __device__ __forceinline__ void store_n(Rsrc r, unsigned off, const float* x) {
+  constexpr int B = N * (int)sizeof(T);
+  unsigned d[(B + 3) / 4] = {};
 #pragma unroll
-    for (int i = 0; i < N; i += sizeof(T) == 4 ? 1 : 2) {
-      if constexpr (sizeof(T) == 4) d[i] = __builtin_bit_cast(unsigned, x[i]);
-      else if constexpr (N == 1) d[0] = __builtin_bit_cast(unsigned short, from_f<T>(x[0]));
-      else {
-        struct Two { T a, b; };
-        d[i / 2] = __builtin_bit_cast(unsigned, Two{from_f<T>(x[i]), from_f<T>(x[i + 1])});
-      }
-    }
-    if constexpr (B == 2) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)d[0], r, off, 0, 0);
-    else if constexpr (B == 4) __builtin_amdgcn_raw_buffer_store_b32(d[0], r, off, 0, 0);
-    else if constexpr (B == 8) __builtin_amdgcn_raw_buffer_store_b64(u2{d[0], d[1]}, r, off, 0, 0);
+  for (int i = 0; i < N; i += sizeof(T) == 4 ? 1 : 2) {
+    if constexpr (sizeof(T) == 4) d[i] = __builtin_bit_cast(unsigned, x[i]);
+    else if constexpr (N == 1) d[0] = __builtin_bit_cast(unsigned short, from_f<T>(x[0]));
     else {
-#pragma unroll
-      for (int i = 0; i < B / 16; i++)
-        __builtin_amdgcn_raw_buffer_store_b128(u4{d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]}, r, off + 16 * i, 0, 0);
+      struct Two { T a, b; };
+      d[i / 2] = __builtin_bit_cast(unsigned, Two{from_f<T>(x[i]), from_f<T>(x[i + 1])});
     }
-  } else {
+  }
+  if constexpr (B == 2) __builtin_amdgcn_raw_buffer_store_b16((unsigned short)d[0], r, off, 0, 0);
+  else if constexpr (B == 4) __builtin_amdgcn_raw_buffer_store_b32(d[0], r, off, 0, 0);
+  else if constexpr (B == 8) __builtin_amdgcn_raw_buffer_store_b64(u2{d[0], d[1]}, r, off, 0, 0);
+  else {
 #pragma unroll
-    for (int i = 0; i < N; i++) {
-      const unsigned o = at(off + i * (int)sizeof(T), i < left, FAR_T);
-      if constexpr (sizeof(T) == 4) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(unsigned, x[i]), r, o, 0, 0);
-      else __builtin_amdgcn_raw_buffer_store_b16(__builtin_bit_cast(unsigned short, from_f<T>(x[i])), r, o, 0, 0);
-    }
+    for (int i = 0; i < B / 16; i++)
+      __builtin_amdgcn_raw_buffer_store_b128(u4{d[4 * i], d[4 * i + 1], d[4 * i + 2], d[4 * i + 3]}, r, off + 16 * i, 0, 0);
   }
 }
 
@@ -253,46 +237,54 @@ __device__ __forceinline__ u2 split4(f4& x, u2 minus_one) {
 }
 __device__ __forceinline__ u2 pack4(f4 x) { return u2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])}; }
 
-/* Which channels position 4 g + e of N tiles stands for: N consecutive ones from here on.  Groups e lie so that the
-   four lanes of a token read 64 consecutive bytes of its row with each load (C groups of a lane at once, up to
-   16 bytes): half the cache lines a load of 32 bytes a lane would touch. */
+/* Which channels position 4 g + e of N tiles stands for: N consecutive ones from `of` on.  Groups e lie so that the
+   four lanes of a token read 64 consecutive bytes of its row with each load (C groups of a lane at once, NC channels,
+   up to 16 bytes): half the cache lines a load of 32 bytes a lane would touch.
+   The lanes' NC channels number NC (4 (e / C) + g) on; where dim ends inside them they are taken from dim - NC on
+   instead, so that no load leaves its row.  The channels that come twice then are harmless as values (the
+   same results are stored twice); as keys they are zeros (`own` tells which), and so are their rows of the state. */
 template <class T, int N> struct Place {
-  static constexpr int U = N * (int)sizeof(T), C = U >= 16 ? 1 : U >= 4 ? 16 / U : 4, R = 4 / C;
-  static __device__ __forceinline__ int of(int g, int e) { return N * (e / C * 4 * C + g * C + e % C); }
+  static constexpr int U = N * (int)sizeof(T), C = U >= 16 ? 1 : U >= 4 ? 16 / U : 4, R = 4 / C, NC = N * C;
+  static __device__ __forceinline__ int first(int g, int e) { return NC * (e / C * 4 + g); }
+  static __device__ __forceinline__ bool there(int g, int e, int dim) { return first(g, e) < dim; }
+  /* low: the first channel there is (rows of less than NC are copied into wider ones and start there) */
+  static __device__ __forceinline__ int of(int g, int e, int dim, int low = 0) {
+    const int f = first(g, e), last = dim - NC < f ? dim - NC : f;
+    return (last > low ? last : low) + e % C * N;
+  }
 };
 /* the row form of a token: channels of(g, 0 .. 3) + 0 .. N - 1 */
-template <class T, int N, bool VEC> struct Row {
+template <class T, int N> struct Row {
   typedef Place<T, N> P;
-  Raw<T, N * P::C, VEC> x[P::R];
-  __device__ __forceinline__ void load(Rsrc r, const unsigned (&off)[P::R], int g, int dim) {
+  Raw<T, N * P::C> x[P::R];
+  __device__ __forceinline__ void load(Rsrc r, const unsigned (&off)[P::R]) {
 #pragma unroll
-    for (int i = 0; i < P::R; i++) x[i].load(r, off[i], dim - P::of(g, i * P::C));
+    for (int i = 0; i < P::R; i++) x[i].load(r, off[i]);
   }
   __device__ __forceinline__ float get(int e, int mt) const { return x[e / P::C].get(e % P::C * N + mt); }
 };
 /* elements i of x and j of y as two halves */
-template <class X> __device__ __forceinline__ unsigned halves(const X& x, int i, const X& y, int j, bool vec) {
-  if (!vec) return x.d[i] | y.d[j] << 16;
+template <class X> __device__ __forceinline__ unsigned halves(const X& x, int i, const X& y, int j) {
   if (&x == &y && i + 1 == j && i % 2 == 0) return x.d[i / 2];
   const unsigned sel = (i & 1 ? 0x0302u : 0x0100u) | (j & 1 ? 0x07060000u : 0x05040000u);
   return __builtin_amdgcn_perm(y.d[j / 2], x.d[i / 2], sel);
 }
 /* the four tokens of tile nt in the column form */
-template <int VT, bool VEC> __device__ __forceinline__ u2 pack_col(const Raw<Bf16, VT, VEC> (&x)[4], int nt) {
-  return u2{halves(x[0], nt, x[1], nt, VEC), halves(x[2], nt, x[3], nt, VEC)};
+template <int VT> __device__ __forceinline__ u2 pack_col(const Raw<Bf16, VT> (&x)[4], int nt) {
+  return u2{halves(x[0], nt, x[1], nt), halves(x[2], nt, x[3], nt)};
 }
 /* the row form by tiles: e = 0 .. 3 of tile mt, as the rows of an accumulator lie */
-template <int KT, bool VEC> __device__ __forceinline__ void pack_row(const Row<Bf16, KT, VEC>& r, u2 (&y)[KT]) {
+template <int KT> __device__ __forceinline__ void pack_row(const Row<Bf16, KT>& r, u2 (&y)[KT]) {
   constexpr int C = Place<Bf16, KT>::C;
 #pragma unroll
   for (int mt = 0; mt < KT; mt++)
-    y[mt] = u2{halves(r.x[0], mt, r.x[1 / C], 1 % C * KT + mt, VEC), halves(r.x[2 / C], 2 % C * KT + mt, r.x[3 / C], 3 % C * KT + mt, VEC)};
+    y[mt] = u2{halves(r.x[0], mt, r.x[1 / C], 1 % C * KT + mt), halves(r.x[2 / C], 2 % C * KT + mt, r.x[3 / C], 3 % C * KT + mt)};
 }
 
 /* KT, VT: tiles of 16 key channels and of 16 value channels per wave.  STATE: only the state at the end of
    each split (from zero), for sequences that several waves share.  FINE (bfloat16): a state leaves as floats and is
    summed to their precision, from keys in three parts; where it only feeds 16-bit outputs, from keys in two. */
-template <class T, int KT, int VT, bool VEC, bool STATE, int H, bool FINE>
+template <class T, int KT, int VT, bool STATE, int H, bool FINE>
 __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   constexpr int ES = (int)sizeof(T), C = 16 * H;
   static_assert(H == 1 || __is_same(T, Bf16), "two tiles of tokens: bfloat16 only");
@@ -324,26 +316,25 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   const bool rev = w.reversed;
   const char* q = (const char*)w.q.p + ES * (b * w.q.sb + (h / w.q.hdiv) * w.q.sh);
   const char* k = (const char*)w.k.p + ES * (b * w.k.sb + (h / w.k.hdiv) * w.k.sh);
-  const char* v = (const char*)w.v.p + ES * (b * w.v.sb + (h / w.v.hdiv) * w.v.sh + v0);
+  const char* v = (const char*)w.v.p + ES * (b * w.v.sb + (h / w.v.hdiv) * w.v.sh);
   const int os = w.out_f32 ? 4 : ES;
-  char* out = (char*)const_cast<void*>(w.o.p) + os * (b * w.o.sb + (h / w.o.hdiv) * w.o.sh + v0);
+  char* out = (char*)const_cast<void*>(w.o.p) + os * (b * w.o.sb + (h / w.o.hdiv) * w.o.sh);
   const long long qst = ES * w.q.st, kst = ES * w.k.st, vst = ES * w.v.st, ost = os * w.o.st;
   const unsigned char* starts = a.starts ? a.starts + b * a.starts_sb : nullptr;
 
-  /* byte offsets of a lane's channels, in the row form and in the column form ... */
+  /* byte offsets of a lane's channels and tokens, in the row form and in the column form, for tiles of n: the lowest
+     token of the tile is the base */
   typedef Place<T, KT> PK;
   typedef Place<T, VT> PV;
-  const int kmine = PK::of(idx >> 2, idx & 3), vmine = PV::of(idx >> 2, idx & 3);
-  /* ... and of its tokens, for tiles of n: the lowest token of the tile is the base */
   unsigned qrow[PK::R], krow[PK::R], kcol[4], vcol[4];
   auto place = [&](int n) {
-    const int idx = fresh(lane & 15), g = fresh(lane >> 4), kmine = PK::of(idx >> 2, idx & 3), vmine = PV::of(idx >> 2, idx & 3);
+    const int idx = fresh(lane & 15), g = fresh(lane >> 4), gi = idx >> 2, ei = idx & 3;
     const unsigned back = n - 1 - idx, rel = rev ? back : idx;
-    const unsigned kidx = at(kmine * ES, kmine < kdim, FAR_D), vidx = at(vmine * ES, vmine < vleft, FAR_D);
+    const unsigned kidx = at(PK::of(gi, ei, kdim) * ES, PK::there(gi, ei, kdim), FAR_D);
+    const unsigned vidx = at((v0 + PV::of(gi, ei, vleft, -v0)) * ES, PV::there(gi, ei, vleft), FAR_D);
 #pragma unroll
     for (int i = 0; i < PK::R; i++) {
-      const int d = PK::of(g, i * PK::C);
-      const unsigned kd = at(d * ES, d < kdim, FAR_D);
+      const unsigned kd = at(PK::of(g, i * PK::C, kdim) * ES, PK::there(g, i * PK::C, kdim), FAR_D);
       qrow[i] = at(rel * (unsigned)qst, idx < n, FAR_T) + kd;
       krow[i] = at(rel * (unsigned)kst, idx < n, FAR_T) + kd;
     }
@@ -360,18 +351,15 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
     const unsigned orow = at(rel * (unsigned)ost, there, FAR_T);
     if (w.out_f32) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) {
-        const int d = PV::of(g, e);
-        store_n<float, VT, VEC>(ro, orow + at(4 * d, d < vleft, FAR_D), vleft - d, o[e]);
-      }
+      for (int e = 0; e < 4; e++)
+        store_n<float, VT>(ro, orow + at(4 * (v0 + PV::of(g, e, vleft, -v0)), PV::there(g, e, vleft), FAR_D), o[e]);
     } else {
 #pragma unroll
       for (int i = 0; i < PV::R; i++) {
-        float x[VT * PV::C];
+        float x[PV::NC];
 #pragma unroll
-        for (int j = 0; j < VT * PV::C; j++) x[j] = o[i * PV::C + j / VT][j % VT];
-        const int d = PV::of(g, i * PV::C);
-        store_n<T, VT * PV::C, VEC>(ro, orow + at(d * ES, d < vleft, FAR_D), vleft - d, x);
+        for (int j = 0; j < PV::NC; j++) x[j] = o[i * PV::C + j / VT][j % VT];
+        store_n<T, PV::NC>(ro, orow + at((v0 + PV::of(g, i * PV::C, vleft, -v0)) * ES, PV::there(g, i * PV::C, vleft), FAR_D), x);
       }
     }
   };
@@ -391,44 +379,44 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   f4 S[KT][VT];
   const float* s_in = STATE ? nullptr : nsplit > 1 ? w.ws + (bh * nsplit + split) * elems
                                                      : w.s_in ? w.s_in + bh * elems : nullptr;
-  /* S[mt][nt][e]: key channel of(g, e) + mt, value channel v0 + of(idx >> 2, idx & 3) + nt */
+  /* S[mt][nt][e]: key channel of(g, e) + mt, value channel of this lane's column + nt */
+  const int vcolumn = v0 + PV::of(idx >> 2, idx & 3, vleft, -v0);
+  const bool vthere = PV::there(idx >> 2, idx & 3, vleft) & (vcolumn < vdim);
   const unsigned srow = 4 * (w.state_t ? 1 : vdim), scol = 4 * (w.state_t ? kdim : 1);
-  auto state_off = [&](int dk, int dv) {
-    return at(dk * srow, dk < kdim, FAR_T) + at((v0 + dv) * scol, dv < vleft, FAR_D);
+  auto own = [&](int e, int mt) {
+    const int d = PK::of(g, e, kdim) + mt;
+    return (d >= PK::first(g, e)) & (d < kdim);
   };
   if (s_in) {
     const Rsrc rs = rsrc_of(s_in);
-    if (a.state_vec && !w.state_t) {
+    if (!w.state_t) {
 #pragma unroll
       for (int mt = 0; mt < KT; mt++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          Raw<float, VT, true> x;
-          x.load(rs, state_off(PK::of(g, e) + mt, vmine), VT);
+          Raw<float, VT> x;
+          x.load(rs, at((PK::of(g, e, kdim) + mt) * srow, own(e, mt), FAR_T) + at(vcolumn * scol, vthere, FAR_D));
 #pragma unroll
           for (int nt = 0; nt < VT; nt++) S[mt][nt][e] = x.get(nt);
         }
-    } else if (a.state_vec) {
+    } else {
 #pragma unroll
       for (int nt = 0; nt < VT; nt++)
 #pragma unroll
         for (int e = 0; e < 4; e++) {
-          Raw<float, KT, true> x;
-          x.load(rs, state_off(PK::of(g, e), vmine + nt), KT);
+          Raw<float, KT> x;
+          x.load(rs, at(PK::of(g, e, kdim) * srow, PK::there(g, e, kdim) & (PK::of(g, e, kdim) < kdim), FAR_T) + at((vcolumn + nt) * scol, vthere, FAR_D));
 #pragma unroll
           for (int mt = 0; mt < KT; mt++) S[mt][nt][e] = x.get(mt);
         }
-    } else {
+      if (kdim % PK::NC) {
 #pragma unroll
-      for (int mt = 0; mt < KT; mt++)
+        for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-        for (int nt = 0; nt < VT; nt++)
+          for (int e = 0; e < 4; e++)
 #pragma unroll
-          for (int e = 0; e < 4; e++) {
-            Raw<float, 1, true> x;
-            x.load(rs, state_off(PK::of(g, e) + mt, vmine + nt), 1);
-            S[mt][nt][e] = x.get(0);
-          }
+            for (int nt = 0; nt < VT; nt++) S[mt][nt][e] = own(e, mt) ? S[mt][nt][e] : 0.0f;
+      }
     }
   } else {
 #pragma unroll
@@ -465,9 +453,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
     return rev ? len - p - n0 - 16 * f : p + 16 * f;
   };
   struct Chunk {
-    Row<T, KT, VEC> kr[H], qr[H];
-    Raw<T, KT, VEC> kc[H][4];
-    Raw<T, VT, VEC> vc[H][4];
+    Row<T, KT> kr[H], qr[H];
+    Raw<T, KT> kc[H][4];
+    Raw<T, VT> vc[H][4];
     unsigned start;
   };
   /* The keys' column form is the state's, which is done last: where registers are short it is read behind the
@@ -476,8 +464,17 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   auto load_columns = [&](Chunk& c, Rsrc rk, int f) {
     if (STATE || carried(n)) {
 #pragma unroll
-      for (int e = 0; e < 4; e++) c.kc[f][e].load(rk, kcol[e], kdim - kmine);
+      for (int e = 0; e < 4; e++) c.kc[f][e].load(rk, kcol[e]);
     }
+  };
+  const int twice = kdim > PK::NC && kdim % PK::NC ? PK::NC - kdim % PK::NC : 0;
+  auto clear_columns = [&](Chunk& c) {
+    const int gi = fresh(idx >> 2), ei = idx & 3;
+    const int n = ei / PK::C * 4 + gi == kdim / PK::NC ? twice - ei % PK::C * KT : 0;
+#pragma unroll
+    for (int f = 0; f < H; f++)
+#pragma unroll
+      for (int e = 0; e < 4; e++) c.kc[f][e].clear(n);
   };
   auto load = [&](Chunk& c, int p, int n) {
     const int n0 = n < 16 ? n : 16;
@@ -499,10 +496,10 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       const long long low = low_of(n, f);
       const Rsrc rk = rsrc_of(k + low * kst, there), rv = rsrc_of(v + low * vst, there), rq = rsrc_of(q + low * qst, there);
 #pragma unroll
-      for (int e = 0; e < 4; e++) c.vc[f][e].load(rv, vcol[e], vleft - vmine);
+      for (int e = 0; e < 4; e++) c.vc[f][e].load(rv, vcol[e]);
       if (!STATE) {
-        c.kr[f].load(rk, krow, g, kdim);
-        c.qr[f].load(rq, qrow, g, kdim);
+        c.kr[f].load(rk, krow);
+        c.qr[f].load(rq, qrow);
       }
       if (STATE || !LATE) load_columns(c, rk, f);
     }
@@ -527,8 +524,21 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
       for (int e = 0; e < 4; e++)
 #pragma unroll
-        for (int i = 0; i < Raw<T, VT, VEC>::D; i++) peak.add(c.vc[f][e].d[i]);
+        for (int i = 0; i < Raw<T, VT>::D; i++) peak.add(c.vc[f][e].d[i]);
     if (n > 1 && __any(peak.not_finite())) return false;
+
+    /* key channels that come twice */
+    if (twice) {
+      const int g = fresh(lane >> 4);
+      if constexpr (!STATE) {
+#pragma unroll
+        for (int i = 0; i < PK::R; i++)
+          if (i == kdim / PK::NC / 4)
+#pragma unroll
+            for (int f = 0; f < H; f++) c.kr[f].x[i].clear(g == kdim / PK::NC % 4 ? twice : 0);
+      }
+      if (!LATE || STATE) clear_columns(c);
+    }
 
     /* bit i: an episode starts between positions i - 1 and i.  Most chunks have none, and skip what a start cuts. */
     const unsigned brk = (unsigned)__ballot(c.start != 0) & (unsigned)((1ull << C) - 1);
@@ -567,7 +577,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
             const int j = 16 * f + fresh(4 * g) + e;
             const bool ok = (brk & ~((2u << j) - 1u)) == 0;
 #pragma unroll
-            for (int i = 0; i < Raw<T, KT, VEC>::D; i++) c.kc[f][e].d[i] = ok ? c.kc[f][e].d[i] : 0;
+            for (int i = 0; i < Raw<T, KT>::D; i++) c.kc[f][e].d[i] = ok ? c.kc[f][e].d[i] : 0;
           }
       } else {
 #pragma unroll
@@ -591,13 +601,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
       for (int f = 0; f < H; f++)
 #pragma unroll
-        for (int nt = 0; nt < VT; nt++) vq[f][nt] = pack_col<VT, VEC>(c.vc[f], nt);
+        for (int nt = 0; nt < VT; nt++) vq[f][nt] = pack_col<VT>(c.vc[f], nt);
       if (!STATE) {
         u2 kq[H][KT], qq[H][KT];
 #pragma unroll
         for (int f = 0; f < H; f++) {
-          pack_row<KT, VEC>(c.kr[f], kq[f]);
-          pack_row<KT, VEC>(c.qr[f], qq[f]);
+          pack_row<KT>(c.kr[f], kq[f]);
+          pack_row<KT>(c.qr[f], qq[f]);
         }
         /* Instructions that add to the same accumulators stand apart by those of the other tiles. */
         f4 pt[H][H]; /* [query tile][key tile] */
@@ -639,6 +649,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         if constexpr (LATE) {
 #pragma unroll
           for (int f = 0; f < H; f++) load_columns(c, rsrc_of(k + low_of(n, f) * kst, 16 * f < n), f);
+          if (twice) clear_columns(c);
         }
         if (cut) {
 #pragma unroll
@@ -807,37 +818,45 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         for (int nt = 0; nt < VT; nt++) S[mt][nt] = f4{0, 0, 0, 0};
     }
     const Rsrc rs = rsrc_of(s_out);
-    if (a.state_vec && !w.state_t) {
+    /* (the walks on transposed states only read them) */
 #pragma unroll
-      for (int mt = 0; mt < KT; mt++)
+    for (int mt = 0; mt < KT; mt++)
 #pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float x[VT];
+      for (int e = 0; e < 4; e++) {
+        float x[VT];
 #pragma unroll
-          for (int nt = 0; nt < VT; nt++) x[nt] = S[mt][nt][e];
-          store_n<float, VT, true>(rs, state_off(PK::of(g, e) + mt, vmine), VT, x);
-        }
-    } else if (a.state_vec) {
+        for (int nt = 0; nt < VT; nt++) x[nt] = S[mt][nt][e];
+        store_n<float, VT>(rs, at((PK::of(g, e, kdim) + mt) * srow, own(e, mt), FAR_T) + at(vcolumn * scol, vthere, FAR_D), x);
+      }
+  }
+}
+
+/* Rows of less than four channels, which no lane's load fits, are copied into rows of eight, padded with zeros;
+   padding tokens are left out.  A thread moves a row. */
+struct PackArgs {
+  struct One {
+    Tok src;
+    void* dst;
+    int heads, d;
+  } x[4];
+  int b, t;
+  const int* lengths;
+};
+template <class T> __global__ __launch_bounds__(256) void k_attn_pack(PackArgs a) {
+  const PackArgs::One x = a.x[blockIdx.y];
+  const unsigned long long n = (unsigned long long)a.b * a.t * x.heads;
+  struct alignas(16) Whole { T e[8]; };
+  for (unsigned long long i = (unsigned long long)blockIdx.x * 256 + threadIdx.x; i < n; i += (unsigned long long)gridDim.x * 256) {
+    unsigned long long r = i;
+    const int h = (int)(r % x.heads);
+    r /= x.heads;
+    const int t = (int)(r % a.t), b = (int)(r / a.t);
+    if (a.lengths && t >= a.lengths[b]) continue;
+    const T* src = (const T*)x.src.p + b * x.src.sb + t * x.src.st + h * x.src.sh;
+    Whole y;
 #pragma unroll
-      for (int nt = 0; nt < VT; nt++)
-#pragma unroll
-        for (int e = 0; e < 4; e++) {
-          float x[KT];
-#pragma unroll
-          for (int mt = 0; mt < KT; mt++) x[mt] = S[mt][nt][e];
-          store_n<float, KT, true>(rs, state_off(PK::of(g, e), vmine + nt), KT, x);
-        }
-    } else {
-#pragma unroll
-      for (int mt = 0; mt < KT; mt++)
-#pragma unroll
-        for (int nt = 0; nt < VT; nt++)
-#pragma unroll
-          for (int e = 0; e < 4; e++) {
-            const float x = S[mt][nt][e];
-            store_n<float, 1, true>(rs, state_off(PK::of(g, e) + mt, vmine + nt), 1, &x);
-          }
-    }
+    for (int e = 0; e < 8; e++) y.e[e] = e < x.d ? src[e] : from_f<T>(0.0f);
+    reinterpret_cast<Whole*>(x.dst)[i] = y;
   }
 }
 
@@ -884,24 +903,26 @@ template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(Wal
   }
 }
 
-/* sums of the per-query-head gradients over the heads that share a key / value head: [b][t][h][d] floats to
-   [b][t][hk][d], VW channels a thread */
+/* Sums of the per-query-head gradients over the `grp` heads that share a key / value head: rows of `width` floats,
+   [b][t][hk][grp][width], to `groups` x VW channels of [b][t][hk] rows.  With grp = 1 it narrows the rows of less
+   than four channels that the walks write eight wide. */
 template <class T, int VW>
 __global__ __launch_bounds__(256) void k_attn_group_sum(const float* __restrict__ src, T* __restrict__ dst, unsigned t,
-                                                        unsigned hk, unsigned grp, unsigned groups, unsigned n, long long sb,
-                                                        long long st, long long sh) {
+                                                        unsigned hk, unsigned grp, unsigned groups, unsigned width, unsigned n,
+                                                        long long sb, long long st, long long sh) {
   struct alignas(4 * VW) Pack { float x[VW]; };
   for (unsigned long long i0 = (unsigned long long)blockIdx.x * 256; i0 < n; i0 += (unsigned long long)gridDim.x * 256) {
     const unsigned i = (unsigned)i0 + threadIdx.x;
     if (i >= n) return;
     unsigned r = i / groups;
-    const unsigned c = (i - r * groups) * VW, kh = r % hk;
+    const unsigned c = (i - r * groups) * VW;
+    const float* s = src + (long long)r * grp * width + c;
+    const unsigned kh = r % hk;
     r /= hk;
     const unsigned tt = r % t, bb = r / t;
-    const float* s = src + ((long long)r * hk + kh) * grp * (groups * VW) + c;
     float x[VW] = {};
     for (unsigned k = 0; k < grp; k++) {
-      const Pack y = *reinterpret_cast<const Pack*>(s + (long long)k * groups * VW);
+      const Pack y = *reinterpret_cast<const Pack*>(s + (long long)k * width);
 #pragma unroll
       for (int e = 0; e < VW; e++) x[e] += y.x[e];
     }
@@ -1050,6 +1071,9 @@ static int attn_check(const ur3e_attn_t* a) {
   if (a->dk < 1 || a->dk > UR3E_ATTN_MAX_DIM || a->dv < 1 || a->dv > UR3E_ATTN_MAX_DIM)
     return bad_arg("attention: dk and dv must be in [1, 128]");
   if ((long long)a->b * a->heads > 4194303) return bad_arg("attention: b * heads must be below 2^22");
+  /* 32-bit indices in k_attn_group_sum */
+  if ((a->heads != a->kv_heads || a->dk < 4 || a->dv < 4) && (long long)a->b * a->t * a->heads * UR3E_ATTN_MAX_DIM > 0xffffff00LL)
+    return bad_arg("attention: too many tokens for shared heads or for less than 4 channels");
   if (a->b == 0) return UR3E_OK;
   if (a->q.st < 0 || a->k.st < 0 || a->v.st < 0 || a->starts_st < 0) return bad_arg("attention: token strides must not be negative");
   if (!a->log_decay) return bad_arg("attention: null log_decay");
@@ -1109,30 +1133,27 @@ static void split_use(const ur3e_attn_t* a, const Splits& p, void* ws, Walk& w) 
   w.wf = w.ws + (long long)a->b * a->heads * p.n * a->dk * a->dv;
 }
 
-/* n tiles of channels can be moved whole: all of a lane's load there or none of it, and on its boundary */
-static bool aligned(const Tok& t, int e, int n, int d) {
-  const int by = 4 * n * e < 16 ? 4 * n * e : 16, unit = n * e > by ? n : by / e;
-  return d % unit == 0 && (uintptr_t)t.p % by == 0 && t.sb * e % by == 0 && t.st * e % by == 0 && t.sh * e % by == 0;
-}
+/* the rows hold a lane's load (Place::NC is 4 for up to 16 channels) */
+static bool whole(int d) { return d >= 4; }
 
 /* what a launch does: the states at the ends of the splits and their join, or the outputs */
 enum Phase { STATES, OUTPUTS };
 
-template <class T, int KT, int VT, bool VEC, bool STATE>
+template <class T, int KT, int VT, bool STATE>
 static void walk_kernel(const WalkArgs& a, bool fine, dim3 grid, dim3 block, hipStream_t s) {
   if constexpr (__is_same(T, Bf16)) {
     /* two tiles of tokens at a time where there is more than one */
     if (a.t > 16) {
-      if (fine) hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, STATE, 2, true>), grid, block, 0, s, a);
-      else hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, STATE, 2, false>), grid, block, 0, s, a);
+      if (fine) hipLaunchKernelGGL((k_attn_walk<T, KT, VT, STATE, 2, true>), grid, block, 0, s, a);
+      else hipLaunchKernelGGL((k_attn_walk<T, KT, VT, STATE, 2, false>), grid, block, 0, s, a);
       return;
     }
   }
   /* (splits, and with them STATE, are for longer sequences) */
   if constexpr (!STATE || !__is_same(T, Bf16))
-    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, VEC, STATE, 1, true>), grid, block, 0, s, a);
+    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, STATE, 1, true>), grid, block, 0, s, a);
 }
-template <class T, int KT, int VT, bool VEC> static int walk_launch(WalkArgs& a, Phase phase, hipStream_t s) {
+template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase phase, hipStream_t s) {
   const long long streams = (long long)a.b * a.h * a.nw * a.slabs;
   /* the waves that share a sequence's tensors in one workgroup, where they are at most four */
   const int share = a.nw * a.slabs, waves = share <= 4 ? share : 4;
@@ -1142,23 +1163,23 @@ template <class T, int KT, int VT, bool VEC> static int walk_launch(WalkArgs& a,
   bool fine = false;
   for (int i = 0; i < a.nw; i++) fine = fine || a.w[i].s_out;
   if (phase == STATES) {
-    walk_kernel<T, KT, VT, VEC, true>(a, fine, grid, block, s);
+    walk_kernel<T, KT, VT, true>(a, fine, grid, block, s);
     PL_CHK(hipGetLastError());
     const int elems = a.kdim * a.vdim;
     const unsigned bh = (unsigned)(a.b * a.h), nw = (unsigned)a.nw;
-    if (a.state_vec && elems % 4 == 0 && (long long)bh * nw * elems >= 64 * 4096)
+    bool four = elems % 4 == 0;
+    for (int i = 0; i < a.nw; i++) four = four && (uintptr_t)a.w[i].s_in % 16 == 0 && (uintptr_t)a.w[i].ws % 16 == 0;
+    if (four && (long long)bh * nw * elems >= 64 * 4096)
       hipLaunchKernelGGL((k_attn_join<4, 8>), dim3((elems + 255) / 256, bh, nw), dim3(64), 0, s, a);
     else
       hipLaunchKernelGGL((k_attn_join<1, 32>), dim3((elems + 63) / 64, bh, nw), dim3(64), 0, s, a);
   } else {
-    walk_kernel<T, KT, VT, VEC, false>(a, fine, grid, block, s);
+    walk_kernel<T, KT, VT, false>(a, fine, grid, block, s);
   }
   PL_CHK(hipGetLastError());
   return UR3E_OK;
 }
-template <class T, int KT, int VT> static int walk_vec(WalkArgs& a, Phase phase, hipStream_t s) {
-  bool vec = true;
-  a.state_vec = 1;
+template <class T, int KT, int VT> static int walk_tile(WalkArgs& a, Phase phase, hipStream_t s) {
   a.chunk = 16;
   /* a tile's tokens (a chunk's starts) within its 30-bit offsets, else token by token */
   const long long far = ((1LL << 30) - 1024) / 64;
@@ -1166,18 +1187,13 @@ template <class T, int KT, int VT> static int walk_vec(WalkArgs& a, Phase phase,
   for (int i = 0; i < a.nw; i++) {
     const Walk& w = a.w[i];
     if (w.q.st > far || w.k.st > far || w.v.st > far || w.o.st > far) a.chunk = 1;
-    if ((w.state_t ? a.kdim % KT : a.vdim % VT) || (uintptr_t)w.s_in % 16 || (uintptr_t)w.s_out % 16 || (uintptr_t)w.ws % 16)
-      a.state_vec = 0;
-    vec = vec && aligned(w.k, sizeof(T), KT, a.kdim) && aligned(w.v, sizeof(T), VT, a.vdim);
-    if (phase == OUTPUTS)
-      vec = vec && aligned(w.q, sizeof(T), KT, a.kdim) && (w.out_f32 || aligned(w.o, sizeof(T), VT, a.vdim));
   }
-  return vec ? walk_launch<T, KT, VT, true>(a, phase, s) : walk_launch<T, KT, VT, false>(a, phase, s);
+  return walk_launch<T, KT, VT>(a, phase, s);
 }
 template <class T, int KT> static int walk_vt(WalkArgs& a, int vt, Phase phase, hipStream_t s) {
-  if (vt == 1) return walk_vec<T, KT, 1>(a, phase, s);
-  if (vt == 2) return walk_vec<T, KT, 2>(a, phase, s);
-  if constexpr (KT < 8) return walk_vec<T, KT, 4>(a, phase, s);
+  if (vt == 1) return walk_tile<T, KT, 1>(a, phase, s);
+  if (vt == 2) return walk_tile<T, KT, 2>(a, phase, s);
+  if constexpr (KT < 8) return walk_tile<T, KT, 4>(a, phase, s);
   return bad_arg("attention: no such tile");
 }
 template <class T> static int walk_kt(WalkArgs& a, const Tiles& p, Phase phase, hipStream_t s) {
@@ -1210,19 +1226,126 @@ static WalkArgs args_of(const ur3e_attn_t* a, int kdim, int vdim, const Splits& 
 
 static size_t up256(size_t x) { return (x + 255) / 256 * 256; }
 
-static size_t attn_bytes(const ur3e_attn_t* a, int backward) {
-  if (a->b == 0) return 0;
-  if (!backward) return split_bytes(a, splits_of(a, 0));
-  size_t n = 2 * up256(split_bytes(a, splits_of(a, 1)));
-  if (a->heads != a->kv_heads) n += up256((size_t)a->b * a->t * a->heads * a->dk * 4) + up256((size_t)a->b * a->t * a->heads * a->dv * 4);
-  return n;
+/* The tokens of a call as the walks read them: in place, or as copies behind `used` bytes of the workspace. */
+struct Packer {
+  const ur3e_attn_t* a;
+  char* ws = nullptr;
+  size_t used = 0;
+  PackArgs args = {};
+  int n = 0;
+  long long most = 0;
+  Tok use(const ur3e_tokens_t& x, int heads, int d, int hdiv) {
+    Tok t = tok_of(x, hdiv);
+    const int e = elem_size(a->dtype);
+    if (whole(d) || a->t == 0) return t;
+    PackArgs::One& o = args.x[n++];
+    o.src = t;
+    o.dst = ws + used;
+    o.heads = heads; o.d = d;
+    const long long rows = (long long)a->b * a->t * heads;
+    if (rows > most) most = rows;
+    used += up256((size_t)rows * 8 * e);
+    return Tok{o.dst, (long long)a->t * heads * 8, (long long)heads * 8, 8, hdiv};
+  }
+  int run(hipStream_t s) {
+    if (!n) return UR3E_OK;
+    args.b = a->b; args.t = a->t; args.lengths = a->lengths;
+    const long long blocks = (most + 255) / 256;
+    const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20), n);
+    if (a->dtype == UR3E_F32) hipLaunchKernelGGL(k_attn_pack<float>, grid, dim3(256), 0, s, args);
+    else if (a->dtype == UR3E_BF16) hipLaunchKernelGGL(k_attn_pack<Bf16>, grid, dim3(256), 0, s, args);
+    else hipLaunchKernelGGL(k_attn_pack<F16>, grid, dim3(256), 0, s, args);
+    PL_CHK(hipGetLastError());
+    return UR3E_OK;
+  }
+};
+
+/* An output that the walks write as float rows of their own: one a query head for gradients of shared heads, eight
+   wide for rows that hold no lane's store. */
+struct Wide {
+  const ur3e_attn_t* a;
+  float* p = nullptr;
+  int d = 0, grp = 1, width = 0;
+  ur3e_tokens_t to = {};
+  /* the walk's output: `x` itself or these rows, `used` bytes into the workspace */
+  Tok use(const ur3e_tokens_t& x, int channels, int heads_per, char* ws, size_t& used) {
+    if (heads_per == 1 && whole(channels)) return tok_of(x, 1);
+    d = channels; grp = heads_per; to = x;
+    width = whole(d) ? d : 8;
+    p = (float*)(ws + used);
+    used += up256((size_t)a->b * a->t * a->heads * width * 4);
+    return Tok{p, (long long)a->t * a->heads * width, (long long)a->heads * width, width, 1};
+  }
+  template <class T> void launch(hipStream_t s) const {
+    const int vw = d % 4 == 0 ? 4 : 1;
+    const unsigned hk = a->heads / grp;
+    const long long n = (long long)a->b * a->t * hk * (d / vw), blocks = (n + 255) / 256;
+    const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
+    if (vw == 4)
+      hipLaunchKernelGGL((k_attn_group_sum<T, 4>), grid, dim3(256), 0, s, p, (T*)to.p, (unsigned)a->t, hk, (unsigned)grp, (unsigned)(d / 4), (unsigned)width, (unsigned)n, to.sb, to.st, to.sh);
+    else
+      hipLaunchKernelGGL((k_attn_group_sum<T, 1>), grid, dim3(256), 0, s, p, (T*)to.p, (unsigned)a->t, hk, (unsigned)grp, (unsigned)d, (unsigned)width, (unsigned)n, to.sb, to.st, to.sh);
+  }
+  int finish(hipStream_t s) const {
+    if (!width || a->t == 0) return UR3E_OK;
+    if (a->dtype == UR3E_F32) launch<float>(s);
+    else if (a->dtype == UR3E_BF16) launch<Bf16>(s);
+    else launch<F16>(s);
+    PL_CHK(hipGetLastError());
+    return UR3E_OK;
+  }
+};
+
+/* The workspace of a call: the states of its splits, its wide outputs, its copied inputs. */
+struct ForwardSpace {
+  Splits p;
+  size_t used;
+  Wide out;
+  Packer pack;
+  Tok q, k, v, o;
+  ForwardSpace(const ur3e_attn_t* a, const ur3e_tokens_t& to, void* ws) : p(splits_of(a, 0)), out{a}, pack{a} {
+    const int grp = a->heads / a->kv_heads;
+    used = up256(split_bytes(a, p));
+    o = out.use(to, a->dv, 1, (char*)ws, used);
+    pack.ws = (char*)ws; pack.used = used;
+    q = pack.use(a->q, a->heads, a->dk, 1); k = pack.use(a->k, a->kv_heads, a->dk, grp); v = pack.use(a->v, a->kv_heads, a->dv, grp);
+    used = pack.used;
+  }
+};
+struct BackwardSpace {
+  Splits p;
+  size_t states, used; /* bytes of one walk's states, of everything */
+  Wide wq, wk, wv;
+  Packer pack;
+  Tok q, k, v, dout, dq, dk, dv;
+  BackwardSpace(const ur3e_attn_t* a, const ur3e_tokens_t& g, const ur3e_tokens_t& tq, const ur3e_tokens_t& tk,
+                const ur3e_tokens_t& tv, void* ws)
+      : p(splits_of(a, 1)), wq{a}, wk{a}, wv{a}, pack{a} {
+    const int grp = a->heads / a->kv_heads;
+    states = up256(split_bytes(a, p));
+    used = 2 * states;
+    dq = wq.use(tq, a->dk, 1, (char*)ws, used);
+    dk = wk.use(tk, a->dk, grp, (char*)ws, used);
+    dv = wv.use(tv, a->dv, grp, (char*)ws, used);
+    pack.ws = (char*)ws; pack.used = used;
+    q = pack.use(a->q, a->heads, a->dk, 1); k = pack.use(a->k, a->kv_heads, a->dk, grp); v = pack.use(a->v, a->kv_heads, a->dv, grp);
+    dout = pack.use(g, a->heads, a->dv, 1);
+    used = pack.used;
+  }
+};
+
+static int space_check(size_t need, const void* ws, size_t bytes) {
+  if (bytes < need || (need && !ws)) return bad_arg("attention: workspace too small");
+  if ((uintptr_t)ws % 16) return bad_arg("attention: workspace must be on a boundary of 16 bytes");
+  return UR3E_OK;
 }
 
 extern "C" int ur3e_attn_workspace(const ur3e_attn_t* a, int backward, size_t* bytes) {
   const int rc = attn_check(a);
   if (rc) return rc;
   if (!bytes) return bad_arg("attention: null bytes");
-  *bytes = attn_bytes(a, backward);
+  const ur3e_tokens_t any = {};
+  *bytes = a->b == 0 ? 0 : backward ? BackwardSpace(a, any, any, any, any, nullptr).used : ForwardSpace(a, any, nullptr).used;
   return UR3E_OK;
 }
 
@@ -1233,32 +1356,27 @@ extern "C" int ur3e_attn_forward(const ur3e_attn_t* a, const ur3e_tokens_t* out,
   if (a->b == 0) return UR3E_OK;
   if (!out || (a->t > 0 && !out->p)) return bad_arg("attention: null out");
   if (out->st < 0) return bad_arg("attention: token strides must not be negative");
-  if (workspace_bytes < attn_bytes(a, 0) || (attn_bytes(a, 0) && !workspace)) return bad_arg("attention: workspace too small");
-  const Splits p = splits_of(a, 0);
-  WalkArgs w = args_of(a, a->dk, a->dv, p);
-  const int grp = a->heads / a->kv_heads;
+  ForwardSpace ws(a, *out, workspace);
+  rc = space_check(ws.used, workspace, workspace_bytes);
+  if (rc) return rc;
+  hipStream_t s = (hipStream_t)stream;
+  rc = ws.pack.run(s);
+  if (rc) return rc;
+  WalkArgs w = args_of(a, a->dk, a->dv, ws.p);
   w.nw = 1;
   Walk& f = w.w[0];
-  f.q = tok_of(a->q, 1); f.k = tok_of(a->k, grp); f.v = tok_of(a->v, grp); f.o = tok_of(*out, 1);
+  f.q = ws.q; f.k = ws.k; f.v = ws.v; f.o = ws.o;
+  f.out_f32 = ws.out.width != 0;
   f.s_in = a->s0; f.s_out = s_out;
   f.in_scale = f.p_scale = a->scale; f.w_scale = 1.0f;
-  split_use(a, p, workspace, f);
-  if (p.n > 1) {
-    rc = walk_run(a->dtype, w, STATES, (hipStream_t)stream);
+  split_use(a, ws.p, workspace, f);
+  if (ws.p.n > 1) {
+    rc = walk_run(a->dtype, w, STATES, s);
     if (rc) return rc;
   }
-  return walk_run(a->dtype, w, OUTPUTS, (hipStream_t)stream);
-}
-
-template <class T> static void group_sum(const ur3e_attn_t* a, const float* src, const ur3e_tokens_t& d, int c, hipStream_t s) {
-  const int vw = c % 4 == 0 ? 4 : 1;
-  const long long n = (long long)a->b * a->t * a->kv_heads * (c / vw), blocks = (n + 255) / 256;
-  const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
-  const unsigned grp = a->heads / a->kv_heads;
-  if (vw == 4)
-    hipLaunchKernelGGL((k_attn_group_sum<T, 4>), grid, dim3(256), 0, s, src, (T*)d.p, (unsigned)a->t, (unsigned)a->kv_heads, grp, (unsigned)(c / 4), (unsigned)n, d.sb, d.st, d.sh);
-  else
-    hipLaunchKernelGGL((k_attn_group_sum<T, 1>), grid, dim3(256), 0, s, src, (T*)d.p, (unsigned)a->t, (unsigned)a->kv_heads, grp, (unsigned)c, (unsigned)n, d.sb, d.st, d.sh);
+  rc = walk_run(a->dtype, w, OUTPUTS, s);
+  if (rc) return rc;
+  return ws.out.finish(s);
 }
 
 extern "C" int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dout, const float* ds_out,
@@ -1268,75 +1386,62 @@ extern "C" int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dou
   if (rc) return rc;
   if (a->b == 0) return UR3E_OK;
   if (!dout || !dq || !dk || !dv) return bad_arg("attention: null gradient");
-  if (a->heads != a->kv_heads && (long long)a->b * a->t * a->kv_heads * (a->dk > a->dv ? a->dk : a->dv) > 0xffffff00LL)
-    return bad_arg("attention: too many tokens for shared heads");
   if (a->t > 0 && (!dout->p || !dq->p || !dk->p || !dv->p)) return bad_arg("attention: null gradient");
   if (dout->st < 0 || dq->st < 0 || dk->st < 0 || dv->st < 0) return bad_arg("attention: token strides must not be negative");
-  if (workspace_bytes < attn_bytes(a, 1) || (attn_bytes(a, 1) && !workspace)) return bad_arg("attention: workspace too small");
+  BackwardSpace ws(a, *dout, *dq, *dk, *dv, workspace);
+  rc = space_check(ws.used, workspace, workspace_bytes);
+  if (rc) return rc;
   hipStream_t s = (hipStream_t)stream;
-  const int grp = a->heads / a->kv_heads;
-  const Splits p = splits_of(a, 1);
-  char* ws = (char*)workspace;
-  const size_t n = up256(split_bytes(a, p));
-  float *fk = nullptr, *fv = nullptr;
-  if (grp > 1) {
-    fk = (float*)(ws + 2 * n);
-    fv = (float*)(ws + 2 * n + up256((size_t)a->b * a->t * a->heads * a->dk * 4));
-  }
-  const Tok tq = tok_of(a->q, 1), tk = tok_of(a->k, grp), tv = tok_of(a->v, grp), tdo = tok_of(*dout, 1);
-  auto wide = [&](const float* x, int d) { return Tok{x, (long long)a->t * a->heads * d, (long long)a->heads * d, d, 1}; };
+  rc = ws.pack.run(s);
+  if (rc) return rc;
   Walk f = {}, q = {}, k = {}, v = {};
   /* dq = walk(do, v, k) on S^T */
-  q.q = tdo; q.k = tv; q.v = tk; q.o = tok_of(*dq, 1);
+  q.q = ws.dout; q.k = ws.v; q.v = ws.k; q.o = ws.dq;
+  q.out_f32 = ws.wq.width != 0;
   q.state_t = 1;
   q.s_in = a->s0;
   q.in_scale = q.p_scale = a->scale; q.w_scale = 1.0f;
-  split_use(a, p, ws, q);
+  split_use(a, ws.p, workspace, q);
   /* dv = reversed walk(k, q, do) on G */
-  v.q = tk; v.k = tq; v.v = tdo; v.o = grp > 1 ? wide(fv, a->dv) : tok_of(*dv, 1);
-  v.out_f32 = grp > 1;
+  v.q = ws.k; v.k = ws.q; v.v = ws.dout; v.o = ws.dv;
+  v.out_f32 = ws.wv.width != 0;
   v.s_in = ds_out; v.s_out = ds0;
   v.reversed = 1;
   v.in_scale = 1.0f; v.p_scale = v.w_scale = a->scale;
-  split_use(a, p, ws + n, v);
+  split_use(a, ws.p, (char*)workspace + ws.states, v);
   /* dk = reversed walk(v, do, q) on G^T */
   k = v;
-  k.q = tv; k.k = tdo; k.v = tq; k.o = grp > 1 ? wide(fk, a->dk) : tok_of(*dk, 1);
+  k.q = ws.v; k.k = ws.dout; k.v = ws.q; k.o = ws.dk;
+  k.out_f32 = ws.wk.width != 0;
   k.state_t = 1;
   k.s_out = nullptr;
-  if (p.n > 1) {
+  if (ws.p.n > 1) {
     /* the states of the splits: S of the forward walk, and G, which dk and dv share */
-    f.k = tk; f.v = tv;
+    f.k = ws.k; f.v = ws.v;
     f.s_in = a->s0;
     f.w_scale = 1.0f;
-    split_use(a, p, ws, f);
-    WalkArgs w = args_of(a, a->dk, a->dv, p);
+    split_use(a, ws.p, workspace, f);
+    WalkArgs w = args_of(a, a->dk, a->dv, ws.p);
     w.w[0] = f; w.w[1] = v;
     w.nw = 2;
     rc = walk_run(a->dtype, w, STATES, s);
     if (rc) return rc;
   }
-  WalkArgs w = args_of(a, a->dv, a->dk, p);
+  WalkArgs w = args_of(a, a->dv, a->dk, ws.p);
   w.w[0] = q; w.w[1] = k; w.w[2] = v;
   w.nw = a->dk == a->dv ? 3 : 2;
   rc = walk_run(a->dtype, w, OUTPUTS, s);
   if (rc) return rc;
   if (w.nw == 2) {
-    WalkArgs x = args_of(a, a->dk, a->dv, p);
+    WalkArgs x = args_of(a, a->dk, a->dv, ws.p);
     x.w[0] = v;
     x.nw = 1;
     rc = walk_run(a->dtype, x, OUTPUTS, s);
     if (rc) return rc;
   }
-  if (grp > 1 && a->t > 0) {
-    auto sum = [&](const float* src, const ur3e_tokens_t& d, int c) {
-      if (a->dtype == UR3E_F32) group_sum<float>(a, src, d, c, s);
-      else if (a->dtype == UR3E_BF16) group_sum<Bf16>(a, src, d, c, s);
-      else group_sum<F16>(a, src, d, c, s);
-      return hipGetLastError();
-    };
-    PL_CHK(sum(fk, *dk, a->dk));
-    PL_CHK(sum(fv, *dv, a->dv));
+  for (const Wide* x : {&ws.wq, &ws.wk, &ws.wv}) {
+    rc = x->finish(s);
+    if (rc) return rc;
   }
   return UR3E_OK;
 }

@@ -188,8 +188,8 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
     if (s0.defined() && ctx->needs_input_grad(3)) /* an absent state has no edge */
       ds0 = at::empty_like(s0);
     const ur3e_attn_t a = args(q, k, v, x[4], s0, x[5], x[6], ctx->saved_data["scale"].toDouble());
-    const Tensor ws = workspace(a, 1, q);
     const ur3e_tokens_t g = tok(dout), tq = tok(dq), tk = tok(dk), tv = tok(dv);
+    const Tensor ws = workspace(a, 1, q);
     chk(ur3e_attn_backward(&a, &g, (const float*)ptr(ds), &tq, &tk, &tv, (float*)ptr(ds0), (void*)ptr(ws),
                            ws.defined() ? ws.numel() : 0, stream_of(q)));
     return {dq, dk, dv, ds0, Tensor(), Tensor(), Tensor(), Tensor(), Tensor()};
