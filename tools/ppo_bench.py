@@ -5,7 +5,8 @@ One process per GPU under torchrun: each rank steps its own env shard; gradients
 one flattened RCCL all-reduce per minibatch.  Prints one JSON line (rank 0) with
   rollout env-steps/s  (env + normalisation + policy inference, all ranks),
   iteration env-steps/s (rollout + the PPO update, all ranks).
-usage: python tools/ppo_bench.py [--envs-per-gpu 4096] [--n-steps 16] [--batch-size 256] [--n-epochs 30]"""
+usage: python tools/ppo_bench.py [--envs-per-gpu 4096] [--n-steps 16] [--batch-size 256] [--n-epochs 30]
+       [--policy mlp|memory] [--dropout 0.0]"""
 import argparse
 import json
 import os
@@ -23,6 +24,8 @@ def main():
     ap.add_argument("--batch-size", type=int, default=256)
     ap.add_argument("--n-epochs", type=int, default=30)
     ap.add_argument("--iterations", type=int, default=2)
+    ap.add_argument("--policy", choices=("mlp", "memory"), default="mlp")
+    ap.add_argument("--dropout", type=float, default=0.0)
     a = ap.parse_args()
     import torch
     import torch.distributed as dist
@@ -41,7 +44,7 @@ def main():
     venv = UR3eVecEnv(num_envs=n, device=local, seed=0, env_id_offset=rank * n)
     env = VecNormalize(venv, norm_obs=True, norm_reward=False, clip_obs=10.0, group=group)
     algo = PPO(env, n_steps=a.n_steps, batch_size=a.batch_size, n_epochs=a.n_epochs, device=f"cuda:{local}",
-               seed=rank, group=group)
+               seed=rank, group=group, policy=a.policy, dropout=a.dropout)
     algo.learn(1)  # warm-up: allocations, first kernels
     if group is not None:
         dist.barrier()
@@ -59,7 +62,7 @@ def main():
             "rollout_env_steps_per_s": steps / roll, "iteration_env_steps_per_s": steps / it,
             "rollout_ms_per_env_step": 1e3 * roll / a.n_steps, "train_s_per_iteration": it - roll,
             "config": {"envs_per_gpu": n, "n_steps": a.n_steps, "batch_size": a.batch_size, "n_epochs": a.n_epochs,
-                       "net_arch": [256, 256], "obs_norm": "on-device VecNormalize", "dtype": "env f64, policy f32"},
+                       "net_arch": [256, 256], "policy": a.policy, "dropout": a.dropout, "obs_norm": "on-device VecNormalize", "dtype": "env f64, policy f32"},
             "losses": algo.stats}), flush=True)
     if group is not None:
         dist.destroy_process_group()

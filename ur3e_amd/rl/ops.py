@@ -27,6 +27,8 @@ import torch
 
 from .. import runtime as rt
 
+MAX_DIM = 128  # channels of a head (UR3E_ATTN_MAX_DIM)
+
 _ext = None
 
 

@@ -16,6 +16,13 @@ policy forward with no host round trip.  With several ranks (one process per GPU
 own env shard and keeps a policy replica; gradients are flattened into ONE buffer and all-reduced
 (averaged) per minibatch, a single RCCL call over xGMI instead of one per parameter tensor.
 
+Beyond the reference's MLP (`policy="mlp"`, the default) there is a policy that remembers (`policy="memory"`: attention
+with a decaying state, ur3e_amd/rl/ops.py, in the place of the reference's sequence feature extractor over
+stacked frames, train_rl.py:26-35), and dropout (`dropout=p`) for either.  The memory is carried from step to step of a
+rollout, cut where an episode starts, and the update runs over whole rollouts of a few envs from the states their
+rollouts began with.  A dropped unit is a function of the transition's number, so every epoch of the update
+drops what the rollout dropped and the probability ratio measures the policy's change alone.
+
 The env object only needs `num_envs`, `action_space` (low/high), `reset_torch()` and
 `step_torch(actions) -> (obs f32, reward, terminated, truncated, terminal_obs f32)`: the GPU
 `VecNormalize` provides it, and tests use a CPU stand-in with the same interface.
@@ -27,6 +34,8 @@ import time
 
 import torch
 import torch.nn as nn
+
+from . import ops
 
 
 def _mlp(sizes, gain):
@@ -41,10 +50,13 @@ def _mlp(sizes, gain):
 
 class ActorCritic(nn.Module):
     """SB3 ActorCriticPolicy for a Box action space with net_arch=[256, 256]: separate pi / vf MLPs
-    over the flattened observation, Gaussian head with a state-independent log_std."""
+    over the flattened observation, Gaussian head with a state-independent log_std.  `rows` (transition numbers)
+    turn dropout on: hidden units of a transition are dropped by its number (ops.keyed_dropout)."""
 
-    def __init__(self, obs_dim: int, act_dim: int, net_arch=(256, 256), log_std_init: float = 0.0):
+    def __init__(self, obs_dim: int, act_dim: int, net_arch=(256, 256), log_std_init: float = 0.0,
+                 dropout: float = 0.0, seed: int = 0):
         super().__init__()
+        self.dropout, self.seed = dropout, seed
         self.pi_net = _mlp([obs_dim, *net_arch], gain=math.sqrt(2))
         self.vf_net = _mlp([obs_dim, *net_arch], gain=math.sqrt(2))
         self.action_net = nn.Linear(net_arch[-1], act_dim)
@@ -55,17 +67,114 @@ class ActorCritic(nn.Module):
         nn.init.zeros_(self.value_net.bias)
         self.log_std = nn.Parameter(torch.full((act_dim,), float(log_std_init)))
 
-    def dist(self, obs):
-        mean = self.action_net(self.pi_net(obs))
+    def _hidden(self, net, obs, rows, substream):
+        if rows is None or not self.dropout:
+            return net(obs)
+        for i, layer in enumerate(net):
+            obs = layer(obs)
+            if isinstance(layer, nn.Tanh):
+                obs = ops.keyed_dropout(obs, self.dropout, self.seed, rows, substream + i)
+        return obs
+
+    def mean(self, obs, rows=None):
+        return self.action_net(self._hidden(self.pi_net, obs, rows, PI_STREAM))
+
+    def normal(self, mean):
         # validate_args=False: the argument checks synchronise with the host every rollout step
         return torch.distributions.Normal(mean, self.log_std.exp().expand_as(mean), validate_args=False)
 
-    def value(self, obs):
-        return self.value_net(self.vf_net(obs)).squeeze(-1)
+    def dist(self, obs, rows=None):
+        return self.normal(self.mean(obs, rows))
 
-    def evaluate(self, obs, actions):
-        d = self.dist(obs)
-        return self.value(obs), d.log_prob(actions).sum(-1), d.entropy().sum(-1)
+    def value(self, obs, rows=None):
+        return self.value_net(self._hidden(self.vf_net, obs, rows, VF_STREAM)).squeeze(-1)
+
+    def evaluate(self, obs, actions, rows=None):
+        d = self.dist(obs, rows)
+        return self.value(obs, rows), d.log_prob(actions).sum(-1), d.entropy().sum(-1)
+
+
+# substreams of the dropout masks: one for each place of a network
+PI_STREAM, VF_STREAM = 0, 1 << 16
+
+
+class MemoryNet(nn.Module):
+    """A trunk that remembers: tanh encoder, attention with a decaying state (`heads` heads of width / heads
+    channels, each normalised to unit mean square), projected and added to the encoder's output, tanh layer.
+    `sequence` runs over [B, T, obs] from a state, `step` one token of N envs."""
+
+    def __init__(self, obs_dim: int, net_arch=(256, 256), heads: int = 4, dropout: float = 0.0, seed: int = 0,
+                 substream: int = 0):
+        super().__init__()
+        width = net_arch[0]
+        if len(net_arch) != 2 or width % heads or width // heads > ops.MAX_DIM:
+            raise ValueError(f"a memory needs two layers, the first of {heads} heads of at most {ops.MAX_DIM} "
+                             f"channels: net_arch={tuple(net_arch)}")
+        self.heads, self.dim = heads, width // heads
+        self.dropout, self.seed, self.substream = dropout, seed, substream
+        gain = math.sqrt(2)
+        self.encoder = _mlp([obs_dim, width], gain)
+        self.qkv = nn.Linear(width, 3 * width, bias=False)
+        self.out = nn.Linear(width, width, bias=False)
+        self.tail = _mlp([width, net_arch[1]], gain)
+        nn.init.orthogonal_(self.qkv.weight)
+        nn.init.orthogonal_(self.out.weight)
+        # the heads forget over 4 to 256 steps
+        over = torch.linspace(2.0, 8.0, heads) if heads > 1 else torch.tensor([5.0])
+        self.register_buffer("log_decay", torch.log1p(-torch.exp2(-over)))
+
+    def state(self, n: int, device):
+        """n empty memories"""
+        return torch.zeros((n, self.heads, self.dim, self.dim), dtype=torch.float32, device=device)
+
+    def _qkv(self, e):
+        return self.qkv(e).unflatten(-1, (3, self.heads, self.dim)).unbind(-3)
+
+    def _merge(self, e, y, rows):
+        y = y * torch.rsqrt(y.pow(2).mean(-1, keepdim=True) + 1e-6)
+        y = self.out(y.flatten(-2))
+        if rows is None or not self.dropout:
+            h = e + y
+        else:
+            h = ops.keyed_dropout(y, self.dropout, self.seed, rows, self.substream, residual=e)
+        return self.tail(h)
+
+    def sequence(self, obs, state, starts, rows=None):
+        e = self.encoder(obs)
+        y, _ = ops.decay_attention(*self._qkv(e), self.log_decay, initial_state=state, starts=starts)
+        return self._merge(e, y, rows)
+
+    def step(self, obs, state, starts=None, rows=None, next_state=None, update=True):
+        e = self.encoder(obs)
+        y = ops.decay_attention_step(*self._qkv(e), self.log_decay, state, starts=starts, next_state=next_state,
+                                     update=update)
+        return self._merge(e, y, rows)
+
+
+class MemoryActorCritic(nn.Module):
+    """ActorCritic with a memory in each trunk"""
+
+    def __init__(self, obs_dim: int, act_dim: int, net_arch=(256, 256), log_std_init: float = 0.0,
+                 dropout: float = 0.0, seed: int = 0, heads: int = 4):
+        super().__init__()
+        self.pi_net = MemoryNet(obs_dim, net_arch, heads, dropout, seed, PI_STREAM)
+        self.vf_net = MemoryNet(obs_dim, net_arch, heads, dropout, seed, VF_STREAM)
+        self.action_net = nn.Linear(net_arch[-1], act_dim)
+        self.value_net = nn.Linear(net_arch[-1], 1)
+        nn.init.orthogonal_(self.action_net.weight, gain=0.01)
+        nn.init.zeros_(self.action_net.bias)
+        nn.init.orthogonal_(self.value_net.weight, gain=1.0)
+        nn.init.zeros_(self.value_net.bias)
+        self.log_std = nn.Parameter(torch.full((act_dim,), float(log_std_init)))
+
+    normal = ActorCritic.normal
+
+    def evaluate(self, obs, actions, states, starts, rows=None):
+        """obs [B, T, .], actions [B, T, .], states = (pi, vf) in front of the first token, starts [B, T]; every result
+        flattened to B * T"""
+        d = self.normal(self.action_net(self.pi_net.sequence(obs, states[0], starts, rows)).flatten(0, 1))
+        v = self.value_net(self.vf_net.sequence(obs, states[1], starts, rows)).flatten()
+        return v, d.log_prob(actions.flatten(0, 1)).sum(-1), d.entropy().sum(-1)
 
 
 def compute_gae(rewards, values, episode_starts, last_values, dones, gamma, lam):
@@ -91,7 +200,17 @@ class PPO:
     def __init__(self, env, n_steps: int = 16, batch_size: int = 256, n_epochs: int = 30, learning_rate: float = 3e-4,
                  gamma: float = 0.99, gae_lambda: float = 0.95, clip_range: float = 0.2, ent_coef: float = 0.01,
                  vf_coef: float = 0.5, max_grad_norm: float = 0.5, net_arch=(256, 256), device=None, seed: int = 0,
-                 group=None, graphs=None):
+                 group=None, graphs=None, policy: str = "mlp", dropout: float = 0.0, heads: int = 4):
+        """policy: "mlp" or "memory"; dropout: probability of dropping a hidden unit; heads: of the memory.  With a
+        memory a minibatch is the whole rollouts of batch_size / n_steps envs."""
+        if policy not in ("mlp", "memory"):
+            raise ValueError(f"policy must be 'mlp' or 'memory', got {policy!r}")
+        if not 0.0 <= dropout < 1.0:
+            raise ValueError(f"dropout must be in [0, 1), got {dropout}")
+        self.memory = policy == "memory"
+        if self.memory and batch_size % n_steps:
+            raise ValueError(f"a memory's minibatch is whole rollouts: batch_size ({batch_size}) must be a multiple of "
+                             f"n_steps ({n_steps})")
         self.env = env
         self.n_envs = env.num_envs
         self.device = torch.device(device) if device is not None else torch.device("cpu")
@@ -105,7 +224,9 @@ class PPO:
         self.max_grad_norm = max_grad_norm
         self.group = group
         torch.manual_seed(seed)
-        self.policy = ActorCritic(self.obs_dim, self.act_dim, net_arch).to(self.device)
+        kw = dict(dropout=dropout, seed=seed)
+        self.policy = (MemoryActorCritic(self.obs_dim, self.act_dim, net_arch, heads=heads, **kw) if self.memory else
+                       ActorCritic(self.obs_dim, self.act_dim, net_arch, **kw)).to(self.device)
         if group is not None:  # identical replicas: broadcast rank 0's initial weights
             import torch.distributed as dist
             for p in self.policy.parameters():
@@ -134,12 +255,31 @@ class PPO:
         self.buf_val = torch.zeros((T, N), **f)
         self.buf_logp = torch.zeros((T, N), **f)
         self._noise = torch.zeros((T, N, self.act_dim), **f)
+        # transition (t, n) of the running rollout has number _first + t * N + n
+        self.dropout = dropout
+        self._first = torch.zeros((), dtype=torch.int64, device=self.device)
+        self._numbers = torch.arange((T + 1) * N, device=self.device).view(T + 1, N)
+        if self.memory:
+            # pi's and vf's memories in front of the current observation; vf's behind it; what the rollout began with
+            self._pi, self._vf, self._vf_next = (self.policy.pi_net.state(N, self.device) for _ in range(3))
+            self._began = (torch.empty_like(self._pi), torch.empty_like(self._vf))
         self._obs = None
         self._start = torch.ones(N, **f)
         self.num_timesteps = 0
         self.stats = {}
 
     # -- rollout ---------------------------------------------------------------
+    def _rows(self, t: int):
+        """numbers of the transitions at rollout index t (None: nothing is dropped)"""
+        return self._first + self._numbers[t] if self.dropout else None
+
+    def _current_value(self):
+        """the critic on the current observation"""
+        if not self.memory:
+            return self.policy.value(self._obs, self._rows(0))
+        h = self.policy.vf_net.step(self._obs, self._vf, self._start > 0, self._rows(0), next_state=self._vf_next)
+        return self.policy.value_net(h).squeeze(-1)
+
     def _rollout_step(self, t: int):
         """One env step at rollout index t (persistent tensors; no host synchronisation).
         Launch count is what limits a 4,096-env rollout step, so: the sampling noise and the
@@ -148,13 +288,25 @@ class PPO:
         observation and of the terminal observation share one critic pass over 2N rows."""
         N = self.n_envs
         obs = self._obs
-        act = self.policy.action_net(self.policy.pi_net(obs)) + self._std * self._noise[t]
+        if self.memory:
+            h = self.policy.pi_net.step(obs, self._pi, self._start > 0, self._rows(t))
+            act = self.policy.action_net(h) + self._std * self._noise[t]
+        else:
+            act = self.policy.mean(obs, self._rows(t)) + self._std * self._noise[t]
         clipped = torch.maximum(torch.minimum(act, self.high), self.low)
         nobs, rew, term, trunc, tobs = self.env.step_torch(clipped.to(torch.float64))
-        self._vin[:N].copy_(nobs)
-        self._vin[N:].copy_(tobs)
-        v2 = self.policy.value(self._vin)
         term, trunc = term.bool(), trunc.bool()
+        if self.memory:
+            # behind this observation: what the terminal observation would be worth, and the next one's value
+            self._vf, self._vf_next = self._vf_next, self._vf
+            end = self.policy.vf_net.step(tobs.to(torch.float32), self._vf, None, self._rows(t), update=False)
+            nxt = self.policy.vf_net.step(nobs, self._vf, term | trunc, self._rows(t + 1), next_state=self._vf_next)
+            v2 = self.policy.value_net(torch.cat([nxt, end])).squeeze(-1)
+        else:
+            self._vin[:N].copy_(nobs)
+            self._vin[N:].copy_(tobs)
+            rows = torch.cat([self._rows(t + 1), self._rows(t)]) if self.dropout else None
+            v2 = self.policy.value(self._vin, rows)
         # SB3 timeout bootstrap: truncated-not-terminated envs get gamma * V(terminal obs); evaluated
         # for every env and masked, so the rollout never waits on the host for an any()
         rew = rew.to(torch.float32) + self.gamma * torch.where(trunc & ~term, v2[N:], torch.zeros_like(v2[N:]))
@@ -171,10 +323,13 @@ class PPO:
     def collect_rollouts(self):
         if self._obs is None:
             self._obs = self.env.reset_torch().to(torch.float32).clone()
-            self._val = self.policy.value(self._obs)
+            self._val = self._current_value()
             self._vin = torch.empty((2 * self.n_envs, self.obs_dim), dtype=torch.float32, device=self.device)
         else:  # the critic changed in train(): value the carried-over observation with the new one
-            self._val = self.policy.value(self._obs)
+            self._val = self._current_value()
+        if self.memory:
+            self._began[0].copy_(self._pi)
+            self._began[1].copy_(self._vf)
         # all sampling noise of the rollout in one draw
         self._noise.normal_(generator=self.gen)
         self._std = self.policy.log_std.exp()
@@ -186,6 +341,7 @@ class PPO:
         self.adv, self.ret = compute_gae(self.buf_rew, self.buf_val, self.buf_start, last_val, self._start > 0,
                                          self.gamma, self.lam)
         self.num_timesteps += self.n_steps * self.n_envs
+        self._first += self.n_steps * self.n_envs
 
     # -- update ----------------------------------------------------------------
     def _allreduce_grads(self):
@@ -195,7 +351,15 @@ class PPO:
 
     def _loss(self, idx):
         """SB3 PPO.train minibatch loss (clipped surrogate, value MSE, entropy bonus)."""
-        v, logp, ent = self.policy.evaluate(self._obs_all[idx], self._act_all[idx])
+        if self.memory:
+            # idx: envs, each with its whole rollout
+            seq = [x[:, idx].transpose(0, 1) for x in (self.buf_obs, self.buf_act, self.buf_start)]
+            numbers = self._update_numbers[:, idx].transpose(0, 1) if self.dropout else None
+            v, logp, ent = self.policy.evaluate(seq[0], seq[1], [s[idx] for s in self._began], seq[2] > 0, numbers)
+            idx = (idx[:, None] + self._starts_at).flatten()  # of the flat buffers below, in the same order
+        else:
+            numbers = self._update_numbers.view(-1)[idx] if self.dropout else None
+            v, logp, ent = self.policy.evaluate(self._obs_all[idx], self._act_all[idx], numbers)
         adv = self._adv_s[idx]
         if adv.numel() > 1:
             adv = (adv - adv.mean()) / (adv.std() + 1e-8)
@@ -242,7 +406,7 @@ class PPO:
 
     def train(self):
         T, N = self.n_steps, self.n_envs
-        B = self.batch_size
+        B = self.batch_size // T if self.memory else self.batch_size
         total = T * N
         self._obs_all = self.buf_obs.reshape(total, -1)
         self._act_all = self.buf_act.reshape(total, -1)
@@ -251,13 +415,17 @@ class PPO:
             self._adv_s = torch.empty(total, dtype=torch.float32, device=self.device)
             self._ret_s = torch.empty(total, dtype=torch.float32, device=self.device)
             self._g_idx = torch.zeros(B, dtype=torch.long, device=self.device)
+            self._update_numbers = torch.empty_like(self._numbers[:T])
+            self._starts_at = torch.arange(0, total, N, device=self.device)
+        # the numbers that the rollout drew its masks with
+        torch.add(self._numbers[:T], self._first - total, out=self._update_numbers)
         self._adv_s.copy_(self.adv.reshape(-1))
         self._ret_s.copy_(self.ret.reshape(-1))
         last = None
         warm = 0
         for _ in range(self.n_epochs):
-            perm = torch.randperm(total, generator=self.gen, device=self.device)
-            for s in range(0, total, B):
+            perm = torch.randperm(N if self.memory else total, generator=self.gen, device=self.device)
+            for s in range(0, perm.numel(), B):
                 idx = perm[s:s + B]
                 if not self.use_graphs or idx.numel() != B:
                     last = self._minibatch_eager(idx)
