@@ -1101,9 +1101,10 @@ struct Splits {
   int n, len;
 };
 /* How many waves share a sequence, from the waves of the smallest launch.  Two waves a SIMD (2,048) fill the card,
-   and what does not fit beside them waits for a second round, so as many splits as still fit.  A split costs a
-   chain of chunks, and its state one more link of the chain of the join, so the shortest worth having grows with
-   the square root of the length. */
+   and what does not fit beside them waits for a second round, so as many splits as still fit.  Padded sequences
+   leave the waves of their padding idle: twice as many, unless the states of the splits, which are written, joined
+   and read, would then move more bytes than the tokens.  A split costs a chain of chunks, and its state one more
+   link of the chain of the join, so the shortest worth having grows with the square root of the length. */
 static Splits splits_of(const ur3e_attn_t* a, int backward) {
   long long waves = (long long)a->b * a->heads * tiles_of(a->dk, a->dv).slabs;
   if (backward && a->dk == a->dv) waves *= 3;
@@ -1112,14 +1113,21 @@ static Splits splits_of(const ur3e_attn_t* a, int backward) {
     if (other < waves) waves = other;
   }
   Splits p = {1, a->t > 0 ? a->t : 1};
-  const long long want = 2048 / waves;
-  if (want > 1 && a->t >= 64) {
-    int least = 32;
-    while ((long long)least * least * 4 < a->t) least += 16;
-    const int len = (int)(((a->t + want - 1) / want + 15) / 16 * 16);
-    p.len = len > least ? len : least;
-    p.n = (a->t + p.len - 1) / p.len;
+  if (a->t < 64) return p;
+  auto length = [&](long long n) { return (int)(((a->t + n - 1) / n + 15) / 16 * 16); };
+  int least = 32;
+  while ((long long)least * least * 4 < a->t) least += 16;
+  const long long once = 2048 / waves, again = 4096 / waves;
+  int len = once > 1 ? length(once) : a->t;
+  if (a->lengths && again > 1) {
+    const int even = 8 * a->dk * a->dv / ((a->dk + a->dv) * elem_size(a->dtype)), twice = length(again);
+    const int more = twice > even ? twice : (even + 15) / 16 * 16;
+    if (more < len) len = more;
   }
+  if (len >= a->t) return p;
+  p.len = len > least ? len : least;
+  p.n = (a->t + p.len - 1) / p.len;
+  if (p.n < 2) p = {1, a->t};
   return p;
 }
 
