@@ -62,6 +62,22 @@ def test_attention_sizes(b, t, h, hk, dk, dv, dtype):
     check_all(*make(b, t, h, hk, dk, dv, DT[dtype], seed=t))
 
 
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("first", range(1, 129, 8))
+def test_attention_every_channel_count(first, dtype):
+    """keys and values of 1 to 128 channels, each with another partner: rows that end anywhere in a lane's load"""
+    for d in range(first, first + 8):
+        dv = (d * 37) % 128 + 1
+        check_all(*make(1, 19, 2, 1, d, dv, DT[dtype], seed=d))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dk,dv", [(2, 3), (3, 66), (66, 1), (3, 3), (100, 70), (45, 45)])
+def test_attention_odd_rows_in_splits(dk, dv, dtype):
+    """rows of less than four channels and rows that fill no tile, over several waves a sequence, ragged, with starts"""
+    check_all(*make(3, 400, 4, 2, dk, dv, DT[dtype], seed=dk, starts=0.02, lengths=[400, 0, 333]))
+
+
 @pytest.mark.parametrize("dtype", ["f32", "bf16"])
 @pytest.mark.parametrize("t,starts,time_major", [(16, 0.3, True), (37, 0.1, False), (40, 1.0, True), (400, 0.02, False),
                                                  (400, 0.5, True)])
@@ -287,6 +303,54 @@ def test_streams_and_graphs():
             graphs[i].replay()
             torch.cuda.synchronize()
             assert all(torch.equal(want[n], outs[i][n]) for n in want), (r, i)
+
+
+def test_two_calls_at_once():
+    """calls on two streams that overlap on the card share nothing"""
+    cases = [make(2, 3000, 4, 4, 64, 64, torch.bfloat16, seed=i, starts=0.001) for i in range(2)]
+    want = [run(*c) for c in cases]
+    torch.cuda.synchronize()
+    streams = [torch.cuda.Stream() for _ in cases]
+    got = [[], []]
+    for _ in range(3):
+        for i, st in enumerate(streams):
+            with torch.cuda.stream(st):
+                got[i].append(run(*cases[i]))
+    torch.cuda.synchronize()
+    for i in range(2):
+        for g in got[i]:
+            assert all(torch.equal(g[n], want[i][n]) for n in g)
+
+
+def test_differentiable_once_and_too_large():
+    from ur3e_amd.rl import ops
+    x, dout, _ = make(1, 4, 1, 1, 8, 8, torch.float32, state=False)
+    q = x["q"].requires_grad_()
+    out, _ = ops.decay_attention(q, x["k"], x["v"], x["log_decay"])
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(out, [q], dout, create_graph=True)
+    y = ops.keyed_dropout(q, 0.5, 1)
+    with pytest.raises(RuntimeError, match="differentiable once"):
+        torch.autograd.grad(y, [q], torch.ones_like(y), create_graph=True)
+    big = torch.zeros((1, 1, 1, 8), device="cuda").expand(1 << 22, 1, 1, 8)
+    with pytest.raises(ValueError, match="2\\^22"):
+        ops.decay_attention(big, big, big, x["log_decay"])
+
+
+def test_gradients_of_some_inputs():
+    """a gradient is the same whichever of the others are asked for, and an unused output counts as zero"""
+    from ur3e_amd.rl import ops
+    x, dout, dfinal = make(2, 40, 4, 2, 24, 40, torch.float32)
+    full = run(x, dout, dfinal)
+    for n, dn in (("q", "dq"), ("k", "dk"), ("v", "dv"), ("initial_state", "ds0")):
+        leaf = x[n].detach().requires_grad_()
+        out, state = ops.decay_attention(**{**x, n: leaf}, return_state=True)
+        g, = torch.autograd.grad([out, state], [leaf], [dout, dfinal])
+        assert torch.equal(g, full[dn])
+        g1, = torch.autograd.grad(ops.decay_attention(**{**x, n: leaf}, return_state=True)[0], [leaf], dout)
+        g2, = torch.autograd.grad(ops.decay_attention(**{**x, n: leaf}, return_state=True)[1], [leaf], dfinal, allow_unused=True)
+        size = full[dn].abs().max()
+        assert (g1 + (0 if g2 is None else g2) - g).abs().max() <= 64 * 2.0 ** -24 * size * 40
 
 
 # -- keyed dropout -----------------------------------------------------------------

@@ -933,8 +933,10 @@ __global__ __launch_bounds__(256) void k_attn_group_sum(const float* __restrict_
 }
 
 /* ---- one token -----------------------------------------------------------------------------------
-   A wave owns one (sequence, head): lanes are CL groups of VW channels of v by 64 / CL rows of the state, rows
-   streamed once: S' = a S + k v^T stored, o += q S' kept per lane and summed over the row groups at the end. */
+   The state is read and written once and bounds the call: 4,096 envs x 4 heads of 64 x 64 take 108 us, 5.1 TB/s.
+   A wave owns one (sequence, head) and a slab of CL groups of VW value channels: its lanes are the groups by 64 / CL
+   rows, which they stream ROWS at a time: S' = a S + k v^T stored, o += q S' kept per lane and summed over the rows
+   at the end.  Few sequences are cut into narrower slabs, so that more waves share their rows. */
 struct StepArgs {
   Tok q, k, v, o;
   int b, h, kdim, vdim;
@@ -945,53 +947,56 @@ struct StepArgs {
   const float* s_in;
   float* s_out;
 };
-template <class T, int VW> __global__ __launch_bounds__(256) void k_attn_step(StepArgs a, int cl_log) {
+template <class T, int VW> __global__ __launch_bounds__(256) void k_attn_step(StepArgs a, int cl_log, int slabs) {
+  constexpr int ES = (int)sizeof(T), ROWS = 8;
   const int lane = threadIdx.x & 63;
-  const long long bh = (long long)blockIdx.x * 4 + (threadIdx.x >> 6);
-  if (bh >= (long long)a.b * a.h) return;
-  const int b = (int)(bh / a.h), h = (int)(bh % a.h);
+  const unsigned task = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+  const unsigned bh = task / slabs;
+  if (bh >= (unsigned)a.b * a.h) return;
+  const int slab = task % slabs, b = (int)(bh / a.h), h = (int)(bh % a.h);
   const int CL = 1 << cl_log, RG = 64 >> cl_log;
-  const int c = lane & (CL - 1), r0 = lane >> cl_log;
+  const int r0 = lane >> cl_log, d = (slab * CL + (lane & (CL - 1))) * VW;
+  const bool ok = d < a.vdim; /* VW divides vdim */
   const bool cut = a.starts && a.starts[b * a.starts_sb];
-  const float decay = cut ? 0.0f : expf(a.log_decay[h]);
-  const T* q = (const T*)a.q.p + b * a.q.sb + h / a.q.hdiv * a.q.sh;
-  const T* k = (const T*)a.k.p + b * a.k.sb + h / a.k.hdiv * a.k.sh;
+  const float decay = expf(a.log_decay[h]);
+  const Rsrc rq = rsrc_of((const char*)a.q.p + ES * (b * a.q.sb + h / a.q.hdiv * a.q.sh));
+  const Rsrc rk = rsrc_of((const char*)a.k.p + ES * (b * a.k.sb + h / a.k.hdiv * a.k.sh));
   const T* v = (const T*)a.v.p + b * a.v.sb + h / a.v.hdiv * a.v.sh;
   T* o = (T*)a.o.p + b * a.o.sb + h / a.o.hdiv * a.o.sh;
-  const long long base = bh * a.kdim * a.vdim;
-  struct alignas(4 * VW) Pack { float e[VW]; };
-  for (int c0 = 0; c0 < a.vdim; c0 += CL * VW) {
-    const int d = c0 + c * VW;
-    const bool ok = d < a.vdim; /* VW divides vdim */
-    float vv[VW], acc[VW];
+  const long long base = (long long)bh * a.kdim * a.vdim;
+  const Rsrc rs = rsrc_of(a.s_in + base, !cut); /* a state in front of a start is not read: zeros */
+  const Rsrc rw = rsrc_of(a.s_out + base, a.s_out != nullptr);
+  float vv[VW], acc[VW];
 #pragma unroll
-    for (int i = 0; i < VW; i++) { vv[i] = ok ? to_f(v[d + i]) : 0.0f; acc[i] = 0.0f; }
-#pragma unroll 4
-    for (int rr = 0; rr < a.kdim; rr += RG) {
-      const int row = rr + r0;
-      if (ok && row < a.kdim) {
-        const long long at = base + (long long)row * a.vdim + d;
-        const float kk = to_f(k[row]), qq = to_f(q[row]);
-        Pack s;
-        if (cut) {
+  for (int i = 0; i < VW; i++) { vv[i] = ok ? to_f(v[d + i]) : 0.0f; acc[i] = 0.0f; }
+  for (int rr = r0; rr < a.kdim + r0; rr += RG * ROWS) {
+    Raw<float, VW> s[ROWS];
+    Raw<T, 1> kk[ROWS], qq[ROWS];
+    unsigned off[ROWS];
 #pragma unroll
-          for (int i = 0; i < VW; i++) s.e[i] = 0.0f;
-        } else {
-          s = *reinterpret_cast<const Pack*>(a.s_in + at);
-        }
+    for (int u = 0; u < ROWS; u++) {
+      const int row = rr + u * RG;
+      const bool in = row < a.kdim;
+      off[u] = at(4 * (row * a.vdim + d), in & ok, FAR_T);
+      s[u].load(rs, off[u]);
+      kk[u].load(rk, at(row * ES, in, FAR_T));
+      qq[u].load(rq, at(row * ES, in, FAR_T));
+    }
 #pragma unroll
-        for (int i = 0; i < VW; i++) {
-          s.e[i] = fmaf(kk, vv[i], cut ? 0.0f : decay * s.e[i]);
-          acc[i] = fmaf(qq, s.e[i], acc[i]);
-        }
-        if (a.s_out) *reinterpret_cast<Pack*>(a.s_out + at) = s;
+    for (int u = 0; u < ROWS; u++) {
+      float x[VW];
+#pragma unroll
+      for (int i = 0; i < VW; i++) {
+        x[i] = fmaf(kk[u].get(0), vv[i], decay * s[u].get(i));
+        acc[i] = fmaf(qq[u].get(0), x[i], acc[i]);
       }
+      store_n<float, VW>(rw, off[u], x);
     }
+  }
 #pragma unroll
-    for (int i = 0; i < VW; i++) {
-      for (int m = CL; m < 64; m <<= 1) acc[i] += __shfl_xor(acc[i], m);
-      if (ok && r0 == 0) o[d + i] = from_f<T>(acc[i] * a.scale);
-    }
+  for (int i = 0; i < VW; i++) {
+    for (int m = CL; m < 64; m <<= 1) acc[i] += __shfl_xor(acc[i], m);
+    if (ok && r0 == 0) o[d + i] = from_f<T>(acc[i] * a.scale);
   }
 }
 
@@ -1190,11 +1195,11 @@ template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase pha
 template <class T, int KT, int VT> static int walk_tile(WalkArgs& a, Phase phase, hipStream_t s) {
   a.chunk = 16;
   /* a tile's tokens (a chunk's starts) within its 30-bit offsets, else token by token */
-  const long long far = ((1LL << 30) - 1024) / 64;
-  if (a.starts_st > far) a.chunk = 1;
+  auto far = [](long long st, int e) { return st > ((1LL << 30) - 1024) / 32 / e; };
+  if (far(a.starts_st, 1)) a.chunk = 1;
   for (int i = 0; i < a.nw; i++) {
     const Walk& w = a.w[i];
-    if (w.q.st > far || w.k.st > far || w.v.st > far || w.o.st > far) a.chunk = 1;
+    if (far(w.q.st, sizeof(T)) || far(w.k.st, sizeof(T)) || far(w.v.st, sizeof(T)) || far(w.o.st, w.out_f32 ? 4 : sizeof(T))) a.chunk = 1;
   }
   return walk_launch<T, KT, VT>(a, phase, s);
 }
@@ -1469,17 +1474,18 @@ extern "C" int ur3e_attn_step(const ur3e_attn_t* a, const ur3e_tokens_t* out, co
   s.scale = a->scale; s.log_decay = a->log_decay;
   s.starts = a->starts; s.starts_sb = a->starts_sb;
   s.s_in = state_in; s.s_out = state_out;
-  const bool v4 = a->dv % 4 == 0 && (uintptr_t)state_in % 16 == 0 && (uintptr_t)state_out % 16 == 0;
+  const bool v4 = a->dv % 4 == 0;
   const int groups = v4 ? a->dv / 4 : a->dv;
   int cl = 0;
   while ((1 << cl) < groups && cl < 6) cl++;
-  const dim3 grid((unsigned)(((long long)a->b * a->heads + 3) / 4));
+  auto slabs = [&] { return (groups + (1 << cl) - 1) >> cl; };
+  while (cl > 2 && (long long)a->b * a->heads * slabs() < 1024) cl--;
+  const dim3 grid((unsigned)(((long long)a->b * a->heads * slabs() + 3) / 4));
   hipStream_t st = (hipStream_t)stream;
-#define STEP(T)                                                                              \
-  if (v4) hipLaunchKernelGGL((k_attn_step<T, 4>), grid, dim3(256), 0, st, s, cl);            \
-  else hipLaunchKernelGGL((k_attn_step<T, 1>), grid, dim3(256), 0, st, s, cl);
-  if (a->dtype == UR3E_F32) { STEP(float) } else if (a->dtype == UR3E_BF16) { STEP(Bf16) } else { STEP(F16) }
-#undef STEP
+  auto run = [&](auto four, auto one) { hipLaunchKernelGGL(v4 ? four : one, grid, dim3(256), 0, st, s, cl, slabs()); };
+  if (a->dtype == UR3E_F32) run(k_attn_step<float, 4>, k_attn_step<float, 1>);
+  else if (a->dtype == UR3E_BF16) run(k_attn_step<Bf16, 4>, k_attn_step<Bf16, 1>);
+  else run(k_attn_step<F16, 4>, k_attn_step<F16, 1>);
   PL_CHK(hipGetLastError());
   return UR3E_OK;
 }

@@ -10,9 +10,8 @@
 
 #include <cmath>
 
+#include "../../include/ur3e_batch.h"
 #include "../../include/ur3e_policy.h"
-
-extern "C" const char* ur3e_last_error(void);
 
 namespace {
 
@@ -30,7 +29,10 @@ int dtype_of(const Tensor& x) {
   }
 }
 
-void chk(int rc) { TORCH_CHECK(rc == 0, "ur3e library error ", rc, ": ", ur3e_last_error()); }
+void chk(int rc) {
+  TORCH_CHECK_VALUE(rc != UR3E_EINVAL, ur3e_last_error());
+  TORCH_CHECK(rc == UR3E_OK, "ur3e library error ", rc, ": ", ur3e_last_error());
+}
 
 void* stream_of(const Tensor& x) {
   return (void*)at::hip::getCurrentHIPStreamMasqueradingAsCUDA(x.device().index()).stream();
