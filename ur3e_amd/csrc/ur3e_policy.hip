@@ -1118,7 +1118,8 @@ static Splits splits_of(const ur3e_attn_t* a, int backward) {
     if (other < waves) waves = other;
   }
   Splits p = {1, a->t > 0 ? a->t : 1};
-  if (a->t < 64) return p;
+  /* three launches take ~13 us more than one, the time of ~7 chunks */
+  if (a->t < (a->dtype == UR3E_BF16 ? 192 : 128)) return p;
   auto length = [&](long long n) { return (int)(((a->t + n - 1) / n + 15) / 16 * 16); };
   int least = 32;
   while ((long long)least * least * 4 < a->t) least += 16;
@@ -1195,8 +1196,8 @@ template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase pha
 template <class T, int KT, int VT> static int walk_tile(WalkArgs& a, Phase phase, hipStream_t s) {
   a.chunk = 16;
   /* a tile's tokens (a chunk's starts) within its 30-bit offsets, else token by token */
-  auto far = [](long long st, int e) { return st > ((1LL << 30) - 1024) / 32 / e; };
-  if (far(a.starts_st, 1)) a.chunk = 1;
+  auto far = [](long long st, int e, int tokens = 16) { return st > ((1LL << 30) - 1024) / tokens / e; };
+  if (far(a.starts_st, 1, 32)) a.chunk = 1;
   for (int i = 0; i < a.nw; i++) {
     const Walk& w = a.w[i];
     if (far(w.q.st, sizeof(T)) || far(w.k.st, sizeof(T)) || far(w.v.st, sizeof(T)) || far(w.o.st, w.out_f32 ? 4 : sizeof(T))) a.chunk = 1;
@@ -1218,7 +1219,13 @@ template <class T> static int walk_kt(WalkArgs& a, const Tiles& p, Phase phase, 
   }
 }
 static int walk_run(int dtype, WalkArgs& a, Phase phase, hipStream_t s) {
-  const Tiles p = tiles_of(a.kdim, a.vdim);
+  Tiles p = tiles_of(a.kdim, a.vdim);
+  /* Where the card has room, narrower slabs: a wave's chunk of 16 tokens of 64 x 64 float channels takes 3.3 us, with
+     a quarter of the value channels 2.1 us, for keys and scores that four waves then read and form. */
+  while (p.vt > 1 && (long long)a.b * a.h * a.nw * p.slabs * a.nsplit <= 1024) {
+    p.vt /= 2;
+    p.slabs = (a.vdim + 16 * p.vt - 1) / (16 * p.vt);
+  }
   a.slabs = p.slabs;
   if (dtype == UR3E_F32) return walk_kt<float>(a, p, phase, s);
   if (dtype == UR3E_BF16) return walk_kt<Bf16>(a, p, phase, s);
