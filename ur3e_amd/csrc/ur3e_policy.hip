@@ -904,31 +904,46 @@ template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(Wal
 }
 
 /* Sums of the per-query-head gradients over the `grp` heads that share a key / value head: rows of `width` floats,
-   [b][t][hk][grp][width], to `groups` x VW channels of [b][t][hk] rows.  With grp = 1 it narrows the rows of less
-   than four channels that the walks write eight wide. */
-template <class T, int VW>
-__global__ __launch_bounds__(256) void k_attn_group_sum(const float* __restrict__ src, T* __restrict__ dst, unsigned t,
-                                                        unsigned hk, unsigned grp, unsigned groups, unsigned width, unsigned n,
-                                                        long long sb, long long st, long long sh) {
-  struct alignas(4 * VW) Pack { float x[VW]; };
-  for (unsigned long long i0 = (unsigned long long)blockIdx.x * 256; i0 < n; i0 += (unsigned long long)gridDim.x * 256) {
+   [b][t][hk][grp][width], to d channels of [b][t][hk] rows.  With grp = 1 it narrows the rows of less than four
+   channels that the walks write eight wide.  A thread sums four channels; every tensor of a call in one launch. */
+struct SumArgs {
+  struct One {
+    const float* src;
+    void* dst;
+    long long sb, st, sh;
+    unsigned hk, grp, d, width, n; /* n: threads */
+  } x[3];
+  unsigned t;
+};
+template <class T> __global__ __launch_bounds__(256) void k_attn_group_sum(SumArgs a) {
+  const SumArgs::One x = a.x[blockIdx.y];
+  struct alignas(4) Four { float e[4]; };
+  const unsigned groups = (x.d + 3) / 4;
+  for (unsigned long long i0 = (unsigned long long)blockIdx.x * 256; i0 < x.n; i0 += (unsigned long long)gridDim.x * 256) {
     const unsigned i = (unsigned)i0 + threadIdx.x;
-    if (i >= n) return;
+    if (i >= x.n) return;
     unsigned r = i / groups;
-    const unsigned c = (i - r * groups) * VW;
-    const float* s = src + (long long)r * grp * width + c;
-    const unsigned kh = r % hk;
-    r /= hk;
-    const unsigned tt = r % t, bb = r / t;
-    float x[VW] = {};
-    for (unsigned k = 0; k < grp; k++) {
-      const Pack y = *reinterpret_cast<const Pack*>(s + (long long)k * width);
+    const unsigned c = (i - r * groups) * 4, left = x.d - c;
+    const float* s = x.src + (long long)r * x.grp * x.width + c;
+    const unsigned kh = r % x.hk;
+    r /= x.hk;
+    T* o = (T*)x.dst + r / a.t * x.sb + r % a.t * x.st + kh * x.sh + c;
+    if (left >= 4) {
+      Four y = {};
+      for (unsigned k = 0; k < x.grp; k++) {
+        const Four z = *reinterpret_cast<const Four*>(s + (long long)k * x.width);
 #pragma unroll
-      for (int e = 0; e < VW; e++) x[e] += y.x[e];
+        for (int e = 0; e < 4; e++) y.e[e] += z.e[e];
+      }
+#pragma unroll
+      for (int e = 0; e < 4; e++) o[e] = from_f<T>(y.e[e]);
+    } else {
+      for (unsigned e = 0; e < left; e++) {
+        float y = 0.0f;
+        for (unsigned k = 0; k < x.grp; k++) y += s[(long long)k * x.width + e];
+        o[e] = from_f<T>(y);
+      }
     }
-    T* o = dst + bb * sb + tt * st + kh * sh + c;
-#pragma unroll
-    for (int e = 0; e < VW; e++) o[e] = from_f<T>(x[e]);
   }
 }
 
@@ -1296,25 +1311,31 @@ struct Wide {
     used += up256((size_t)a->b * a->t * a->heads * width * 4);
     return Tok{p, (long long)a->t * a->heads * width, (long long)a->heads * width, width, 1};
   }
-  template <class T> void launch(hipStream_t s) const {
-    const int vw = d % 4 == 0 ? 4 : 1;
-    const unsigned hk = a->heads / grp;
-    const long long n = (long long)a->b * a->t * hk * (d / vw), blocks = (n + 255) / 256;
-    const dim3 grid((unsigned)(blocks < (1 << 20) ? blocks : 1 << 20));
-    if (vw == 4)
-      hipLaunchKernelGGL((k_attn_group_sum<T, 4>), grid, dim3(256), 0, s, p, (T*)to.p, (unsigned)a->t, hk, (unsigned)grp, (unsigned)(d / 4), (unsigned)width, (unsigned)n, to.sb, to.st, to.sh);
-    else
-      hipLaunchKernelGGL((k_attn_group_sum<T, 1>), grid, dim3(256), 0, s, p, (T*)to.p, (unsigned)a->t, hk, (unsigned)grp, (unsigned)d, (unsigned)width, (unsigned)n, to.sb, to.st, to.sh);
-  }
-  int finish(hipStream_t s) const {
-    if (!width || a->t == 0) return UR3E_OK;
-    if (a->dtype == UR3E_F32) launch<float>(s);
-    else if (a->dtype == UR3E_BF16) launch<Bf16>(s);
-    else launch<F16>(s);
-    PL_CHK(hipGetLastError());
-    return UR3E_OK;
-  }
 };
+static int wide_finish(const ur3e_attn_t* a, const Wide* const* wide, int count, hipStream_t s) {
+  SumArgs args = {};
+  int n = 0;
+  unsigned most = 0;
+  for (int i = 0; i < count; i++) {
+    const Wide& w = *wide[i];
+    if (!w.width || a->t == 0) continue;
+    SumArgs::One& x = args.x[n++];
+    x.src = w.p; x.dst = w.to.p;
+    x.sb = w.to.sb; x.st = w.to.st; x.sh = w.to.sh;
+    x.hk = a->heads / w.grp; x.grp = w.grp; x.d = w.d; x.width = w.width;
+    x.n = (unsigned)((long long)a->b * a->t * x.hk * ((w.d + 3) / 4));
+    if (x.n > most) most = x.n;
+  }
+  if (!n) return UR3E_OK;
+  args.t = a->t;
+  const unsigned blocks = (most + 255) / 256;
+  const dim3 grid(blocks < (1 << 20) ? blocks : 1 << 20, n);
+  if (a->dtype == UR3E_F32) hipLaunchKernelGGL(k_attn_group_sum<float>, grid, dim3(256), 0, s, args);
+  else if (a->dtype == UR3E_BF16) hipLaunchKernelGGL(k_attn_group_sum<Bf16>, grid, dim3(256), 0, s, args);
+  else hipLaunchKernelGGL(k_attn_group_sum<F16>, grid, dim3(256), 0, s, args);
+  PL_CHK(hipGetLastError());
+  return UR3E_OK;
+}
 
 /* The workspace of a call: the states of its splits, its wide outputs, its copied inputs. */
 struct ForwardSpace {
@@ -1396,7 +1417,8 @@ extern "C" int ur3e_attn_forward(const ur3e_attn_t* a, const ur3e_tokens_t* out,
   }
   rc = walk_run(a->dtype, w, OUTPUTS, s);
   if (rc) return rc;
-  return ws.out.finish(s);
+  const Wide* wide[] = {&ws.out};
+  return wide_finish(a, wide, 1, s);
 }
 
 extern "C" int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dout, const float* ds_out,
@@ -1459,11 +1481,8 @@ extern "C" int ur3e_attn_backward(const ur3e_attn_t* a, const ur3e_tokens_t* dou
     rc = walk_run(a->dtype, x, OUTPUTS, s);
     if (rc) return rc;
   }
-  for (const Wide* x : {&ws.wq, &ws.wk, &ws.wv}) {
-    rc = x->finish(s);
-    if (rc) return rc;
-  }
-  return UR3E_OK;
+  const Wide* wide[] = {&ws.wq, &ws.wk, &ws.wv};
+  return wide_finish(a, wide, 3, s);
 }
 
 extern "C" int ur3e_attn_step(const ur3e_attn_t* a, const ur3e_tokens_t* out, const float* state_in, float* state_out,
