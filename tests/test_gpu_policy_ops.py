@@ -97,6 +97,44 @@ def test_attention_starts_and_lengths(t, starts, time_major, dtype):
     assert all(torch.equal(got[n], again[n]) for n in got)
 
 
+@pytest.mark.parametrize("t,dk,dv", [(1500, 16, 16), (1700, 33, 20)])
+def test_attention_many_splits_of_one_sequence(t, dk, dv):
+    """more than 32 splits: the join's waves hand the state on to each other, through decays and starts"""
+    check_all(*make(1, t, 1, 1, dk, dv, torch.float32, seed=t, starts=0.004, decay=[-0.002]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_attention_exact_over_hundreds_of_splits(dtype):
+    """more than 512 splits, two rounds of the join.  Without decay and with values of -1, 0 and 1 every sum is a whole number:
+    the state stays below 2^11 (three are drawn, so it is a walk of 0.67 sqrt(t) = 180 on average), exact in any of the kernel's
+    forms, and so do the outputs in float; a 16-bit output is the exact one rounded once."""
+    from ur3e_amd.rl import ops
+    t, d = 70000, 16
+    g = torch.Generator().manual_seed(1)
+    q, k, v, do = (torch.randint(-1, 2, (1, t, 1, d), generator=g).float() for _ in range(4))
+    starts = torch.zeros((1, t), dtype=torch.bool)
+    starts[0, [0, 30001, 30002]] = True
+    leaves = [z.to(DT[dtype]).cuda().requires_grad_() for z in (q, k, v)]
+    s0 = torch.full((1, 1, d, d), float("nan"), device="cuda")
+    out, state = ops.decay_attention(*leaves, torch.zeros(1, device="cuda"), initial_state=s0, starts=starts.cuda(), scale=1.0,
+                                     return_state=True)
+    grads = torch.autograd.grad(out, leaves, do.to(DT[dtype]).cuda())
+    q, k, v, do = (z[0, :, 0].double() for z in (q, k, v, do))
+    segs = [(0, 30001), (30001, 30002), (30002, t)]
+    eo, eq, ek, ev = (torch.zeros(t, d, dtype=torch.float64) for _ in range(4))
+    for lo, hi in segs:
+        s = (k[lo:hi, :, None] * v[lo:hi, None, :]).cumsum(0)
+        gs = (q[lo:hi, :, None] * do[lo:hi, None, :]).flip(0).cumsum(0).flip(0)
+        eo[lo:hi] = (q[lo:hi, :, None] * s).sum(1)
+        eq[lo:hi] = (s * do[lo:hi, None, :]).sum(2)
+        ek[lo:hi] = (gs * v[lo:hi, None, :]).sum(2)
+        ev[lo:hi] = (gs * k[lo:hi, :, None]).sum(1)
+        assert max(s.abs().max(), gs.abs().max()) < 2 ** 11
+    assert torch.equal(state.cpu().double()[0, 0], s[-1])
+    for got, e in zip((out, *grads), (eo, eq, ek, ev)):
+        assert torch.equal(got.detach().cpu()[0, :, 0], e.float().to(DT[dtype]))
+
+
 def test_attention_lengths_are_clamped():
     x, dout, dfinal = make(3, 20, 2, 2, 16, 16, torch.float32, lengths=[-5, 99, 20])
     got = run(x, dout, dfinal)

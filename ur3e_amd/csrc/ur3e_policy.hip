@@ -861,10 +861,15 @@ template <class T> __global__ __launch_bounds__(256) void k_attn_pack(PackArgs a
 }
 
 /* States that enter each split: ws[s] holds split s - 1's own sum (k_attn_walk, STATE) and becomes
-   X_s = wf[s] X_{s-1} + ws[s], X_0 = s_in.  A thread owns VW elements and runs along the splits; nothing but
-   the chain of multiply-adds depends on the split in front, so the sums of LOT splits are loaded at a time, the next
-   ones while one lot is chained.  Few long sequences wait for the chain: one element a thread, long lots.  Many
-   short ones wait for their turn on the card: four elements a thread. */
+   X_s = wf[s] X_{s-1} + ws[s], X_0 = s_in.  Nothing but the chain of multiply-adds depends on the split in front.
+
+   Many sequences: a thread owns VW elements and runs along the splits, whose sums it loads LOT at a time, the next
+   lot while one is chained; the bytes bound it.  (A factor of 0 is an episode start: what was in front of it is
+   dropped whatever it holds.) */
+__device__ __forceinline__ float carry_on(float f, float x, float u) {
+  const float y = f * x;
+  return (f == 0.0f ? 0.0f : y) + u;
+}
 template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(WalkArgs a) {
   const Walk w = a.w[blockIdx.z];
   const long long bh = blockIdx.y;
@@ -894,12 +899,56 @@ template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(Wal
     for (int i = 0; i < LOT; i++) {
       if (s0 + i < nsplit) *reinterpret_cast<Pack*>(ws + (long long)(s0 + i) * elems) = x;
 #pragma unroll
-      for (int c = 0; c < VW; c++) {
-        const float y = l.f[i] * x.x[c];
-        x.x[c] = (l.f[i] == 0.0f ? 0.0f : y) + l.u[i].x[c];
-      }
+      for (int c = 0; c < VW; c++) x.x[c] = carry_on(l.f[i], x.x[c], l.u[i].x[c]);
     }
     l = next;
+  }
+}
+/* Few sequences wait for the chain: the waves of a workgroup take 32 splits each of the same 64 elements, all loads at
+   once, chain their own from zero and pass on the result and the product of their factors; each then starts from
+   what the waves in front make of the state.  219 splits of one demonstration: 15.7 us by the kernel above. */
+#define JOIN_WAVES 16
+__global__ __launch_bounds__(64 * JOIN_WAVES) void k_attn_join_wide(WalkArgs a) {
+  constexpr int LOT = 32;
+  __shared__ float sum[JOIN_WAVES][64], factor[JOIN_WAVES], last[64];
+  const Walk w = a.w[blockIdx.z];
+  const long long bh = blockIdx.y;
+  const int elems = a.kdim * a.vdim, nsplit = a.nsplit;
+  const int lane = threadIdx.x & 63, me = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
+  const int e = blockIdx.x * 64 + lane;
+  const bool ok = e < elems;
+  float* ws = w.ws + bh * nsplit * elems + (ok ? e : 0);
+  const float* wf = w.wf + bh * nsplit;
+  float start = ok && w.s_in ? w.s_in[bh * elems + e] : 0.0f;
+  for (int s0 = 0; s0 < nsplit; s0 += waves * LOT) {
+    const int mine = s0 + me * LOT; /* this wave turns ws[mine + 1 ..] into the states behind the state of split `mine` */
+    float u[LOT], f[LOT], x = 0.0f, g = 1.0f;
+#pragma unroll
+    for (int i = 0; i < LOT; i++) {
+      const int s = mine + 1 + i < nsplit ? mine + 1 + i : nsplit - 1;
+      u[i] = ws[(long long)s * elems];
+      f[i] = wf[s];
+    }
+#pragma unroll
+    for (int i = 0; i < LOT; i++)
+      if (mine + 1 + i < nsplit) {
+        x = carry_on(f[i], x, u[i]);
+        g *= f[i];
+      }
+    sum[me][lane] = x;
+    if (lane == 0) factor[me] = g;
+    __syncthreads();
+    x = start;
+    for (int i = 0; i < me; i++) x = carry_on(factor[i], x, sum[i][lane]);
+#pragma unroll
+    for (int i = 0; i < LOT; i++)
+      if (mine + i < nsplit) {
+        if (ok) ws[(long long)(mine + i) * elems] = x;
+        x = carry_on(f[i], x, u[i]);
+      }
+    if (me == waves - 1) last[lane] = x;
+    __syncthreads();
+    start = last[lane];
   }
 }
 
@@ -1200,6 +1249,8 @@ template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase pha
     for (int i = 0; i < a.nw; i++) four = four && (uintptr_t)a.w[i].s_in % 16 == 0 && (uintptr_t)a.w[i].ws % 16 == 0;
     if (four && (long long)bh * nw * elems >= 64 * 4096)
       hipLaunchKernelGGL((k_attn_join<4, 8>), dim3((elems + 255) / 256, bh, nw), dim3(64), 0, s, a);
+    else if (a.nsplit > 32)
+      hipLaunchKernelGGL(k_attn_join_wide, dim3((elems + 63) / 64, bh, nw), dim3(64 * ((a.nsplit + 31) / 32 < JOIN_WAVES ? (a.nsplit + 31) / 32 : JOIN_WAVES)), 0, s, a);
     else
       hipLaunchKernelGGL((k_attn_join<1, 32>), dim3((elems + 63) / 64, bh, nw), dim3(64), 0, s, a);
   } else {
