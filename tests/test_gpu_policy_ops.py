@@ -343,6 +343,63 @@ def test_streams_and_graphs():
             assert all(torch.equal(want[n], outs[i][n]) for n in want), (r, i)
 
 
+def test_capture_refuses_leaves_of_a_live_eager_graph():
+    """a captured backward pass cannot reach leaves whose gradients belong to an eager graph of the default stream"""
+    from ur3e_amd.rl import ops
+    w = torch.randn((8, 24), device="cuda", requires_grad=True)
+    x = torch.randn((2, 5, 8), device="cuda")
+    ld = torch.zeros(2, device="cuda")
+
+    def loss():
+        q, k, v = (x @ w).unflatten(-1, (3, 2, 4)).unbind(-3)
+        return ops.keyed_dropout(ops.decay_attention(q, k, v, ld)[0].flatten(-2), 0.5, 1).sum()
+
+    def drop():
+        return ops.keyed_dropout(x @ w, 0.5, 1)
+    for f in (loss, drop):
+        alive = f()
+        gr = torch.cuda.CUDAGraph()
+        with pytest.raises(RuntimeError, match="eager graph"):
+            with torch.cuda.graph(gr):
+                f()
+        gr = torch.cuda.CUDAGraph()
+        with torch.no_grad(), torch.cuda.graph(gr):  # the forward pass alone is free
+            y = f()
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(y, alive.detach())
+        del alive, y, gr
+    want, = torch.autograd.grad(loss(), [w])
+    gr = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(gr):
+        got, = torch.autograd.grad(loss(), [w])
+    for _ in range(3):
+        gr.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(got, want)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+def test_nothing_to_do(dtype):
+    """no sequences, no tokens, no rows, no columns"""
+    from ur3e_amd.rl import ops
+    for b, t, h, hk, dk, dv in ((0, 5, 4, 2, 8, 2), (3, 0, 4, 2, 8, 2), (0, 0, 2, 2, 64, 64), (3, 0, 2, 2, 64, 64)):
+        x, dout, dfinal = make(b, t, h, hk, dk, dv, DT[dtype], starts=0.5, lengths=[0] * b)
+        got = run(x, dout, dfinal)
+        assert torch.equal(got["state"], x["initial_state"]) and torch.equal(got["ds0"], dfinal)
+        assert all(got[n].shape == y.shape for n, y in (("out", dout), ("dq", x["q"]), ("dk", x["k"]), ("dv", x["v"])))
+        x, dout, dfinal = make(b, t, h, hk, dk, dv, DT[dtype], state=False)
+        assert run(x, dout, dfinal)["state"].abs().sum() == 0
+    s = torch.zeros((0, 2, 8, 8), device="cuda")
+    q = torch.zeros((0, 2, 8), device="cuda", dtype=DT[dtype])
+    assert ops.decay_attention_step(q, q, q, torch.zeros(2, device="cuda"), s).shape == (0, 2, 8)
+    for shape in ((0, 8), (8, 0), (2, 3, 0), (0, 2, 8), (0,), (0, 0)):
+        z = torch.zeros(shape, device="cuda", dtype=DT[dtype], requires_grad=True)
+        y = ops.keyed_dropout(z, 0.5, 1, residual=z)
+        g, = torch.autograd.grad(y.sum(), [z])
+        assert y.shape == g.shape == z.shape
+
+
 def test_two_calls_at_once():
     """calls on two streams that overlap on the card share nothing"""
     cases = [make(2, 3000, 4, 4, 64, 64, torch.bfloat16, seed=i, starts=0.001) for i in range(2)]

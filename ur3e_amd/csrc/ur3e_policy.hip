@@ -1140,8 +1140,11 @@ static int attn_check(const ur3e_attn_t* a) {
   if (a->dk < 1 || a->dk > UR3E_ATTN_MAX_DIM || a->dv < 1 || a->dv > UR3E_ATTN_MAX_DIM)
     return bad_arg("attention: dk and dv must be in [1, 128]");
   if ((long long)a->b * a->heads > 4194303) return bad_arg("attention: b * heads must be below 2^22");
-  /* 32-bit indices in k_attn_group_sum */
-  if ((a->heads != a->kv_heads || a->dk < 4 || a->dv < 4) && (long long)a->b * a->t * a->heads * UR3E_ATTN_MAX_DIM > 0xffffff00LL)
+  if (a->t > 1 << 30) return bad_arg("attention: t must be at most 2^30");
+  /* 32-bit indices in k_attn_group_sum, of groups of four channels (query heads where nothing is shared) */
+  const int most = a->dk > a->dv ? a->dk : a->dv;
+  if ((a->heads != a->kv_heads || a->dk < 4 || a->dv < 4) &&
+      (long long)a->b * a->t * (a->dk < 4 || a->dv < 4 ? a->heads : a->kv_heads) * ((most + 3) / 4) > 0xffffff00LL)
     return bad_arg("attention: too many tokens for shared heads or for less than 4 channels");
   if (a->b == 0) return UR3E_OK;
   if (a->q.st < 0 || a->k.st < 0 || a->v.st < 0 || a->starts_st < 0) return bad_arg("attention: token strides must not be negative");

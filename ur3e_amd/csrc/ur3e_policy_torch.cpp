@@ -9,6 +9,7 @@
 #include <torch/extension.h>
 
 #include <cmath>
+#include <unordered_set>
 
 #include "../../include/ur3e_batch.h"
 #include "../../include/ur3e_policy.h"
@@ -42,6 +43,33 @@ const void* ptr(const Tensor& x) { return x.defined() ? x.const_data_ptr() : nul
 
 /* the tensor, with the channels of a token next to each other */
 Tensor unit(const Tensor& x) { return x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.contiguous(); }
+
+/* Gradients under capture: where a leaf in front of x is held by an eager graph that still lives, its gradient is
+   accumulated on that graph's stream.  From a capture, torch's engine then makes the default stream wait for work that is
+   only being recorded, and the process ends.  So the call is refused while its graph is built. */
+void check_capture(const char* what, std::initializer_list<Tensor> xs) {
+  using torch::autograd::Node;
+  const hipStream_t stream = (hipStream_t)stream_of(*xs.begin());
+  hipStreamCaptureStatus status = hipStreamCaptureStatusNone;
+  /* (the default stream cannot be captured) */
+  if (!stream || hipStreamIsCapturing(stream, &status) != hipSuccess || status == hipStreamCaptureStatusNone) return;
+  std::vector<std::shared_ptr<Node>> todo;
+  std::unordered_set<const Node*> met;
+  for (const Tensor& x : xs)
+    if (x.defined() && x.requires_grad()) todo.push_back(torch::autograd::impl::gradient_edge(x).function);
+  while (!todo.empty()) {
+    const std::shared_ptr<Node> n = todo.back();
+    todo.pop_back();
+    if (!n || !met.insert(n.get()).second) continue;
+    if (n->name() == "torch::autograd::AccumulateGrad") {
+      const auto st = n->stream();
+      TORCH_CHECK(!st || st->id() != 0, what, ": under capture, but an eager graph of the default stream still holds one "
+                  "of the leaves, which a captured backward pass cannot reach; drop its outputs first (or capture the "
+                  "forward pass alone under torch.no_grad())");
+    }
+    for (const auto& edge : n->next_edges()) todo.push_back(edge.function);
+  }
+}
 
 /* ---- attention ---- */
 
@@ -112,7 +140,7 @@ void check_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
     TORCH_CHECK_VALUE(next->is_contiguous(), what, ": next_state must be contiguous");
     const char *x = (const char*)state.const_data_ptr(), *y = (const char*)next->const_data_ptr();
     const int64_t n = state.numel() * 4;
-    TORCH_CHECK_VALUE(x == y || (x - y < n ? y - x >= n : true) , what, ": next_state overlaps state");
+    TORCH_CHECK_VALUE(x == y || (x > y ? x - y >= n : y - x >= n), what, ": next_state overlaps state");
   }
 }
 
@@ -210,6 +238,7 @@ std::pair<Tensor, OptT> decay_attention(const Tensor& q, const Tensor& k, const 
     const auto [out, state] = forward(x, return_state);
     return {out, return_state ? OptT(state) : OptT()};
   }
+  check_capture("decay_attention", {x.q, x.k, x.v, x.s0});
   auto opt = [](const Tensor& t) { return t.defined() ? OptT(t) : OptT(); };
   const variable_list r = DecayAttention::apply(x.q, x.k, x.v, opt(x.s0), x.log_decay, opt(x.starts), opt(x.lengths), scale,
                                                 return_state);
@@ -265,6 +294,7 @@ struct Key {
 
 Tensor dropout(const Tensor& x, const Tensor& residual, const Tensor& rows, const Key& key) {
   c10::DeviceGuard guard(x.device());
+  if (x.numel() == 0) return at::empty(x.sizes(), x.options());
   const Tensor x2 = rows2d(x), r2 = residual.defined() ? rows2d(residual) : Tensor();
   const Tensor y = at::empty(x.sizes(), x.options());
   TORCH_CHECK_VALUE(x2.size(1) <= INT32_MAX - 8, "keyed_dropout: too many columns");
@@ -297,8 +327,10 @@ Tensor keyed_dropout(const Tensor& x, int64_t count, uint64_t seed, const OptT& 
                      const OptT& residual) {
   check_dropout(x, rows, residual);
   const OptT ids = rows ? OptT(rows->reshape(-1).contiguous()) : OptT();
-  if (at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad())))
+  if (at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad()))) {
+    check_capture("keyed_dropout", {x, residual.value_or(Tensor())});
     return KeyedDropout::apply(x, residual, ids, count, (int64_t)seed, substream);
+  }
   return dropout(x, residual.value_or(Tensor()), ids.value_or(Tensor()), {count, substream, seed});
 }
 
