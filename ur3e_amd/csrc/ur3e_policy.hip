@@ -226,6 +226,12 @@ __device__ __forceinline__ f4 mfma32(u4 a, u4 b, f4 c) {
   typedef __bf16 b8 __attribute__((ext_vector_type(8)));
   return __builtin_amdgcn_mfma_f32_16x16x32_bf16(__builtin_bit_cast(b8, a), __builtin_bit_cast(b8, b), c, 0, 0, 0);
 }
+/* the same of half elements, as they are in memory */
+template <class T> __device__ __forceinline__ f4 mfma_raw(u4 a, u4 b, f4 c) {
+  typedef _Float16 h8 __attribute__((ext_vector_type(8)));
+  if constexpr (__is_same(T, F16)) return __builtin_amdgcn_mfma_f32_16x16x32_f16(__builtin_bit_cast(h8, a), __builtin_bit_cast(h8, b), c, 0, 0, 0);
+  else return mfma32(a, b, c);
+}
 /* The packed leading parts of four elements that lie as an accumulator does (rows 4 g + e of column idx); x
    becomes the rest, x - hi, a product with the negative unit matrix: one instruction of the matrix pipe
    in place of eight of the vector pipe, which is the busier one.  Exact: every sum has one product.  An infinity
@@ -270,12 +276,12 @@ template <class X> __device__ __forceinline__ unsigned halves(const X& x, int i,
   return __builtin_amdgcn_perm(y.d[j / 2], x.d[i / 2], sel);
 }
 /* the four tokens of tile nt in the column form */
-template <int VT> __device__ __forceinline__ u2 pack_col(const Raw<Bf16, VT> (&x)[4], int nt) {
+template <class T, int VT> __device__ __forceinline__ u2 pack_col(const Raw<T, VT> (&x)[4], int nt) {
   return u2{halves(x[0], nt, x[1], nt), halves(x[2], nt, x[3], nt)};
 }
 /* the row form by tiles: e = 0 .. 3 of tile mt, as the rows of an accumulator lie */
-template <int KT> __device__ __forceinline__ void pack_row(const Row<Bf16, KT>& r, u2 (&y)[KT]) {
-  constexpr int C = Place<Bf16, KT>::C;
+template <class T, int KT> __device__ __forceinline__ void pack_row(const Row<T, KT>& r, u2 (&y)[KT]) {
+  constexpr int C = Place<T, KT>::C;
 #pragma unroll
   for (int mt = 0; mt < KT; mt++)
     y[mt] = u2{halves(r.x[0], mt, r.x[1 / C], 1 % C * KT + mt), halves(r.x[2 / C], 2 % C * KT + mt, r.x[3 / C], 3 % C * KT + mt)};
@@ -287,7 +293,8 @@ template <int KT> __device__ __forceinline__ void pack_row(const Row<Bf16, KT>& 
 template <class T, int KT, int VT, bool STATE, int H, bool FINE>
 __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   constexpr int ES = (int)sizeof(T), C = 16 * H;
-  static_assert(H == 1 || __is_same(T, Bf16), "two tiles of tokens: bfloat16 only");
+  constexpr bool TWO = __is_same(T, F16); /* an element is two bfloat16 parts */
+  static_assert(H == 1 || ES == 2, "two tiles of tokens: 16-bit types only");
   const int lane = threadIdx.x & 63, idx = lane & 15, g = lane >> 4;
   /* Workgroups go round the 8 XCDs in turn; the `near` of them that share a sequence's tensors and states stay on
      one, behind its L2.  The wave's task is in scalar registers, and with it every address base and loop bound. */
@@ -596,18 +603,29 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       const int n0 = n < 16 ? n : 16;
       put(rsrc_of(out + low_of(n, f) * ost, 16 * f < n), rev ? n0 - 1 - idx : idx, idx < n0, o);
     };
-    if constexpr (__is_same(T, Bf16)) {
-      u2 vq[H][VT];
+    if constexpr (ES == 2) {
+      u2 vq[H][VT], vr[H][VT]; /* leading part (the element itself where it is bfloat16) and rest */
+      auto values = [&] {
 #pragma unroll
-      for (int f = 0; f < H; f++)
+        for (int f = 0; f < H; f++)
 #pragma unroll
-        for (int nt = 0; nt < VT; nt++) vq[f][nt] = pack_col<VT>(c.vc[f], nt);
+          for (int nt = 0; nt < VT; nt++) {
+            if constexpr (TWO) {
+              f4 x;
+#pragma unroll
+              for (int e = 0; e < 4; e++) x[e] = c.vc[f][e].get(nt);
+              vq[f][nt] = split4(x, minus_one);
+              vr[f][nt] = pack4(x);
+            } else vq[f][nt] = pack_col<T, VT>(c.vc[f], nt);
+          }
+      };
+      if (STATE || !TWO) values();
       if (!STATE) {
         u2 kq[H][KT], qq[H][KT];
 #pragma unroll
         for (int f = 0; f < H; f++) {
-          pack_row<KT>(c.kr[f], kq[f]);
-          pack_row<KT>(c.qr[f], qq[f]);
+          pack_row<T, KT>(c.kr[f], kq[f]);
+          pack_row<T, KT>(c.qr[f], qq[f]);
         }
         /* Instructions that add to the same accumulators stand apart by those of the other tiles. */
         f4 pt[H][H]; /* [query tile][key tile] */
@@ -619,26 +637,40 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
             for (int fk = 0; fk <= fq; fk++) {
               const auto &x = kq[fk], &y = qq[fq];
               const f4 z = i ? pt[fq][fk] : f4{0, 0, 0, 0};
-              if constexpr (KT == 1) pt[fq][fk] = mfma32(u4{x[0].x, x[0].y, 0, 0}, u4{y[0].x, y[0].y, 0, 0}, z);
+              if constexpr (KT == 1) pt[fq][fk] = mfma_raw<T>(u4{x[0].x, x[0].y, 0, 0}, u4{y[0].x, y[0].y, 0, 0}, z);
               else
-                pt[fq][fk] = mfma32(u4{x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y},
+                pt[fq][fk] = mfma_raw<T>(u4{x[2 * i].x, x[2 * i].y, x[2 * i + 1].x, x[2 * i + 1].y},
                                     u4{y[2 * i].x, y[2 * i].y, y[2 * i + 1].x, y[2 * i + 1].y}, z);
             }
         f4 x[H][VT];
 #pragma unroll
         for (int mt = 0; mt < KT; mt++) {
-          
+          u2 qs[H]; /* the rests of the queries; the leading parts take the elements' place */
+          if constexpr (TWO) {
+#pragma unroll
+            for (int f = 0; f < H; f++) {
+              f4 y;
+#pragma unroll
+              for (int e = 0; e < 4; e++) y[e] = c.qr[f].get(e, mt);
+              qq[f][mt] = split4(y, minus_one);
+              qs[f] = pack4(y);
+            }
+          }
 #pragma unroll
           for (int nt = 0; nt < VT; nt++) {
             f4 rest = S[mt][nt];
             const u2 hi = split4(rest, minus_one), lo = pack4(rest);
+            if constexpr (TWO) {
+#pragma unroll
+              for (int f = 0; f < H; f++)
+                x[f][nt] = mfma32(u4{hi.x, hi.y, lo.x, lo.y}, u4{qs[f].x, qs[f].y, qs[f].x, qs[f].y}, mt ? x[f][nt] : f4{0, 0, 0, 0});
+            }
 #pragma unroll
             for (int f = 0; f < H; f++)
               x[f][nt] = mfma32(u4{hi.x, hi.y, lo.x, lo.y}, u4{qq[f][mt].x, qq[f][mt].y, qq[f][mt].x, qq[f][mt].y},
-                                mt ? x[f][nt] : f4{0, 0, 0, 0});
+                                TWO || mt ? x[f][nt] : f4{0, 0, 0, 0});
           }
         }
-        
 #pragma unroll
         for (int f = 0; f < H; f++) {
 #pragma unroll
@@ -660,6 +692,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
             for (int fk = 0; fk <= f; fk++) cut_scores(pt[f][fk], f, fk);
           }
         }
+        if (TWO) values(); /* (where registers are not needed for queries and scores any more) */
         u2 ph[H][H], pl[H][H]; /* leading part and rest */
 #pragma unroll
         for (int fq = 0; fq < H; fq++)
@@ -682,7 +715,16 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           for (int nt = 0; nt < VT; nt++)
             x[f][nt] = mfma32(u4{vq[0][nt].x, vq[0][nt].y, vq[f][nt].x, vq[f][nt].y},
                               u4{pl[f][0].x, pl[f][0].y, pl[f][f].x, pl[f][f].y}, x[f][nt]);
-        
+        if constexpr (TWO) {
+#pragma unroll
+          for (int f = 0; f < H; f++)
+#pragma unroll
+            for (int nt = 0; nt < VT; nt++) {
+              const u2 y = vr[0][nt], yf = vr[f][nt], z = ph[f][0], zl = pl[f][0], zf = ph[f][f];
+              if (f == 0) x[f][nt] = mfma32(u4{y.x, y.y, y.x, y.y}, u4{z.x, z.y, zl.x, zl.y}, x[f][nt]);
+              else x[f][nt] = mfma32(u4{y.x, y.y, yf.x, yf.y}, u4{z.x, z.y, zf.x, zf.y}, x[f][nt]);
+            }
+        }
 #pragma unroll
         for (int f = 0; f < H; f++) {
           float o[4][VT];
@@ -697,7 +739,6 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       decay();
 #pragma unroll
       for (int mt = 0; mt < KT; mt++) {
-        
         f4 kx[H];
         u2 kh[H], km[H];
 #pragma unroll
@@ -721,6 +762,20 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           for (int nt = 0; nt < VT; nt++)
             S[mt][nt] = mfma32(u4{km[0].x, km[0].y, km[1].x, km[1].y},
                                u4{vq[0][nt].x, vq[0][nt].y, vq[1][nt].x, vq[1][nt].y}, S[mt][nt]);
+        }
+        if constexpr (TWO) {
+#pragma unroll
+          for (int nt = 0; nt < VT; nt++) {
+            const u2 x = vr[0][nt], y = vr[H - 1][nt];
+            if constexpr (H == 1) S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, km[0].x, km[0].y}, u4{x.x, x.y, x.x, x.y}, S[mt][nt]);
+            else S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, kh[1].x, kh[1].y}, u4{x.x, x.y, y.x, y.y}, S[mt][nt]);
+          }
+          if constexpr (FINE && H == 2) {
+#pragma unroll
+            for (int nt = 0; nt < VT; nt++)
+              S[mt][nt] = mfma32(u4{km[0].x, km[0].y, km[1].x, km[1].y},
+                                 u4{vr[0][nt].x, vr[0][nt].y, vr[1][nt].x, vr[1][nt].y}, S[mt][nt]);
+          }
         }
         if constexpr (FINE) {
           u2 kl[H];
@@ -1186,7 +1241,7 @@ static Splits splits_of(const ur3e_attn_t* a, int backward) {
   }
   Splits p = {1, a->t > 0 ? a->t : 1};
   /* three launches take ~13 us more than one, the time of ~7 chunks */
-  if (a->t < (a->dtype == UR3E_BF16 ? 192 : 128)) return p;
+  if (a->t < (a->dtype == UR3E_F32 ? 128 : 192)) return p;
   auto length = [&](long long n) { return (int)(((a->t + n - 1) / n + 15) / 16 * 16); };
   int least = 32;
   while ((long long)least * least * 4 < a->t) least += 16;
@@ -1222,8 +1277,11 @@ enum Phase { STATES, OUTPUTS };
 
 template <class T, int KT, int VT, bool STATE>
 static void walk_kernel(const WalkArgs& a, bool fine, dim3 grid, dim3 block, hipStream_t s) {
-  if constexpr (__is_same(T, Bf16)) {
-    /* two tiles of tokens at a time where there is more than one */
+  /* Two tiles of tokens at a time for bfloat16, where there is more than one and the registers hold them (2,048 x 512
+     tokens x 4 heads forward: 64 channels 487 us so; 128 channels 1.79 ms one at a time, 2.02 ms two at a time; half,
+     whose elements are two parts each, 572 us and 599 us) */
+  constexpr bool PAIRS = __is_same(T, Bf16) && KT < 8;
+  if constexpr (PAIRS) {
     if (a.t > 16) {
       if (fine) hipLaunchKernelGGL((k_attn_walk<T, KT, VT, STATE, 2, true>), grid, block, 0, s, a);
       else hipLaunchKernelGGL((k_attn_walk<T, KT, VT, STATE, 2, false>), grid, block, 0, s, a);
@@ -1231,8 +1289,10 @@ static void walk_kernel(const WalkArgs& a, bool fine, dim3 grid, dim3 block, hip
     }
   }
   /* (splits, and with them STATE, are for longer sequences) */
-  if constexpr (!STATE || !__is_same(T, Bf16))
-    hipLaunchKernelGGL((k_attn_walk<T, KT, VT, STATE, 1, true>), grid, block, 0, s, a);
+  if constexpr (!STATE || !PAIRS) {
+    if (sizeof(T) == 4 || fine) hipLaunchKernelGGL((k_attn_walk<T, KT, VT, STATE, 1, true>), grid, block, 0, s, a);
+    else if constexpr (sizeof(T) == 2) hipLaunchKernelGGL((k_attn_walk<T, KT, VT, STATE, 1, false>), grid, block, 0, s, a);
+  }
 }
 template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase phase, hipStream_t s) {
   const long long streams = (long long)a.b * a.h * a.nw * a.slabs;
