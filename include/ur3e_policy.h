@@ -8,12 +8,17 @@
  *     S_t = a_t S_{t-1} + k_t v_t^T        S_{-1} = s0 (0 when null), [dk][dv], float
  *     o_t = scale * S_t^T q_t
  * Tokens t >= lengths[b] are padding: their outputs and gradients are 0 and they leave the state alone; nothing
- * they hold is used.  Nothing in front of a start, whatever its values, reaches a token behind it.
+ * they hold is used.  Nothing in front of a start, whatever its values, reaches a token behind it.  log_decay is at
+ * most 0; -inf keeps the token alone.  What a NaN or an infinity reaches by the formula is not finite, and nothing else.
  *
  * Element types: 0 float, 1 bfloat16, 2 IEEE half, the same for every token tensor of a call.  States,
  * log_decay and all sums are float.  All pointers are device pointers on the current HIP device; strides
- * are in elements, the channels of a token are contiguous, token strides are not negative.  Work is enqueued on `stream`; nothing is kept
- * between calls, and a call may be captured into a graph.  Results do not depend on timing (no atomics).
+ * are in elements, the channels of a token are contiguous, token strides are not negative.  Outputs overlap nothing
+ * else.  Work is enqueued on `stream`; nothing is kept between calls, and a call may be captured into a graph; calls that
+ * may run at once need workspaces of their own.  Results do not depend on timing (no atomics).
+ *
+ * Limits: dk, dv in [1, 128]; b * heads below 2^22; t at most 2^30; with shared heads or less than four channels,
+ * b * t * heads * ceil(channels / 4) below 2^32 - 256.
  *
  * Errors: UR3E_EINVAL / UR3E_EHIP (ur3e_batch.h) with ur3e_last_error(); nothing is launched on EINVAL.
  */

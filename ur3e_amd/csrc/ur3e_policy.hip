@@ -2,21 +2,34 @@
  * dropout.
  *
  * Attention over a sequence (k_attn_walk).  One wave owns one (sequence, head, slab of value channels) and walks
- * its tokens in chunks of 16 with the state S [dk][slab] in registers.  With chunk-local positions i, j and
- * the state S that enters the chunk:
+ * its tokens in chunks with the state S [dk][slab] in registers.  With chunk-local positions i, j, n tokens in the
+ * chunk and the state S that enters it:
  *     o_i  = scale gamma^(i+1) S^T q_i + sum_{j <= i} scale gamma^(i-j) (q_i . k_j) v_j
  *     S'   = gamma^n S + sum_j gamma^(n-1-j) k_j v_j^T
- * All four products are 16 x 16 matrix instructions, and the register layouts chain without a trip through LDS:
- * the scores are formed transposed (P^T = K Q^T), which leaves them as the right operand of O^T = V^T P^T, and the
- * accumulators of S are the left operand of S^T Q^T as they stand.  That leaves two forms of a token
- * tile: "rows" (lane: one token, 4 x KT consecutive channels) and "columns" (lane: KT consecutive channels of four
- * tokens), both read straight from memory in whole cache lines.  Products are permutation invariant in the
- * contracted index, so channel d of a tile pair is KT * position + tile in either form.
+ * All four products are matrix instructions on tiles of 16 x 16, and the register layouts chain without a trip
+ * through LDS: the scores are formed transposed (P^T = K Q^T), which leaves them as the right operand of O^T = V^T P^T,
+ * and the accumulators of S are the left operand of S^T Q^T as they stand.  That leaves two forms of a token tile,
+ * "rows" (a lane holds one token's channels) and "columns" (a lane holds a few channels of four tokens), both read
+ * straight from memory.  Products do not care in which order the contracted index runs, so the channels are dealt
+ * to the tiles by what reads well (Place), the same way in either form.
+ *
+ * A chunk is a tile of 16 tokens, for bfloat16 of up to 64 key channels two of them.  Sequences that are too few to fill
+ * the card are split along time (splits_of): the sums of the splits first (STATE), joined into the state that enters
+ * each (k_attn_join), then all outputs at once.
+ *
+ * float is multiplied as float.  16-bit elements are multiplied as bfloat16 (a half is the exact sum of two), with
+ * the float operands, scores and state, in leading parts (split4).
  *
  * Gradients are the same walk with other operands.  G_t = scale q_t do_t^T + a_{t+1} G_{t+1} is the state
  * of the reversed sequence, so
  *     dq = walk(do, v, k) on S^T,  dk = reversed walk(v, do, q) on G^T,  dv = reversed walk(k, q, do) on G.
- */
+ *
+ * What bounds it (MI355X, a copy of 4 GiB runs at 4.75 TB/s): 2,048 sequences x 512 tokens x 4 heads of 64 channels take,
+ * forward, 487 us in bfloat16 (4.4 TB/s) and 915 us in float (4.7), bound by memory, and 532 us in half (4.0).  Their
+ * gradients take 1.19 ms in bfloat16 (3.2 TB/s of the tensors; the walks run against each other in time and read some of
+ * them twice), 2.76 ms in float, whose matrix instructions alone take 1.64, and 1.62 ms in half.  With 128 channels the
+ * vector instructions around the products bound it: 1.60 ms in bfloat16 (2.7 TB/s).  Short calls are chains of latencies: a
+ * chunk of 16 float tokens takes a lone wave 3.3 us, 2.1 us in a slab of 16 value channels. */
 #include <hip/hip_runtime.h>
 
 #include <stdint.h>
@@ -108,7 +121,7 @@ struct WalkArgs {
   int nw; /* walks of this launch, all of the same tile shape */
   int b, t, h, kdim, vdim, slabs, nsplit, split_len;
   int near; /* consecutive workgroups that share a sequence's tensors */
-  int chunk;     /* 16, or 1 where tokens lie too far apart for 30-bit offsets inside a chunk */
+  int chunk; /* 16, or 1 where tokens lie too far apart for 30-bit offsets inside a chunk */
   const float* log_decay;
   const unsigned char* starts;
   long long starts_sb, starts_st;
@@ -212,7 +225,7 @@ template <class T> struct Peak {
   }
 };
 
-/* bfloat16 fragments, two elements to a dword.  A 32-bit operand enters the matrix instructions as the sum of
+/* bfloat16 fragments of 16-bit tensors, two elements to a dword.  A 32-bit operand enters the matrix instructions as the sum of
    its leading parts of 8 bits each: two (error 2^-17) for scores and state, whose results are rounded to 2^-9
    on the way out, three (2^-25) for what is added to the state. */
 __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
@@ -287,9 +300,10 @@ template <class T, int KT> __device__ __forceinline__ void pack_row(const Row<T,
     y[mt] = u2{halves(r.x[0], mt, r.x[1 / C], 1 % C * KT + mt), halves(r.x[2 / C], 2 % C * KT + mt, r.x[3 / C], 3 % C * KT + mt)};
 }
 
-/* KT, VT: tiles of 16 key channels and of 16 value channels per wave.  STATE: only the state at the end of
-   each split (from zero), for sequences that several waves share.  FINE (bfloat16): a state leaves as floats and is
-   summed to their precision, from keys in three parts; where it only feeds 16-bit outputs, from keys in two. */
+/* KT, VT: tiles of 16 key channels and of 16 value channels per wave; H: tiles of 16 tokens per chunk.  STATE: only the state at the end of
+   each split (from zero), for sequences that several waves share.  FINE (16-bit types): a state leaves as floats and is
+   summed to their precision, from keys in three parts; where it only feeds 16-bit outputs, from keys in two (of the
+   products of two parts of a half, that of the two rests, 2^-18, is left out then where it is not free). */
 template <class T, int KT, int VT, bool STATE, int H, bool FINE>
 __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   constexpr int ES = (int)sizeof(T), C = 16 * H;
@@ -919,7 +933,7 @@ template <class T> __global__ __launch_bounds__(256) void k_attn_pack(PackArgs a
    X_s = wf[s] X_{s-1} + ws[s], X_0 = s_in.  Nothing but the chain of multiply-adds depends on the split in front.
 
    Many sequences: a thread owns VW elements and runs along the splits, whose sums it loads LOT at a time, the next
-   lot while one is chained; the bytes bound it.  (A factor of 0 is an episode start: what was in front of it is
+   lot while one is chained; the bytes bound it (both directions of eight demonstrations of 10,500 tokens: 15.6 us).  (A factor of 0 is an episode start: what was in front of it is
    dropped whatever it holds.) */
 __device__ __forceinline__ float carry_on(float f, float x, float u) {
   const float y = f * x;
@@ -961,7 +975,8 @@ template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(Wal
 }
 /* Few sequences wait for the chain: the waves of a workgroup take 32 splits each of the same 64 elements, all loads at
    once, chain their own from zero and pass on the result and the product of their factors; each then starts from
-   what the waves in front make of the state.  219 splits of one demonstration: 15.7 us by the kernel above. */
+   what the waves in front make of the state.  The 219 splits of one demonstration of 10,500 tokens take 7.1 us, by the
+   kernel above 15.7. */
 #define JOIN_WAVES 16
 __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attn_join_wide(WalkArgs a) {
   constexpr int LOT = 32;
@@ -1009,7 +1024,8 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attn_join_wide(WalkArgs a) 
 
 /* Sums of the per-query-head gradients over the `grp` heads that share a key / value head: rows of `width` floats,
    [b][t][hk][grp][width], to d channels of [b][t][hk] rows.  With grp = 1 it narrows the rows of less than four
-   channels that the walks write eight wide.  A thread sums four channels; every tensor of a call in one launch. */
+   channels that the walks write eight wide.  A thread sums four channels; every tensor of a call in one launch.  Memory bounds
+   it: 33 x 777 tokens, 6 heads over 2, 48 + 96 channels take 16.4 us (6.2 TB/s: they come from the Infinity Cache). */
 struct SumArgs {
   struct One {
     const float* src;
@@ -1052,7 +1068,8 @@ template <class T> __global__ __launch_bounds__(256) void k_attn_group_sum(SumAr
 }
 
 /* ---- one token -----------------------------------------------------------------------------------
-   The state is read and written once and bounds the call: 4,096 envs x 4 heads of 64 x 64 take 108 us, 5.1 TB/s.
+   The state is read and written once and bounds the call: 4,096 envs x 4 heads of 64 x 64 take 102 us,
+   5.4 TB/s (one env: 4.8 us, a launch and two trips to memory).
    A wave owns one (sequence, head) and a slab of CL groups of VW value channels: its lanes are the groups by 64 / CL
    rows, which they stream ROWS at a time: S' = a S + k v^T stored, o += q S' kept per lane and summed over the rows
    at the end.  Few sequences are cut into narrower slabs, so that more waves share their rows. */
@@ -1138,7 +1155,9 @@ __device__ __forceinline__ void philox(unsigned c0, unsigned c1, unsigned c2, un
   out[0] = c0; out[1] = c1; out[2] = c2; out[3] = c3;
 }
 
-/* a thread takes the 8 columns of one Philox call */
+/* A thread takes the 8 columns of one Philox call, so 131,072 x 256 bfloat16 with a residual, and the gradient, take 64 us,
+   5.2 TB/s: memory bounds it, with ten rounds of products per 8 elements beside.  A row that ends inside a block, or is not
+   on a boundary of 16 bytes, is read element by element: 4,097 x 101 in half take 3.5 us. */
 template <class T, bool VEC>
 __global__ __launch_bounds__(256) void k_keyed_dropout(long long rows, int cols, const T* x, long long xs, const T* res,
                                                        long long rs, T* y, long long ys, const long long* ids,

@@ -14,8 +14,10 @@ feature extractor over stacked frames (gymnasium_src/scripts/regular_rl/rl/train
 
 GPU tensors go through the HIP library, on torch's current stream of their device, whatever the current
 device is; a missing library raises.  CPU tensors are computed with elementary torch operations.  The calls
-never synchronise and may be captured into HIP graphs.  Wrong arguments raise ValueError (TypeError for what is
-no tensor) before any launch.  Gradients are not differentiable again.
+never synchronise and may be captured into HIP graphs, forward and backward; RuntimeError where an eager graph of the
+default stream still holds one of the leaves, which torch cannot capture a backward pass of.  Wrong arguments raise
+ValueError (TypeError for what is no tensor) before any launch.  Gradients are not differentiable again.
+Results do not depend on timing: the same call gives the same bits.
 """
 from __future__ import annotations
 
@@ -90,8 +92,8 @@ def decay_attention(q, k, v, log_decay, initial_state=None, starts=None, lengths
     q [B, T, H, dk], k [B, T, Hk, dk], v [B, T, Hk, dv]: float32, bfloat16 or float16 (all the same), 1 to 128
       channels, any strides (a rollout buffer [T, B, ...] is passed as its transpose).  Query head h reads key
       / value head h // (H // Hk).
-    log_decay [H] float32: a head's state is multiplied by exp(log_decay) a token; 0 never forgets, -inf keeps
-      the token alone.  A constant: it gets no gradient.
+    log_decay [H] float32, at most 0 (not checked): a head's state is multiplied by exp(log_decay) a token; 0 never
+      forgets, -inf keeps the token alone (of states that are finite).  A constant: it gets no gradient.
     initial_state [B, H, dk, dv] float32: the state in front of the first token (default 0).
     starts [B, T] bool or uint8: nonzero where an episode starts; the state in front of that token is dropped.
     lengths [B] int32: the tokens of each sequence (clamped to [0, T]); the rest of a row is padding, which is
@@ -99,7 +101,9 @@ def decay_attention(q, k, v, log_decay, initial_state=None, starts=None, lengths
     scale: of the outputs, default dk ** -0.5.
 
     Returns (out [B, T, H, dv] of q's type, state): the state [B, H, dk, dv] float32 behind each sequence's
-    last token, or None without `return_state`.  States and sums are float32.
+    last token, or None without `return_state`.  States and sums are float32.  What a NaN or an infinity reaches by the
+    formula is not finite (a NaN where the formula may say infinity); nothing else is touched by it.
+    B * H must be below 2**22 and T at most 2**30.
     """
     _tensor("decay_attention", "q", q)
     if scale is None:
