@@ -25,10 +25,10 @@
  *     dq = walk(do, v, k) on S^T,  dk = reversed walk(v, do, q) on G^T,  dv = reversed walk(k, q, do) on G.
  *
  * What bounds it (MI355X, a copy of 4 GiB runs at 4.75 TB/s): 2,048 sequences x 512 tokens x 4 heads of 64 channels take,
- * forward, 487 us in bfloat16 (4.4 TB/s) and 915 us in float (4.7), bound by memory, and 532 us in half (4.0).  Their
- * gradients take 1.19 ms in bfloat16 (3.2 TB/s of the tensors; the walks run against each other in time and read some of
- * them twice), 2.76 ms in float, whose matrix instructions alone take 1.64, and 1.62 ms in half.  With 128 channels the
- * vector instructions around the products bound it: 1.60 ms in bfloat16 (2.7 TB/s).  Short calls are chains of latencies: a
+ * forward, 487 us in bfloat16 (4.4 TB/s) and 915 us in float (4.7), bound by memory, and 488 us in half (4.4).  Their
+ * gradients take 1.17 ms in bfloat16 (3.2 TB/s of the tensors; the walks run against each other in time and read some of
+ * them twice), 2.63 ms in float, whose matrix instructions alone take 1.64, and 1.46 ms in half.  With 128 channels the
+ * vector instructions around the products bound it: 1.51 ms in bfloat16 (2.9 TB/s).  Short calls are chains of latencies: a
  * chunk of 16 float tokens takes a lone wave 3.3 us, 2.1 us in a slab of 16 value channels. */
 #include <hip/hip_runtime.h>
 
@@ -48,6 +48,7 @@ int ur3e_internal_fail(int code, const char* msg);
 typedef float f4 __attribute__((ext_vector_type(4)));
 typedef unsigned u2 __attribute__((ext_vector_type(2)));
 typedef unsigned u4 __attribute__((ext_vector_type(4)));
+typedef unsigned u6 __attribute__((ext_vector_type(6)));
 
 struct Bf16 { unsigned short x; };
 typedef _Float16 F16;
@@ -128,6 +129,10 @@ struct WalkArgs {
   const int* lengths;
 };
 
+/* a value that all lanes share, in a scalar register */
+__device__ __forceinline__ float uniform(float x) {
+  return __builtin_bit_cast(float, __builtin_amdgcn_readfirstlane(__builtin_bit_cast(int, x)));
+}
 /* gamma^n with gamma^0 = 1 whatever gamma (log_decay = -inf is a head without memory) */
 __device__ __forceinline__ float pw(float l, int n) { return n == 0 ? 1.0f : expf((float)n * l); }
 
@@ -249,11 +254,23 @@ template <class T> __device__ __forceinline__ f4 mfma_raw(u4 a, u4 b, f4 c) {
    becomes the rest, x - hi, a product with the negative unit matrix: one instruction of the matrix pipe
    in place of eight of the vector pipe, which is the busier one.  Exact: every sum has one product.  An infinity
    or a NaN spreads to the rest of its column, whose elements all feed the same result. */
-__device__ __forceinline__ u2 split4(f4& x, u2 minus_one) {
+__device__ __forceinline__ u2 split4(f4& x, u6 minus_one) {
   const u2 hi = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])};
-  x = mfma32(u4{minus_one.x, minus_one.y, 0, 0}, u4{hi.x, hi.y, 0, 0}, x);
+  x = mfma32(__builtin_shufflevector(minus_one, minus_one, 0, 1, 2, 3), u4{hi.x, hi.y, 0, 0}, x);
   return hi;
 }
+/* Two at once, packed next to each other: the unit matrix stands in the half of the contraction that is the tile's, so
+   nothing is padded with zeros (which would be moves: the operands are whole quads of registers). */
+__device__ __forceinline__ u4 split4x2(f4& x, f4& y, u6 minus_one) {
+  const u4 hi = {pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+  x = mfma32(__builtin_shufflevector(minus_one, minus_one, 0, 1, 2, 3), hi, x);
+  y = mfma32(__builtin_shufflevector(minus_one, minus_one, 2, 3, 4, 5), hi, y);
+  return hi;
+}
+__device__ __forceinline__ u4 pack4x2(f4 x, f4 y) {
+  return u4{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3]), pack_bf16(y[0], y[1]), pack_bf16(y[2], y[3])};
+}
+__device__ __forceinline__ u4 both(u2 x, u2 y) { return u4{x.x, x.y, y.x, y.y}; }
 __device__ __forceinline__ u2 pack4(f4 x) { return u2{pack_bf16(x[0], x[1]), pack_bf16(x[2], x[3])}; }
 
 /* Which channels position 4 g + e of N tiles stands for: N consecutive ones from `of` on.  Groups e lie so that the
@@ -370,7 +387,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   /* o[e][nt]: channel of(g, e) + nt of this lane's token */
   auto put = [&](Rsrc ro, unsigned rel, bool there, const float (&o)[4][VT]) {
     const unsigned orow = at(rel * (unsigned)ost, there, FAR_T);
-    if (w.out_f32) {
+    int wide = w.out_f32;
+    asm volatile("" : "+s"(wide)); /* (tested here: as a condition kept through the loop it was spilled) */
+    if (wide) {
 #pragma unroll
       for (int e = 0; e < 4; e++)
         store_n<float, VT>(ro, orow + at(4 * (v0 + PV::of(g, e, vleft, -v0)), PV::there(g, e, vleft), FAR_D), o[e]);
@@ -456,9 +475,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
       dm[f][e] = d >= 0 ? w.p_scale * pw(l, d) : 0.0f;
     }
   }
-  const float fi = w.in_scale * pw(l, idx + e0), g16 = pw(l, 16);
+  const float fi = w.in_scale * pw(l, idx + e0), g16 = uniform(pw(l, 16));
   const unsigned unit = idx >> 2 != g ? 0u : idx & 1 ? 0xbf800000u : 0xbf80u;
-  const u2 minus_one = {idx & 2 ? 0u : unit, idx & 2 ? unit : 0u}; /* this lane's part of the negative unit matrix */
+  /* this lane's part of the negative unit matrix, zeros, and the same again: its registers serve either half */
+  u6 minus_one = {idx & 2 ? 0u : unit, idx & 2 ? unit : 0u, 0, 0, idx & 2 ? 0u : unit, idx & 2 ? unit : 0u};
+  asm volatile("" : "+v"(minus_one));
   float gn = 1.0f;
 
   float through = 1.0f; /* STATE: what the split multiplies an entering state by */
@@ -529,7 +550,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   auto work = [&](Chunk& c) {
     if (n != scaled) {
       scaled = n;
-      gn = pw(l, n);
+      gn = uniform(pw(l, n));
       const int n0 = n > 16 ? 16 : n, j0 = fresh(4 * g);
 #pragma unroll
       for (int e = 0; e < 4; e++) {
@@ -600,14 +621,13 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
             for (int i = 0; i < Raw<T, KT>::D; i++) c.kc[f][e].d[i] = ok ? c.kc[f][e].d[i] : 0;
           }
-      } else {
-#pragma unroll
-        for (int mt = 0; mt < KT; mt++)
-#pragma unroll
-          for (int nt = 0; nt < VT; nt++)
-#pragma unroll
-            for (int e = 0; e < 4; e++) S[mt][nt][e] *= gn;
       }
+#pragma unroll
+      for (int mt = 0; mt < KT; mt++)
+#pragma unroll
+        for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) S[mt][nt][e] *= gn;
     };
     const float ahead = H == 2 && n > 16 ? g16 : 1.0f; /* tile 0, where another one follows */
     auto key = [&](int f, int mt, int e) { /* as it enters the state */
@@ -658,37 +678,51 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
             }
         f4 x[H][VT];
 #pragma unroll
-        for (int mt = 0; mt < KT; mt++) {
-          u2 qs[H]; /* the rests of the queries; the leading parts take the elements' place */
-          if constexpr (TWO) {
+        for (int i = 0; i < (KT + 1) / 2; i++) {
+          constexpr int STEP = KT > 1;
+          const int m0 = 2 * i, m1 = 2 * i + STEP;
+          u4 qh[H], ql[H]; /* queries: leading part and rest */
 #pragma unroll
-            for (int f = 0; f < H; f++) {
-              f4 y;
-#pragma unroll
-              for (int e = 0; e < 4; e++) y[e] = c.qr[f].get(e, mt);
-              qq[f][mt] = split4(y, minus_one);
-              qs[f] = pack4(y);
-            }
-          }
-#pragma unroll
-          for (int nt = 0; nt < VT; nt++) {
-            f4 rest = S[mt][nt];
-            const u2 hi = split4(rest, minus_one), lo = pack4(rest);
+          for (int f = 0; f < H; f++) {
             if constexpr (TWO) {
+              f4 y, z;
 #pragma unroll
-              for (int f = 0; f < H; f++)
-                x[f][nt] = mfma32(u4{hi.x, hi.y, lo.x, lo.y}, u4{qs[f].x, qs[f].y, qs[f].x, qs[f].y}, mt ? x[f][nt] : f4{0, 0, 0, 0});
+              for (int e = 0; e < 4; e++) {
+                y[e] = c.qr[f].get(e, m0);
+                z[e] = c.qr[f].get(e, m1);
+              }
+              qh[f] = split4x2(y, z, minus_one);
+              ql[f] = pack4x2(y, z);
+            } else qh[f] = both(qq[f][m0], qq[f][m1]);
+          }
+          u4 lo; /* of the tile in front, whose products wait for this one's: they add to the same accumulators */
+#pragma unroll
+          for (int nt = 0; nt <= VT; nt++) {
+            u4 next;
+            if (nt < VT) {
+              f4 r0 = S[m0][nt], r1 = S[m1][nt];
+              if constexpr (KT == 1) r1 = f4{0, 0, 0, 0};
+              const u4 hi = split4x2(r0, r1, minus_one);
+#pragma unroll
+              for (int f = 0; f < H; f++) {
+                x[f][nt] = mfma32(hi, qh[f], i ? x[f][nt] : f4{0, 0, 0, 0});
+                if constexpr (TWO) x[f][nt] = mfma32(hi, ql[f], x[f][nt]);
+              }
+              next = pack4x2(r0, r1);
             }
+            if (nt > 0) {
 #pragma unroll
-            for (int f = 0; f < H; f++)
-              x[f][nt] = mfma32(u4{hi.x, hi.y, lo.x, lo.y}, u4{qq[f][mt].x, qq[f][mt].y, qq[f][mt].x, qq[f][mt].y},
-                                TWO || mt ? x[f][nt] : f4{0, 0, 0, 0});
+              for (int f = 0; f < H; f++) x[f][nt - 1] = mfma32(lo, qh[f], x[f][nt - 1]);
+            }
+            lo = next;
           }
         }
 #pragma unroll
         for (int f = 0; f < H; f++) {
 #pragma unroll
-          for (int nt = 0; nt < VT; nt++) x[f][nt] *= f ? fi * g16 : fi;
+          for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+            for (int e = 0; e < 4; e++) x[f][nt][e] *= f ? fi * g16 : fi;
 #pragma unroll
           for (int fk = 0; fk <= f; fk++) scores(pt[f][fk], f, fk);
         }
@@ -707,37 +741,30 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           }
         }
         if (TWO) values(); /* (where registers are not needed for queries and scores any more) */
-        u2 ph[H][H], pl[H][H]; /* leading part and rest */
+        /* leading parts and rests of the scores */
+        u2 ph, pl;
+        u4 ph1 = {}, pl1 = {};
+        ph = split4(pt[0][0], minus_one);
+        pl = pack4(pt[0][0]);
+        if constexpr (H == 2) {
+          ph1 = split4x2(pt[1][0], pt[1][1], minus_one);
+          pl1 = pack4x2(pt[1][0], pt[1][1]);
+        }
 #pragma unroll
-        for (int fq = 0; fq < H; fq++)
+        for (int nt = 0; nt < VT; nt++) {
+          x[0][nt] = mfma32(both(vq[0][nt], vq[0][nt]), both(ph, pl), x[0][nt]);
+          if constexpr (H == 2) x[1][nt] = mfma32(both(vq[0][nt], vq[1][nt]), ph1, x[1][nt]);
+        }
+        if constexpr (H == 2) {
 #pragma unroll
-          for (int fk = 0; fk <= fq; fk++) {
-            ph[fq][fk] = split4(pt[fq][fk], minus_one);
-            pl[fq][fk] = pack4(pt[fq][fk]);
-          }
-#pragma unroll
-        for (int f = 0; f < H; f++)
-#pragma unroll
-          for (int nt = 0; nt < VT; nt++) {
-            const u2 y = vq[0][nt], yf = vq[f][nt], z = ph[f][0], zl = pl[f][0], zf = ph[f][f];
-            if (f == 0) x[f][nt] = mfma32(u4{y.x, y.y, y.x, y.y}, u4{z.x, z.y, zl.x, zl.y}, x[f][nt]);
-            else x[f][nt] = mfma32(u4{y.x, y.y, yf.x, yf.y}, u4{z.x, z.y, zf.x, zf.y}, x[f][nt]);
-          }
-#pragma unroll
-        for (int f = 1; f < H; f++)
-#pragma unroll
-          for (int nt = 0; nt < VT; nt++)
-            x[f][nt] = mfma32(u4{vq[0][nt].x, vq[0][nt].y, vq[f][nt].x, vq[f][nt].y},
-                              u4{pl[f][0].x, pl[f][0].y, pl[f][f].x, pl[f][f].y}, x[f][nt]);
+          for (int nt = 0; nt < VT; nt++) x[1][nt] = mfma32(both(vq[0][nt], vq[1][nt]), pl1, x[1][nt]);
+        }
         if constexpr (TWO) {
 #pragma unroll
-          for (int f = 0; f < H; f++)
-#pragma unroll
-            for (int nt = 0; nt < VT; nt++) {
-              const u2 y = vr[0][nt], yf = vr[f][nt], z = ph[f][0], zl = pl[f][0], zf = ph[f][f];
-              if (f == 0) x[f][nt] = mfma32(u4{y.x, y.y, y.x, y.y}, u4{z.x, z.y, zl.x, zl.y}, x[f][nt]);
-              else x[f][nt] = mfma32(u4{y.x, y.y, yf.x, yf.y}, u4{z.x, z.y, zf.x, zf.y}, x[f][nt]);
-            }
+          for (int nt = 0; nt < VT; nt++) {
+            x[0][nt] = mfma32(both(vr[0][nt], vr[0][nt]), both(ph, pl), x[0][nt]);
+            if constexpr (H == 2) x[1][nt] = mfma32(both(vr[0][nt], vr[1][nt]), ph1, x[1][nt]);
+          }
         }
 #pragma unroll
         for (int f = 0; f < H; f++) {
@@ -754,55 +781,47 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
       for (int mt = 0; mt < KT; mt++) {
         f4 kx[H];
-        u2 kh[H], km[H];
 #pragma unroll
-        for (int f = 0; f < H; f++) {
+        for (int f = 0; f < H; f++)
 #pragma unroll
           for (int e = 0; e < 4; e++) kx[f][e] = key(f, mt, e);
-          kh[f] = split4(kx[f], minus_one);
-          km[f] = pack4(kx[f]);
-        }
-#pragma unroll
-        for (int nt = 0; nt < VT; nt++) {
-          const u2 x = vq[0][nt], y = vq[H - 1][nt];
-          if constexpr (H == 1) {
-            S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, km[0].x, km[0].y}, u4{x.x, x.y, x.x, x.y}, S[mt][nt]);
-          } else {
-            S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, kh[1].x, kh[1].y}, u4{x.x, x.y, y.x, y.y}, S[mt][nt]);
-          }
-        }
         if constexpr (H == 2) {
+          const u4 kh = split4x2(kx[0], kx[1], minus_one);
+          u4 km;
+          if constexpr (FINE) km = split4x2(kx[0], kx[1], minus_one);
+          else km = pack4x2(kx[0], kx[1]);
 #pragma unroll
-          for (int nt = 0; nt < VT; nt++)
-            S[mt][nt] = mfma32(u4{km[0].x, km[0].y, km[1].x, km[1].y},
-                               u4{vq[0][nt].x, vq[0][nt].y, vq[1][nt].x, vq[1][nt].y}, S[mt][nt]);
-        }
-        if constexpr (TWO) {
+          for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma32(kh, both(vq[0][nt], vq[1][nt]), S[mt][nt]);
 #pragma unroll
-          for (int nt = 0; nt < VT; nt++) {
-            const u2 x = vr[0][nt], y = vr[H - 1][nt];
-            if constexpr (H == 1) S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, km[0].x, km[0].y}, u4{x.x, x.y, x.x, x.y}, S[mt][nt]);
-            else S[mt][nt] = mfma32(u4{kh[0].x, kh[0].y, kh[1].x, kh[1].y}, u4{x.x, x.y, y.x, y.y}, S[mt][nt]);
+          for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma32(km, both(vq[0][nt], vq[1][nt]), S[mt][nt]);
+          if constexpr (FINE) {
+            const u4 kl = pack4x2(kx[0], kx[1]);
+#pragma unroll
+            for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma32(kl, both(vq[0][nt], vq[1][nt]), S[mt][nt]);
           }
-          if constexpr (FINE && H == 2) {
+          if constexpr (TWO) {
 #pragma unroll
-            for (int nt = 0; nt < VT; nt++)
-              S[mt][nt] = mfma32(u4{km[0].x, km[0].y, km[1].x, km[1].y},
-                                 u4{vr[0][nt].x, vr[0][nt].y, vr[1][nt].x, vr[1][nt].y}, S[mt][nt]);
+            for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma32(kh, both(vr[0][nt], vr[1][nt]), S[mt][nt]);
+            if constexpr (FINE) {
+#pragma unroll
+              for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma32(km, both(vr[0][nt], vr[1][nt]), S[mt][nt]);
+            }
           }
-        }
-        if constexpr (FINE) {
-          u2 kl[H];
+        } else {
+          const u2 kh = split4(kx[0], minus_one);
+          u2 km;
+          if constexpr (FINE) km = split4(kx[0], minus_one);
+          else km = pack4(kx[0]);
 #pragma unroll
-          for (int f = 0; f < H; f++) {
-            (void)split4(kx[f], minus_one);
-            kl[f] = pack4(kx[f]);
+          for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma32(both(kh, km), both(vq[0][nt], vq[0][nt]), S[mt][nt]);
+          if constexpr (TWO) {
+#pragma unroll
+            for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma32(both(kh, km), both(vr[0][nt], vr[0][nt]), S[mt][nt]);
           }
+          if constexpr (FINE) {
+            const u2 kl = pack4(kx[0]);
 #pragma unroll
-          for (int nt = 0; nt < VT; nt++) {
-            const u2 x = vq[0][nt], y = vq[H - 1][nt];
-            const u4 z = {x.x, x.y, H == 1 ? 0 : y.x, H == 1 ? 0 : y.y};
-            S[mt][nt] = mfma32(u4{kl[0].x, kl[0].y, H == 1 ? 0 : kl[H - 1].x, H == 1 ? 0 : kl[H - 1].y}, z, S[mt][nt]);
+            for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma32(both(kl, u2{0, 0}), both(vq[0][nt], vq[0][nt]), S[mt][nt]);
           }
         }
       }
@@ -827,7 +846,9 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
         for (int e = 0; e < 4; e++) pt[e] = (part[0][e] + part[1][e]) + (part[2][e] + part[3][e]);
         scores(pt, 0, 0);
 #pragma unroll
-        for (int nt = 0; nt < VT; nt++) x[nt] *= fi;
+        for (int nt = 0; nt < VT; nt++)
+#pragma unroll
+          for (int e = 0; e < 4; e++) x[nt][e] *= fi;
         if (cut) {
           cut_scores(pt, 0, 0);
 #pragma unroll
