@@ -13,7 +13,7 @@
  * straight from memory.  Products do not care in which order the contracted index runs, so the channels are dealt
  * to the tiles by what reads well (Place), the same way in either form.
  *
- * A chunk is a tile of 16 tokens, for bfloat16 of up to 64 key channels two of them.  Sequences that are too few to fill
+ * A chunk is a tile of 16 tokens, for 16-bit types of up to 64 key channels two of them.  Sequences that are too few to fill
  * the card are split along time (splits_of): the sums of the splits first (STATE), joined into the state that enters
  * each (k_attn_join), then all outputs at once.
  *
@@ -25,9 +25,9 @@
  *     dq = walk(do, v, k) on S^T,  dk = reversed walk(v, do, q) on G^T,  dv = reversed walk(k, q, do) on G.
  *
  * What bounds it (MI355X, a copy of 4 GiB runs at 4.75 TB/s): 2,048 sequences x 512 tokens x 4 heads of 64 channels take,
- * forward, 487 us in bfloat16 (4.4 TB/s) and 915 us in float (4.7), bound by memory, and 488 us in half (4.4).  Their
+ * forward, 487 us in bfloat16 (4.4 TB/s) and 915 us in float (4.7), bound by memory, and 484 us in half (4.4).  Their
  * gradients take 1.17 ms in bfloat16 (3.2 TB/s of the tensors; the walks run against each other in time and read some of
- * them twice), 2.63 ms in float, whose matrix instructions alone take 1.64, and 1.46 ms in half.  With 128 channels the
+ * them twice), 2.63 ms in float, whose matrix instructions alone take 1.64, and 1.34 ms in half.  With 128 channels the
  * vector instructions around the products bound it: 1.51 ms in bfloat16 (2.9 TB/s).  Short calls are chains of latencies: a
  * chunk of 16 float tokens takes a lone wave 3.3 us, 2.1 us in a slab of 16 value channels. */
 #include <hip/hip_runtime.h>
@@ -62,6 +62,12 @@ template <> __device__ __forceinline__ float from_f<float>(float x) { return x; 
 template <> __device__ __forceinline__ F16 from_f<F16>(float x) { return (F16)x; }
 template <> __device__ __forceinline__ Bf16 from_f<Bf16>(float x) {
   return __builtin_bit_cast(Bf16, (__bf16)x);
+}
+
+/* two bfloat16 in a dword */
+__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
+  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
+  return __builtin_bit_cast(unsigned, b2{(__bf16)lo, (__bf16)hi});
 }
 
 /* N consecutive elements; VEC: aligned to min(16, N * sizeof(T)) bytes */
@@ -194,6 +200,7 @@ template <class T, int N> __device__ __forceinline__ void store_n(Rsrc r, unsign
   for (int i = 0; i < N; i += sizeof(T) == 4 ? 1 : 2) {
     if constexpr (sizeof(T) == 4) d[i] = __builtin_bit_cast(unsigned, x[i]);
     else if constexpr (N == 1) d[0] = __builtin_bit_cast(unsigned short, from_f<T>(x[0]));
+    else if constexpr (__is_same(T, Bf16)) d[i / 2] = pack_bf16(x[i], x[i + 1]); /* one conversion for both */
     else {
       struct Two { T a, b; };
       d[i / 2] = __builtin_bit_cast(unsigned, Two{from_f<T>(x[i]), from_f<T>(x[i + 1])});
@@ -233,10 +240,6 @@ template <class T> struct Peak {
 /* bfloat16 fragments of 16-bit tensors, two elements to a dword.  A 32-bit operand enters the matrix instructions as the sum of
    its leading parts of 8 bits each: two (error 2^-17) for scores and state, whose results are rounded to 2^-9
    on the way out, three (2^-25) for what is added to the state. */
-__device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
-  typedef __bf16 b2 __attribute__((ext_vector_type(2)));
-  return __builtin_bit_cast(unsigned, b2{(__bf16)lo, (__bf16)hi});
-}
 /* the K = 32 shape throughout, half empty where four elements are all there is: a K = 16 instruction right behind
    a K = 32 one on the same accumulators read them before the first had written (the compiler had put one wait
    state between the two; measured at one tile, where nothing else stands between them) */
@@ -1317,10 +1320,10 @@ enum Phase { STATES, OUTPUTS };
 
 template <class T, int KT, int VT, bool STATE>
 static void walk_kernel(const WalkArgs& a, bool fine, dim3 grid, dim3 block, hipStream_t s) {
-  /* Two tiles of tokens at a time for bfloat16, where there is more than one and the registers hold them (2,048 x 512
-     tokens x 4 heads forward: 64 channels 487 us so; 128 channels 1.79 ms one at a time, 2.02 ms two at a time; half,
-     whose elements are two parts each, 572 us and 599 us) */
-  constexpr bool PAIRS = __is_same(T, Bf16) && KT < 8;
+  /* Two tiles of tokens at a time for 16-bit types, where there is more than one and the registers hold them (2,048 x 512
+     tokens x 4 heads, gradients, two tiles at a time and one: 64 channels bfloat16 1.16 and 1.37 ms, half 1.34 and 1.46; 128
+     channels bfloat16 4.43 and 4.25) */
+  constexpr bool PAIRS = sizeof(T) == 2 && KT < 8;
   if constexpr (PAIRS) {
     if (a.t > 16) {
       if (fine) hipLaunchKernelGGL((k_attn_walk<T, KT, VT, STATE, 2, true>), grid, block, 0, s, a);
