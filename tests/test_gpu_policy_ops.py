@@ -71,14 +71,14 @@ def test_attention_every_channel_count(first, dtype):
         check_all(*make(1, 19, 2, 1, d, dv, DT[dtype], seed=d))
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("dk,dv", [(2, 3), (3, 66), (66, 1), (3, 3), (100, 70), (45, 45)])
 def test_attention_odd_rows_in_splits(dk, dv, dtype):
     """rows of less than four channels and rows that fill no tile, over several waves a sequence, ragged, with starts"""
     check_all(*make(3, 400, 4, 2, dk, dv, DT[dtype], seed=dk, starts=0.02, lengths=[400, 0, 333]))
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("t,starts,time_major", [(16, 0.3, True), (37, 0.1, False), (40, 1.0, True), (400, 0.02, False),
                                                  (400, 0.5, True)])
 def test_attention_starts_and_lengths(t, starts, time_major, dtype):
@@ -143,7 +143,7 @@ def test_attention_lengths_are_clamped():
     assert all(torch.equal(got[n], want[n]) for n in got)
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_attention_decay_ends(dtype):
     """exp(log_decay) = 0 keeps the token alone, 1 never forgets, and 1 - 2^-12 forgets slowly"""
     x, dout, dfinal = make(2, 300, 3, 3, 32, 32, DT[dtype], decay=[float("-inf"), 0.0, -2.0 ** -12])
@@ -155,7 +155,7 @@ def test_attention_decay_ends(dtype):
 
 
 @pytest.mark.parametrize("t", [32, 300])
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
 def test_attention_what_masks_hide_stays_hidden(t, dtype, value):
     """padding, the tokens and the state in front of a start, and later tokens never reach a token, whatever they hold"""
@@ -379,7 +379,7 @@ def test_capture_refuses_leaves_of_a_live_eager_graph():
         assert torch.equal(got, want)
 
 
-@pytest.mark.parametrize("dtype", ["f32", "bf16"])
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
 def test_nothing_to_do(dtype):
     """no sequences, no tokens, no rows, no columns"""
     from ur3e_amd.rl import ops

@@ -114,6 +114,19 @@ def test_step_refuses():
             ops.decay_attention_step(**{**x, **change})
 
 
+@pytest.mark.parametrize("name", ["q", "k", "v", "state"])
+def test_step_refuses_gradients(name):
+    """a step that autograd would take for a constant is refused; under no_grad the same call runs"""
+    x = dict(q=torch.ones(2, 2, 4), k=torch.ones(2, 2, 4), v=torch.ones(2, 2, 4), log_decay=torch.zeros(2),
+             state=torch.zeros(2, 2, 4, 4))
+    x[name].requires_grad_()
+    with pytest.raises(ValueError, match="no gradients"):
+        ops.decay_attention_step(**x)
+    with torch.no_grad():
+        out = ops.decay_attention_step(**x)
+    assert not out.requires_grad and (out == 2.0).all() and (x["state"].detach() == 1.0).all()
+
+
 def test_philox_known_answers():
     """Random123's kat_vectors for philox4x32 with 10 rounds"""
     kat = [(0, (0, 0), 0, "6627e8d5 e169c58d bc57ac4c 9b00dbd8"),

@@ -134,6 +134,8 @@ void check_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor&
   check_attention(what, 3, q, k, v, log_decay, starts, scale);
   check_state(what, "state", state, q, v);
   TORCH_CHECK_VALUE(state.is_contiguous(), what, ": state must be contiguous");
+  TORCH_CHECK_VALUE(!at::GradMode::is_enabled() || !(q.requires_grad() || k.requires_grad() || v.requires_grad() || state.requires_grad()),
+                    what, ": one token has no gradients; call it under torch.no_grad(), or decay_attention");
   if (next) {
     TORCH_CHECK_VALUE(update, what, ": next_state without an update");
     check_state(what, "next_state", *next, q, v);
@@ -247,8 +249,8 @@ std::pair<Tensor, OptT> decay_attention(const Tensor& q, const Tensor& k, const 
 
 Tensor decay_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, Tensor state,
                             const OptT& starts, double scale, const OptT& next, bool update) {
-  at::NoGradGuard no_grad;
   check_step(q, k, v, log_decay, state, starts, scale, next, update);
+  at::NoGradGuard no_grad;
   c10::DeviceGuard guard(q.device());
   const Tensor q1 = unit(q), k1 = unit(k), v1 = unit(v), ld = log_decay.contiguous();
   Tensor out = at::empty({q.size(0), q.size(1), v.size(2)}, q.options());

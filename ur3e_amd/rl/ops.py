@@ -120,7 +120,8 @@ def decay_attention_step(q, k, v, log_decay, state, starts=None, scale=None, nex
     state [B, H, dk, dv] float32, contiguous.  Returns out [B, H, dv].
 
     The new state overwrites `state`, or goes to `next_state` (a buffer like `state` that does not overlap
-    it), or nowhere with update=False (the value of a terminal observation: a look without a step).  No gradients.
+    it), or nowhere with update=False (the value of a terminal observation: a look without a step).  No gradients:
+    ValueError where one would be recorded.
     """
     _tensor("decay_attention_step", "q", q)
     if scale is None:
