@@ -1340,7 +1340,7 @@ static void walk_kernel(const WalkArgs& a, bool fine, dim3 grid, dim3 block, hip
 template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase phase, hipStream_t s) {
   const long long streams = (long long)a.b * a.h * a.nw * a.slabs;
   /* the waves that share a sequence's tensors in one workgroup, where they are at most four */
-  const int share = a.nw * a.slabs, waves = share <= 4 ? share : 4;
+  const int share = a.nw * a.slabs, waves = share == 3 ? 1 : share <= 4 ? share : 4;
   a.near = (share + waves - 1) / waves;
   const long long tasks = streams * (phase == STATES ? a.nsplit - 1 : a.nsplit), per = 8LL * a.near * waves;
   const dim3 grid((unsigned)((tasks + per - 1) / per * 8 * a.near)), block(64 * waves);
