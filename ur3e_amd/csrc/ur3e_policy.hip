@@ -1338,11 +1338,14 @@ static void walk_kernel(const WalkArgs& a, bool fine, dim3 grid, dim3 block, hip
   }
 }
 template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase phase, hipStream_t s) {
-  const long long streams = (long long)a.b * a.h * a.nw * a.slabs;
-  /* the waves that share a sequence's tensors in one workgroup, where they are at most four */
-  const int share = a.nw * a.slabs, waves = share == 3 ? 1 : share <= 4 ? share : 4;
+  const long long tasks = (long long)a.b * a.h * a.nw * a.slabs * (phase == STATES ? a.nsplit - 1 : a.nsplit);
+  /* The waves that share a sequence's tensors in one workgroup, where they are two or four (128 channels bfloat16: 1.51 ms,
+     in workgroups of one wave 1.58).  Not three: two waves fit a SIMD, so a compute unit would hold two such workgroups and
+     leave two of its eight places empty (float gradients at 64 channels 2.63 ms, one by one 2.43).  Nor where there is less
+     than a wave a SIMD: one by one they spread over all units (16 sequences x 16 tokens, both directions: 14.6 us, 13.3). */
+  const int share = a.nw * a.slabs, waves = tasks <= 1024 || share == 3 ? 1 : share <= 4 ? share : 4;
   a.near = (share + waves - 1) / waves;
-  const long long tasks = streams * (phase == STATES ? a.nsplit - 1 : a.nsplit), per = 8LL * a.near * waves;
+  const long long per = 8LL * a.near * waves;
   const dim3 grid((unsigned)((tasks + per - 1) / per * 8 * a.near)), block(64 * waves);
   bool fine = false;
   for (int i = 0; i < a.nw; i++) fine = fine || a.w[i].s_out;
