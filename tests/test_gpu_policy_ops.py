@@ -452,7 +452,7 @@ def test_gradients_of_some_inputs():
 
 
 @pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
-@pytest.mark.parametrize("r,c", [(1, 1), (3, 7), (5, 8), (4, 256), (129, 101), (7, 1024)])
+@pytest.mark.parametrize("r,c", [(1, 1), (3, 7), (5, 8), (19, 9), (6, 15), (4, 256), (129, 101), (7, 1024)])
 @pytest.mark.parametrize("p", [0.0, 0.1, 0.73, 1.0])
 def test_dropout(r, c, p, dtype):
     from ur3e_amd.rl import ops

@@ -70,40 +70,21 @@ __device__ __forceinline__ unsigned pack_bf16(float lo, float hi) {
   return __builtin_bit_cast(unsigned, b2{(__bf16)lo, (__bf16)hi});
 }
 
-/* N consecutive elements; VEC: aligned to min(16, N * sizeof(T)) bytes */
-template <class T, int N, bool VEC> __device__ __forceinline__ void ld_n(const T* p, float* x) {
-  if constexpr (VEC) {
-    constexpr int B = N * (int)sizeof(T) < 16 ? N * (int)sizeof(T) : 16;
-    constexpr int E = B / (int)sizeof(T);
-    struct alignas(B) Pack { T e[E]; };
+/* eight consecutive elements, on a boundary of 16 bytes (WHOLE) or of an element */
+template <class T, bool WHOLE> struct Eight {
+  struct alignas(WHOLE ? 16 : sizeof(T)) Pack { T e[8]; };
+  static __device__ __forceinline__ void load(const T* p, float* x) {
+    const Pack v = *reinterpret_cast<const Pack*>(p);
 #pragma unroll
-    for (int c = 0; c < N / E; c++) {
-      const Pack v = reinterpret_cast<const Pack*>(p)[c];
-#pragma unroll
-      for (int i = 0; i < E; i++) x[c * E + i] = to_f(v.e[i]);
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i++) x[i] = to_f(p[i]);
+    for (int i = 0; i < 8; i++) x[i] = to_f(v.e[i]);
   }
-}
-template <class T, int N, bool VEC> __device__ __forceinline__ void st_n(T* p, const float* x) {
-  if constexpr (VEC) {
-    constexpr int B = N * (int)sizeof(T) < 16 ? N * (int)sizeof(T) : 16;
-    constexpr int E = B / (int)sizeof(T);
-    struct alignas(B) Pack { T e[E]; };
+  static __device__ __forceinline__ void store(T* p, const float* x) {
+    Pack v;
 #pragma unroll
-    for (int c = 0; c < N / E; c++) {
-      Pack v;
-#pragma unroll
-      for (int i = 0; i < E; i++) v.e[i] = from_f<T>(x[c * E + i]);
-      reinterpret_cast<Pack*>(p)[c] = v;
-    }
-  } else {
-#pragma unroll
-    for (int i = 0; i < N; i++) p[i] = from_f<T>(x[i]);
+    for (int i = 0; i < 8; i++) v.e[i] = from_f<T>(x[i]);
+    *reinterpret_cast<Pack*>(p) = v;
   }
-}
+};
 
 /* One walk: which tensors play q, k and v, and which way time runs.  `kdim` channels are contracted in the
    scores (and are the state's rows), `vdim` are read out. */
@@ -302,6 +283,10 @@ template <class T, int N> struct Row {
   }
   __device__ __forceinline__ float get(int e, int mt) const { return x[e / P::C].get(e % P::C * N + mt); }
 };
+__device__ __forceinline__ f4 four_halves(u2 x) {
+  typedef _Float16 h4 __attribute__((ext_vector_type(4)));
+  return __builtin_convertvector(__builtin_bit_cast(h4, x), f4);
+}
 /* elements i of x and j of y as two halves */
 template <class X> __device__ __forceinline__ unsigned halves(const X& x, int i, const X& y, int j) {
   if (&x == &y && i + 1 == j && i % 2 == 0) return x.d[i / 2];
@@ -688,12 +673,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 #pragma unroll
           for (int f = 0; f < H; f++) {
             if constexpr (TWO) {
-              f4 y, z;
-#pragma unroll
-              for (int e = 0; e < 4; e++) {
-                y[e] = c.qr[f].get(e, m0);
-                z[e] = c.qr[f].get(e, m1);
-              }
+              f4 y = four_halves(qq[f][m0]), z = four_halves(qq[f][m1]);
               qh[f] = split4x2(y, z, minus_one);
               ql[f] = pack4x2(y, z);
             } else qh[f] = both(qq[f][m0], qq[f][m1]);
@@ -1179,10 +1159,13 @@ __device__ __forceinline__ void philox(unsigned c0, unsigned c1, unsigned c2, un
   out[0] = c0; out[1] = c1; out[2] = c2; out[3] = c3;
 }
 
-/* A thread takes the 8 columns of one Philox call, so 131,072 x 256 bfloat16 with a residual, and the gradient, take 64 us,
-   5.2 TB/s: memory bounds it, with ten rounds of products per 8 elements beside.  A row that ends inside a block, or is not
-   on a boundary of 16 bytes, is read element by element: 4,097 x 101 in half take 3.5 us. */
-template <class T, bool VEC>
+/* A thread takes the 8 columns of one Philox call.  131,072 x 256 bfloat16 with a residual, and the gradient, take 64 us,
+   5.2 TB/s: memory bounds it, with ten rounds of products per 8 elements beside.
+   WHOLE: rows of whole blocks on boundaries of 16 bytes.  ROWS: at least 8 columns on any boundary; the last block of a row
+   reads the last 8 columns, its own behind the `back` that the block in front stores (39,049 x 405 bfloat16:
+   15.1 us, 4.2 TB/s; element by element 38 us).  PARTS: less than 8 columns. */
+enum Layout { WHOLE, ROWS, PARTS };
+template <class T, Layout LAY>
 __global__ __launch_bounds__(256) void k_keyed_dropout(long long rows, int cols, const T* x, long long xs, const T* res,
                                                        long long rs, T* y, long long ys, const long long* ids,
                                                        unsigned long long seed, unsigned sub, unsigned count, float up) {
@@ -1193,12 +1176,12 @@ __global__ __launch_bounds__(256) void k_keyed_dropout(long long rows, int cols,
   const long long row = i / blocks;
   const unsigned j = (unsigned)(i % blocks);
   const unsigned long long id = ids ? (unsigned long long)ids[row] : (unsigned long long)row;
-  const int c0 = 8 * (int)j;
+  const int m = LAY == WHOLE || cols - 8 * (int)j >= 8 ? 8 : cols - 8 * (int)j; /* columns of this block */
+  const int back = LAY == ROWS ? 8 - m : 0, c0 = 8 * (int)j - back;
   float xv[8], rv[8];
-  const int m = cols - c0 < 8 ? cols - c0 : 8;
-  if constexpr (VEC) {
-    ld_n<T, 8, true>(x + row * xs + c0, xv);
-    if (res) ld_n<T, 8, true>(res + row * rs + c0, rv);
+  if constexpr (LAY != PARTS) {
+    Eight<T, LAY == WHOLE>::load(x + row * xs + c0, xv);
+    if (res) Eight<T, LAY == WHOLE>::load(res + row * rs + c0, rv);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; e++) {
@@ -1208,19 +1191,23 @@ __global__ __launch_bounds__(256) void k_keyed_dropout(long long rows, int cols,
   }
   unsigned u[4];
   philox(j, (unsigned)id, (unsigned)(id >> 32), sub, (unsigned)seed, (unsigned)(seed >> 32), u);
+  unsigned keep = 0;
+#pragma unroll
+  for (int e = 0; e < 8; e++) keep |= ((e & 1 ? u[e >> 1] >> 16 : u[e >> 1] & 0xffffu) < count ? 1u : 0u) << e;
+  keep <<= back;
 #pragma unroll
   for (int e = 0; e < 8; e++) {
-    const unsigned d = e & 1 ? u[e >> 1] >> 16 : u[e >> 1] & 0xffffu;
-    float z = d < count ? xv[e] * up : 0.0f; /* a dropped element is 0 whatever it held */
+    float z = keep >> e & 1 ? xv[e] * up : 0.0f; /* a dropped element is 0 whatever it held */
     if (res) z += rv[e];
     xv[e] = z;
   }
-  if constexpr (VEC) {
-    st_n<T, 8, true>(y + row * ys + c0, xv);
+  T* const o = y + row * ys + c0;
+  if (LAY == WHOLE || (LAY == ROWS && back == 0)) {
+    Eight<T, LAY == WHOLE>::store(o, xv);
   } else {
 #pragma unroll
     for (int e = 0; e < 8; e++)
-      if (e < m) y[row * ys + c0 + e] = from_f<T>(xv[e]);
+      if (e >= back && e < back + m) o[e] = from_f<T>(xv[e]);
   }
 }
 
@@ -1683,10 +1670,14 @@ static int dropout_launch(long long rows, int cols, const void* x, long long xs,
   const float up = count ? 65536.0f / (float)count : 0.0f;
   constexpr int E = 16 / (int)sizeof(T);
   auto al = [](const void* p, long long st) { return (uintptr_t)p % 16 == 0 && st % E == 0; };
-  const bool vec = cols % 8 == 0 && al(x, xs) && al(y, ys) && (!res || al(res, rs));
+  const Layout lay = cols < 8 ? PARTS : cols % 8 == 0 && al(x, xs) && al(y, ys) && (!res || al(res, rs)) ? WHOLE : ROWS;
   const dim3 grid((unsigned)((n + 255) / 256));
-  if (vec) hipLaunchKernelGGL((k_keyed_dropout<T, true>), grid, dim3(256), 0, s, rows, cols, (const T*)x, xs, (const T*)res, rs, (T*)y, ys, ids, seed, sub, (unsigned)count, up);
-  else hipLaunchKernelGGL((k_keyed_dropout<T, false>), grid, dim3(256), 0, s, rows, cols, (const T*)x, xs, (const T*)res, rs, (T*)y, ys, ids, seed, sub, (unsigned)count, up);
+  auto run = [&](auto kernel) {
+    hipLaunchKernelGGL(kernel, grid, dim3(256), 0, s, rows, cols, (const T*)x, xs, (const T*)res, rs, (T*)y, ys, ids, seed, sub, (unsigned)count, up);
+  };
+  if (lay == WHOLE) run(k_keyed_dropout<T, WHOLE>);
+  else if (lay == ROWS) run(k_keyed_dropout<T, ROWS>);
+  else run(k_keyed_dropout<T, PARTS>);
   PL_CHK(hipGetLastError());
   return UR3E_OK;
 }
