@@ -97,13 +97,15 @@ struct Walk {
   Tok q, k, v, o;           /* o.p is written */
   const float* s_in;        /* [b][h][dk * dv] or null */
   float* s_out;             /* or null (always where state_t) */
-  float* ws;                /* nsplit > 1: [b][h][split][kdim * vdim], split s holds the state that enters it, */
+  float* ws;                /* nsplit > 1: [b][h][split][room(kdim * vdim)], split s holds the state that enters it, */
   float* wf;                /* and [b][h][split], what split s - 1 multiplies the state by */
   int state_t;              /* a [dk][dv] state is this walk's transposed: kdim = dv */
   int reversed;
   int out_f32;              /* out is float whatever the token type (gradients that are summed over heads) */
   float in_scale, p_scale, w_scale; /* on the read-out of the entering state, on the scores, on k in the state */
 };
+/* floats between the states of two splits: on boundaries of 16 bytes */
+__host__ __device__ __forceinline__ int room(int elems) { return (elems + 3) / 4 * 4; }
 struct WalkArgs {
   Walk w[3];
   int nw; /* walks of this launch, all of the same tile shape */
@@ -405,7 +407,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   const long long bh = (long long)b * a.h + h;
   const long long elems = (long long)kdim * vdim;
   f4 S[KT][VT];
-  const float* s_in = STATE ? nullptr : nsplit > 1 ? w.ws + (bh * nsplit + split) * elems
+  const float* s_in = STATE ? nullptr : nsplit > 1 ? w.ws + (bh * nsplit + split) * room((int)elems)
                                                      : w.s_in ? w.s_in + bh * elems : nullptr;
   /* S[mt][nt][e]: key channel of(g, e) + mt, value channel of this lane's column + nt */
   const int vcolumn = v0 + PV::of(idx >> 2, idx & 3, vleft, -v0);
@@ -878,7 +880,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 
   float* s_out = nullptr;
   if (STATE) {
-    s_out = w.ws + (bh * nsplit + split + 1) * elems;
+    s_out = w.ws + (bh * nsplit + split + 1) * room((int)elems);
     if (slab == 0 && lane == 0) w.wf[bh * nsplit + split + 1] = through;
   }
   else if (split == nsplit - 1 && w.s_out) s_out = w.s_out + bh * elems;
@@ -946,31 +948,33 @@ __device__ __forceinline__ float carry_on(float f, float x, float u) {
 template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(WalkArgs a) {
   const Walk w = a.w[blockIdx.z];
   const long long bh = blockIdx.y;
-  const int elems = a.kdim * a.vdim, nsplit = a.nsplit;
+  const int elems = a.kdim * a.vdim, next_state = room(elems), nsplit = a.nsplit;
   const int e = (blockIdx.x * 64 + threadIdx.x) * VW;
   if (e >= elems) return;
   struct alignas(4 * VW) Pack { float x[VW]; };
-  float* ws = w.ws + bh * nsplit * elems + e;
+  float* ws = w.ws + bh * nsplit * next_state + e;
   const float* wf = w.wf + bh * nsplit;
   struct Lot { Pack u[LOT]; float f[LOT]; };
   auto load = [&](Lot& l, int s0) {
 #pragma unroll
     for (int i = 0; i < LOT; i++) {
       const int s = s0 + 1 + i < nsplit ? s0 + 1 + i : nsplit - 1;
-      l.u[i] = *reinterpret_cast<const Pack*>(ws + (long long)s * elems);
+      l.u[i] = *reinterpret_cast<const Pack*>(ws + (long long)s * next_state);
       l.f[i] = wf[s];
     }
   };
   Lot l;
   load(l, 0);
   Pack x = {};
-  if (w.s_in) x = *reinterpret_cast<const Pack*>(w.s_in + bh * elems + e);
+  if (w.s_in)
+#pragma unroll
+    for (int c = 0; c < VW; c++) x.x[c] = e + c < elems ? w.s_in[bh * elems + e + c] : 0.0f;
   for (int s0 = 0; s0 < nsplit; s0 += LOT) {
     Lot next;
     if (s0 + LOT < nsplit) load(next, s0 + LOT);
 #pragma unroll
     for (int i = 0; i < LOT; i++) {
-      if (s0 + i < nsplit) *reinterpret_cast<Pack*>(ws + (long long)(s0 + i) * elems) = x;
+      if (s0 + i < nsplit) *reinterpret_cast<Pack*>(ws + (long long)(s0 + i) * next_state) = x;
 #pragma unroll
       for (int c = 0; c < VW; c++) x.x[c] = carry_on(l.f[i], x.x[c], l.u[i].x[c]);
     }
@@ -987,11 +991,11 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attn_join_wide(WalkArgs a) 
   __shared__ float sum[JOIN_WAVES][64], factor[JOIN_WAVES], last[64];
   const Walk w = a.w[blockIdx.z];
   const long long bh = blockIdx.y;
-  const int elems = a.kdim * a.vdim, nsplit = a.nsplit;
+  const int elems = a.kdim * a.vdim, next_state = room(elems), nsplit = a.nsplit;
   const int lane = threadIdx.x & 63, me = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), waves = blockDim.x >> 6;
   const int e = blockIdx.x * 64 + lane;
   const bool ok = e < elems;
-  float* ws = w.ws + bh * nsplit * elems + (ok ? e : 0);
+  float* ws = w.ws + bh * nsplit * next_state + (ok ? e : 0);
   const float* wf = w.wf + bh * nsplit;
   float start = ok && w.s_in ? w.s_in[bh * elems + e] : 0.0f;
   for (int s0 = 0; s0 < nsplit; s0 += waves * LOT) {
@@ -1000,7 +1004,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attn_join_wide(WalkArgs a) 
 #pragma unroll
     for (int i = 0; i < LOT; i++) {
       const int s = mine + 1 + i < nsplit ? mine + 1 + i : nsplit - 1;
-      u[i] = ws[(long long)s * elems];
+      u[i] = ws[(long long)s * next_state];
       f[i] = wf[s];
     }
 #pragma unroll
@@ -1017,7 +1021,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attn_join_wide(WalkArgs a) 
 #pragma unroll
     for (int i = 0; i < LOT; i++)
       if (mine + i < nsplit) {
-        if (ok) ws[(long long)(mine + i) * elems] = x;
+        if (ok) ws[(long long)(mine + i) * next_state] = x;
         x = carry_on(f[i], x, u[i]);
       }
     if (me == waves - 1) last[lane] = x;
@@ -1291,12 +1295,12 @@ static Splits splits_of(const ur3e_attn_t* a, int backward) {
 
 /* the states that enter the splits, and the factors between them */
 static size_t split_bytes(const ur3e_attn_t* a, const Splits& p) {
-  return p.n > 1 ? (size_t)a->b * a->heads * p.n * (a->dk * a->dv + 1) * sizeof(float) : 0;
+  return p.n > 1 ? (size_t)a->b * a->heads * p.n * (room(a->dk * a->dv) + 1) * sizeof(float) : 0;
 }
 static void split_use(const ur3e_attn_t* a, const Splits& p, void* ws, Walk& w) {
   if (p.n < 2) return;
   w.ws = (float*)ws;
-  w.wf = w.ws + (long long)a->b * a->heads * p.n * a->dk * a->dv;
+  w.wf = w.ws + (long long)a->b * a->heads * p.n * room(a->dk * a->dv);
 }
 
 /* the rows hold a lane's load (Place::NC is 4 for up to 16 channels) */
@@ -1341,9 +1345,7 @@ template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase pha
     PL_CHK(hipGetLastError());
     const int elems = a.kdim * a.vdim;
     const unsigned bh = (unsigned)(a.b * a.h), nw = (unsigned)a.nw;
-    bool four = elems % 4 == 0;
-    for (int i = 0; i < a.nw; i++) four = four && (uintptr_t)a.w[i].s_in % 16 == 0 && (uintptr_t)a.w[i].ws % 16 == 0;
-    if (four && (long long)bh * nw * elems >= 64 * 4096)
+    if ((long long)bh * nw * elems >= 64 * 4096)
       hipLaunchKernelGGL((k_attn_join<4, 8>), dim3((elems + 255) / 256, bh, nw), dim3(64), 0, s, a);
     else if (a.nsplit > 32)
       hipLaunchKernelGGL(k_attn_join_wide, dim3((elems + 63) / 64, bh, nw), dim3(64 * ((a.nsplit + 31) / 32 < JOIN_WAVES ? (a.nsplit + 31) / 32 : JOIN_WAVES)), 0, s, a);
