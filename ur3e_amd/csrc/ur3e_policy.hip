@@ -25,10 +25,10 @@
  *     dq = walk(do, v, k) on S^T,  dk = reversed walk(v, do, q) on G^T,  dv = reversed walk(k, q, do) on G.
  *
  * What bounds it (MI355X, a copy of 4 GiB runs at 4.75 TB/s): 2,048 sequences x 512 tokens x 4 heads of 64 channels take,
- * forward, 487 us in bfloat16 (4.4 TB/s) and 915 us in float (4.7), bound by memory, and 484 us in half (4.4).  Their
- * gradients take 1.17 ms in bfloat16 (3.2 TB/s of the tensors; the walks run against each other in time and read some of
- * them twice), 2.63 ms in float, whose matrix instructions alone take 1.64, and 1.34 ms in half.  With 128 channels the
- * vector instructions around the products bound it: 1.51 ms in bfloat16 (2.9 TB/s).  Short calls are chains of latencies: a
+ * forward, 487 us in bfloat16 (4.4 TB/s) and 930 us in float (4.6), bound by memory, and 484 us in half (4.4).  Their
+ * gradients take 1.15 ms in bfloat16 (3.3 TB/s of the tensors; the walks run against each other in time and read some of
+ * them twice), 2.45 ms in float, whose matrix instructions alone take 1.64, and 1.28 ms in half.  With 128 channels the
+ * vector instructions around the products bound it: 1.54 ms in bfloat16 (2.8 TB/s).  Short calls are chains of latencies: a
  * chunk of 16 float tokens takes a lone wave 3.3 us, 2.1 us in a slab of 16 value channels. */
 #include <hip/hip_runtime.h>
 
@@ -1332,7 +1332,7 @@ template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase pha
   const long long tasks = (long long)a.b * a.h * a.nw * a.slabs * (phase == STATES ? a.nsplit - 1 : a.nsplit);
   /* The waves that share a sequence's tensors in one workgroup, where they are two or four (128 channels bfloat16: 1.51 ms,
      in workgroups of one wave 1.58).  Not three: two waves fit a SIMD, so a compute unit would hold two such workgroups and
-     leave two of its eight places empty (float gradients at 64 channels 2.63 ms, one by one 2.43).  Nor where there is less
+     leave two of its eight places empty (float gradients at 64 channels 2.63 ms, one by one 2.45).  Nor where there is less
      than a wave a SIMD: one by one they spread over all units (16 sequences x 16 tokens, both directions: 14.6 us, 13.3). */
   const int share = a.nw * a.slabs, waves = tasks <= 1024 || share == 3 ? 1 : share <= 4 ? share : 4;
   a.near = (share + waves - 1) / waves;
