@@ -135,6 +135,21 @@ def test_attention_exact_over_hundreds_of_splits(dtype):
         assert torch.equal(got.detach().cpu()[0, :, 0], e.float().to(DT[dtype]))
 
 
+@pytest.mark.parametrize("small", ["q", "k", "v"])
+@pytest.mark.parametrize("t", [16, 300])
+def test_attention_half_below_its_normal_range(small, t):
+    """one operand's elements lie below 2^-14, where half has fewer bits, but has them: nothing is taken for zero.  The others
+    are of the size that keeps sums of 300 products below 2^16."""
+    x, dout, dfinal = make(1, t, 2, 2, 32, 32, torch.float16, seed=t, decay=[-0.1, -0.5])
+    size = {n: 2.0 ** 4 for n in ("q", "k", "v")}
+    size[small] = 2.0 ** -17
+    for n, f in size.items():
+        x[n] = (x[n].float() * f).half()
+    x["initial_state"] *= size["k"] * size["v"]
+    got = check_all(x, dout, dfinal)
+    assert got["out"].abs().max() > 2.0 ** -12 and got["d" + small].abs().max() > 1.0
+
+
 def test_attention_lengths_are_clamped():
     x, dout, dfinal = make(3, 20, 2, 2, 16, 16, torch.float32, lengths=[-5, 99, 20])
     got = run(x, dout, dfinal)
