@@ -220,9 +220,9 @@ template <class T> struct Peak {
   }
 };
 
-/* bfloat16 fragments of 16-bit tensors, two elements to a dword.  A 32-bit operand enters the matrix instructions as the sum of
-   its leading parts of 8 bits each: two (error 2^-17) for scores and state, whose results are rounded to 2^-9
-   on the way out, three (2^-25) for what is added to the state. */
+/* bfloat16 fragments of 16-bit tensors, two elements to a dword.  A 32-bit operand enters the matrix instructions
+   as the sum of its leading parts of 8 bits each: two (error 2^-17) for scores and state, whose results are rounded
+   to 2^-9 or 2^-11 on the way out, three (2^-25) for what is added to a state that leaves. */
 /* the K = 32 shape throughout, half empty where four elements are all there is: a K = 16 instruction right behind
    a K = 32 one on the same accumulators read them before the first had written (the compiler had put one wait
    state between the two; measured at one tile, where nothing else stands between them) */
@@ -285,6 +285,8 @@ template <class T, int N> struct Row {
   }
   __device__ __forceinline__ float get(int e, int mt) const { return x[e / P::C].get(e % P::C * N + mt); }
 };
+/* (From the packed registers.  Taken from the chunk element by element, at one tile of keys, the compiler widened loads
+   past the rows and kept the chunk in memory: 17.5 us a call, with this 4.7.) */
 __device__ __forceinline__ f4 four_halves(u2 x) {
   typedef _Float16 h4 __attribute__((ext_vector_type(4)));
   return __builtin_convertvector(__builtin_bit_cast(h4, x), f4);
@@ -307,10 +309,11 @@ template <class T, int KT> __device__ __forceinline__ void pack_row(const Row<T,
     y[mt] = u2{halves(r.x[0], mt, r.x[1 / C], 1 % C * KT + mt), halves(r.x[2 / C], 2 % C * KT + mt, r.x[3 / C], 3 % C * KT + mt)};
 }
 
-/* KT, VT: tiles of 16 key channels and of 16 value channels per wave; H: tiles of 16 tokens per chunk.  STATE: only the state at the end of
-   each split (from zero), for sequences that several waves share.  FINE (16-bit types): a state leaves as floats and is
-   summed to their precision, from keys in three parts; where it only feeds 16-bit outputs, from keys in two (of the
-   products of two parts of a half, that of the two rests, 2^-18, is left out then where it is not free). */
+/* KT, VT: tiles of 16 key channels and of 16 value channels per wave; H: tiles of 16 tokens per chunk.  STATE: only the
+   state at the end of each split (from zero), for sequences that several waves share.  FINE (16-bit types): a state
+   leaves as floats and is summed to their precision, from keys in three parts; where it only feeds 16-bit outputs,
+   from keys in two (of the products of two parts of a half, that of the two rests, 2^-18, is left out then where it
+   is not free). */
 template <class T, int KT, int VT, bool STATE, int H, bool FINE>
 __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   constexpr int ES = (int)sizeof(T), C = 16 * H;
@@ -1032,8 +1035,9 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attn_join_wide(WalkArgs a) 
 
 /* Sums of the per-query-head gradients over the `grp` heads that share a key / value head: rows of `width` floats,
    [b][t][hk][grp][width], to d channels of [b][t][hk] rows.  With grp = 1 it narrows the rows of less than four
-   channels that the walks write eight wide.  A thread sums four channels; every tensor of a call in one launch.  Memory bounds
-   it: 33 x 777 tokens, 6 heads over 2, 48 + 96 channels take 16.4 us (6.2 TB/s: they come from the Infinity Cache). */
+   channels that the walks write eight wide.  A thread sums four channels; every tensor of a call in one launch.  Memory
+   bounds it: 33 x 777 tokens, 6 heads over 2, 48 + 96 channels take 16.4 us (6.2 TB/s: they come from the Infinity
+   Cache). */
 struct SumArgs {
   struct One {
     const float* src;
