@@ -110,6 +110,10 @@ struct WalkArgs {
   Walk w[3];
   int nw; /* walks of this launch, all of the same tile shape */
   int b, t, h, kdim, vdim, slabs, nsplit, split_len;
+  /* Channels that the last slab takes from the one in front of it: one load of a lane where fewer are left for it, so that no
+     channel is read and written by two slabs (they may round it differently: a chunk with a value that is not finite
+     is taken token by token). */
+  int lent;
   int near; /* consecutive workgroups that share a sequence's tensors */
   int chunk; /* 16, or 1 where tokens lie too far apart for 30-bit offsets inside a chunk */
   const float* log_decay;
@@ -269,7 +273,7 @@ template <class T, int N> struct Place {
   static constexpr int U = N * (int)sizeof(T), C = U >= 16 ? 1 : U >= 4 ? 16 / U : 4, R = 4 / C, NC = N * C;
   static __device__ __forceinline__ int first(int g, int e) { return NC * (e / C * 4 + g); }
   static __device__ __forceinline__ bool there(int g, int e, int dim) { return first(g, e) < dim; }
-  /* low: the first channel there is (rows of less than NC are copied into wider ones and start there) */
+  /* (rows of less than NC are copied into wider ones) */
   static __device__ __forceinline__ int of(int g, int e, int dim, int low = 0) {
     const int f = first(g, e), last = dim - NC < f ? dim - NC : f;
     return (last > low ? last : low) + e % C * N;
@@ -335,7 +339,11 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   const Walk w = a.w[wi];
   const int kdim = a.kdim, vdim = a.vdim, chunk = a.chunk, nsplit = a.nsplit;
   const long long starts_st = a.starts_st;
-  const int v0 = slab * 16 * VT, vleft = vdim - v0; /* first channel of this slab, channels from there on */
+  typedef Place<T, KT> PK;
+  typedef Place<T, VT> PV;
+  /* first channel of this slab, channels from there on */
+  const int v0 = slab * 16 * VT - (slab == a.slabs - 1 ? a.lent : 0);
+  const int vleft = slab == a.slabs - 2 ? 16 * VT - a.lent : vdim - v0;
   const float l = a.log_decay[h];
   int len = a.t;
   if (a.lengths) {
@@ -355,8 +363,6 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
 
   /* byte offsets of a lane's channels and tokens, in the row form and in the column form, for tiles of n: the lowest
      token of the tile is the base */
-  typedef Place<T, KT> PK;
-  typedef Place<T, VT> PV;
   unsigned qrow[PK::R], krow[PK::R], kcol[4], vcol[4];
   auto place = [&](int n) {
     const int idx = fresh(lane & 15), g = fresh(lane >> 4), gi = idx >> 2, ei = idx & 3;
@@ -413,7 +419,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   const float* s_in = STATE ? nullptr : nsplit > 1 ? w.ws + (bh * nsplit + split) * room((int)elems)
                                                      : w.s_in ? w.s_in + bh * elems : nullptr;
   /* S[mt][nt][e]: key channel of(g, e) + mt, value channel of this lane's column + nt */
-  const int vcolumn = v0 + PV::of(idx >> 2, idx & 3, vleft, -v0);
+  const int vcolumn = v0 + PV::of(idx >> 2, idx & 3, vleft);
   const bool vthere = PV::there(idx >> 2, idx & 3, vleft) & (vcolumn < vdim);
   const unsigned srow = 4 * (w.state_t ? 1 : vdim), scol = 4 * (w.state_t ? kdim : 1);
   auto own = [&](int e, int mt) {
@@ -1340,6 +1346,8 @@ template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase pha
      than a wave a SIMD: one by one they spread over all units (16 sequences x 16 tokens, both directions: 14.6 us, 13.3). */
   const int share = a.nw * a.slabs, waves = tasks <= 1024 || share == 3 ? 1 : share <= 4 ? share : 4;
   a.near = (share + waves - 1) / waves;
+  constexpr int load = Place<T, VT>::NC;
+  a.lent = a.slabs > 1 && a.vdim - (a.slabs - 1) * 16 * VT < load ? load : 0;
   const long long per = 8LL * a.near * waves;
   const dim3 grid((unsigned)((tasks + per - 1) / per * 8 * a.near)), block(64 * waves);
   bool fine = false;
