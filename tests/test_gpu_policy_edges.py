@@ -30,3 +30,59 @@ def test_a_value_that_is_not_finite_stays_in_its_slab(b, t, dtype):
     got = run(x, planted(dout), dfinal)
     for n in ("dv", "ds0"):
         assert torch.equal(got[n][..., 60:], clean[n][..., 60:]), n
+
+
+def tokens(g, dtype, b, t, h, d):
+    return torch.randn((b, t, h, d), device="cuda", generator=g).to(dtype)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("b,h,t,d", [
+    (64, 4, 4000, 8),     # a few splits of 500 tokens and more, few elements
+    (1, 1, 10500, 16),    # hundreds of splits of one sequence
+    (64, 4, 4000, 33),    # a few splits, many elements
+])
+def test_what_is_not_finite_is_not_lost_between_splits(b, h, t, d, dtype):
+    """The decay over a split of 368 tokens of a factor of 3/4, or over 32 shorter ones, is less than any float.  A NaN in the state
+    is there behind it all the same, forwards and backwards, up to an episode's start and not past it."""
+    g = torch.Generator(device="cuda").manual_seed(t + d)
+    cut = t - 700
+    x = dict(q=tokens(g, DT[dtype], b, t, h, d), k=tokens(g, DT[dtype], b, t, h, d), v=tokens(g, DT[dtype], b, t, h, d),
+             log_decay=torch.full((h,), 0.75, device="cuda").log(), initial_state=torch.zeros((b, h, d, d), device="cuda"),
+             starts=None, lengths=None)
+    dout = tokens(g, DT[dtype], b, t, h, d)
+    dfinal = torch.zeros_like(x["initial_state"])
+    starts = torch.zeros((b, t), dtype=torch.bool, device="cuda")
+    starts[:, cut] = True
+
+    def nan_at(z, *at):
+        z = z.clone()
+        z[at] = float("nan")
+        return z
+
+    def gone(z):
+        return not torch.isfinite(z).any()
+
+    def whole(z):
+        return torch.isfinite(z).all()
+    # forwards: a value of the first token, and the state in front of it
+    for change in (dict(v=nan_at(x["v"], 0, 0, slice(None), 1)),
+                   dict(initial_state=nan_at(x["initial_state"], 0, slice(None), 0, 1))):
+        got = run({**x, **change}, dout, dfinal)
+        assert gone(got["out"][0, :, :, 1]) and whole(got["out"][0, :, :, 2:]) and whole(got["out"][1:])
+        assert gone(got["dq"][0, :, :, 0]) and whole(got["dq"][1:]) and whole(got["dk"][:, 1:])
+        assert gone(got["state"][0, :, 0, 1]) and whole(got["state"][1:]) and whole(got["state"][0, :, :, 2:])
+        got = run({**x, **change, "starts": starts}, dout, dfinal)
+        assert gone(got["out"][0, :cut, :, 1]) and whole(got["out"][:, cut:])
+        assert gone(got["dq"][0, :cut, :, 0]) and whole(got["dq"][:, cut:]) and whole(got["state"])
+    # backwards: the last output's gradient, and the last state's
+    starts = starts.roll(700 - cut, 1)
+    cut = 700
+    for do, df in ((nan_at(dout, 0, t - 1, slice(None), 1), dfinal), (dout, nan_at(dfinal, 0, slice(None), 0, 1))):
+        got = run(x, do, df)
+        assert gone(got["dv"][0, :, :, 1]) and whole(got["dv"][0, :, :, 2:]) and whole(got["dv"][1:])
+        assert gone(got["dk"][0, :, :, 0]) and whole(got["dk"][1:]) and whole(got["dq"][:, :t - 1])
+        assert gone(got["ds0"][0, :, 0, 1]) and whole(got["ds0"][1:]) and whole(got["ds0"][0, :, :, 2:])
+        got = run(dict(x, starts=starts), do, df)
+        assert gone(got["dv"][0, cut:, :, 1]) and whole(got["dv"][:, :cut])
+        assert gone(got["dk"][0, cut:, :, 0]) and whole(got["dk"][:, :cut]) and whole(got["ds0"])

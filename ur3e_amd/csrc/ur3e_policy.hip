@@ -98,12 +98,15 @@ struct Walk {
   const float* s_in;        /* [b][h][dk * dv] or null */
   float* s_out;             /* or null (always where state_t) */
   float* ws;                /* nsplit > 1: [b][h][split][room(kdim * vdim)], split s holds the state that enters it, */
-  float* wf;                /* and [b][h][split], what split s - 1 multiplies the state by */
+  float* wf;                /* and [b][h][split], what split s - 1 multiplies the state by, or DROPS */
   int state_t;              /* a [dk][dv] state is this walk's transposed: kdim = dv */
   int reversed;
   int out_f32;              /* out is float whatever the token type (gradients that are summed over heads) */
   float in_scale, p_scale, w_scale; /* on the read-out of the entering state, on the scores, on k in the state */
 };
+/* In the place of a factor: an episode starts, and what was in front is dropped whatever it holds.  (A factor of 0 is a product
+   that left float's range.  0 times a NaN or an infinity stays a NaN.) */
+#define DROPS -1.0f
 /* floats between the states of two splits: on boundaries of 16 bytes */
 __host__ __device__ __forceinline__ int room(int elems) { return (elems + 3) / 4 * 4; }
 struct WalkArgs {
@@ -481,7 +484,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
   asm volatile("" : "+v"(minus_one));
   float gn = 1.0f;
 
-  float through = 1.0f; /* STATE: what the split multiplies an entering state by */
+  float through = 1.0f; /* STATE: what the split multiplies an entering state by, or DROPS */
   int single = 0;       /* tokens left to take one by one */
   int placed = 0, scaled = 0; /* the chunk sizes that the offsets and the factors stand for */
   int p = lo, n = 0;
@@ -870,7 +873,7 @@ __global__ __launch_bounds__(256, 2) void k_attn_walk(WalkArgs a) {
           for (int nt = 0; nt < VT; nt++) S[mt][nt] = mfma4(kw, c.vc[0][e].get(nt), S[mt][nt]);
         }
     }
-    if (STATE) through = cut ? 0.0f : through * gn;
+    if (STATE) through = cut || through < 0.0f ? DROPS : through * gn;
     return true;
   };
   while (p < hi) {
@@ -948,12 +951,8 @@ template <class T> __global__ __launch_bounds__(256) void k_attn_pack(PackArgs a
    X_s = wf[s] X_{s-1} + ws[s], X_0 = s_in.  Nothing but the chain of multiply-adds depends on the split in front.
 
    Many sequences: a thread owns VW elements and runs along the splits, whose sums it loads LOT at a time, the next
-   lot while one is chained; the bytes bound it (both directions of eight demonstrations of 10,500 tokens: 15.6 us).  (A factor of 0 is an episode start: what was in front of it is
-   dropped whatever it holds.) */
-__device__ __forceinline__ float carry_on(float f, float x, float u) {
-  const float y = f * x;
-  return (f == 0.0f ? 0.0f : y) + u;
-}
+   lot while one is chained; the bytes bound it (both directions of eight demonstrations of 10,500 tokens: 15.6 us). */
+__device__ __forceinline__ float carry_on(float f, float x, float u) { return (f < 0.0f ? 0.0f : f * x) + u; }
 template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(WalkArgs a) {
   const Walk w = a.w[blockIdx.z];
   const long long bh = blockIdx.y;
@@ -1020,7 +1019,7 @@ __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attn_join_wide(WalkArgs a) 
     for (int i = 0; i < LOT; i++)
       if (mine + 1 + i < nsplit) {
         x = carry_on(f[i], x, u[i]);
-        g *= f[i];
+        g = g < 0.0f || f[i] < 0.0f ? DROPS : g * f[i];
       }
     sum[me][lane] = x;
     if (lane == 0) factor[me] = g;
