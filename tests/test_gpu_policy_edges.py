@@ -86,3 +86,35 @@ def test_what_is_not_finite_is_not_lost_between_splits(b, h, t, d, dtype):
         got = run(dict(x, starts=starts), do, df)
         assert gone(got["dv"][0, cut:, :, 1]) and whole(got["dv"][:, :cut])
         assert gone(got["dk"][0, cut:, :, 0]) and whole(got["dk"][:, :cut]) and whole(got["ds0"])
+
+
+def test_forward_mode_is_refused():
+    """a tangent that the kernels would drop is refused, in the inputs and in the gradients of a backward pass"""
+    import torch.autograd.forward_ad as fwd
+    from ur3e_amd.rl import ops
+    x, dout, dfinal = make(2, 5, 2, 1, 8, 8, torch.float32, state=True)
+    ld = x["log_decay"]
+    leaf = x["q"].detach().requires_grad_()
+    with fwd.dual_level():
+        def dual(z):
+            return fwd.make_dual(z, torch.ones_like(z))
+        for n in ("q", "k", "v", "initial_state", "log_decay"):
+            with pytest.raises(ValueError, match="forward-mode"):
+                ops.decay_attention(**dict(x, **{n: dual(x[n])}))
+        with pytest.raises(ValueError, match="forward-mode"):
+            ops.decay_attention(dual(leaf), x["k"], x["v"], ld)
+        with pytest.raises(ValueError, match="forward-mode"):
+            ops.decay_attention_step(x["q"][:, 0], x["k"][:, 0], dual(x["v"])[:, 0], ld, x["initial_state"])
+        with pytest.raises(ValueError, match="forward-mode"):
+            ops.keyed_dropout(dual(x["q"]), 0.5, 1)
+        out, _ = ops.decay_attention(leaf, x["k"], x["v"], ld)
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.autograd.grad(out, [leaf], dual(dout))
+        y = ops.keyed_dropout(leaf, 0.5, 1)
+        with pytest.raises(ValueError, match="forward-mode"):
+            torch.autograd.grad(y, [leaf], dual(torch.ones_like(y)))
+        # switched off, a tangent is nothing to carry
+        q = dual(x["q"])
+        with fwd._set_fwd_grad_enabled(False):
+            off, _ = ops.decay_attention(q, x["k"], x["v"], ld)
+        assert torch.equal(off, out)

@@ -44,6 +44,15 @@ const void* ptr(const Tensor& x) { return x.defined() ? x.const_data_ptr() : nul
 /* the tensor, with the channels of a token next to each other */
 Tensor unit(const Tensor& x) { return x.stride(-1) == 1 || x.size(-1) == 1 ? x : x.contiguous(); }
 
+/* Forward-mode derivatives: the kernels compute none, and their outputs would be taken for constants. */
+bool has_tangent(const Tensor& x) {
+  return x.defined() && c10::AutogradState::get_tls_state().get_fw_grad_mode() && x._fw_grad(0).defined();
+}
+void check_tangents(const char* what, std::initializer_list<Tensor> xs) {
+  for (const Tensor& x : xs)
+    TORCH_CHECK_VALUE(!has_tangent(x), what, ": no forward-mode derivatives on the GPU; pass primals (forward_ad.unpack_dual)");
+}
+
 /* Gradients under capture: where a leaf in front of x is held by an eager graph that still lives, its gradient is
    accumulated on that graph's stream.  From a capture, torch's engine then makes the default stream wait for work that is
    only being recorded, and the process ends.  So the call is refused while its graph is built. */
@@ -100,6 +109,7 @@ void check_attention(const std::string& what, int64_t dims, const Tensor& q, con
                     what, ": log_decay must be a float32 tensor of shape (", h, ",) on ", q.device());
   TORCH_CHECK_VALUE(!(log_decay.requires_grad() && at::GradMode::is_enabled()), what,
                     ": log_decay is a constant of the heads and gets no gradient; detach it");
+  TORCH_CHECK_VALUE(!has_tangent(log_decay), what, ": log_decay is a constant of the heads and has no forward-mode derivative; detach it");
   if (starts)
     TORCH_CHECK_VALUE((starts->scalar_type() == at::kBool || starts->scalar_type() == at::kByte) &&
                           starts->device() == q.device() && starts->sizes() == lead,
@@ -212,6 +222,7 @@ struct DecayAttention : torch::autograd::Function<DecayAttention> {
     const Tensor &q = x[0], &k = x[1], &v = x[2], &s0 = x[3];
     c10::DeviceGuard guard(q.device());
     Tensor dout = grads[0], ds = grads.size() > 1 ? grads[1] : Tensor();
+    check_tangents("decay_attention", {dout, ds});
     dout = dout.defined() ? unit(dout) : at::zeros({1, 1, 1, v.size(3)}, q.options()).expand({q.size(0), q.size(1), q.size(2), v.size(3)});
     if (ds.defined()) ds = ds.contiguous();
     const Tensor dq = tokens_like(q, q.size(2), q.size(3)), dk = tokens_like(k, k.size(2), k.size(3)),
@@ -232,6 +243,7 @@ std::pair<Tensor, OptT> decay_attention(const Tensor& q, const Tensor& k, const 
                                         const OptT& s0, const OptT& starts, const OptT& lengths, double scale,
                                         bool return_state) {
   check_sequences(q, k, v, log_decay, s0, starts, lengths, scale);
+  check_tangents("decay_attention", {q, k, v, s0.value_or(Tensor())});
   Inputs x{unit(q), unit(k), unit(v), s0 ? s0->contiguous() : Tensor(), log_decay.detach().contiguous(),
            starts ? *starts : Tensor(), lengths ? lengths->contiguous() : Tensor(), scale};
   const bool grad = at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad() ||
@@ -250,6 +262,7 @@ std::pair<Tensor, OptT> decay_attention(const Tensor& q, const Tensor& k, const 
 Tensor decay_attention_step(const Tensor& q, const Tensor& k, const Tensor& v, const Tensor& log_decay, Tensor state,
                             const OptT& starts, double scale, const OptT& next, bool update) {
   check_step(q, k, v, log_decay, state, starts, scale, next, update);
+  check_tangents("decay_attention_step", {q, k, v, state, next.value_or(Tensor())});
   at::NoGradGuard no_grad;
   c10::DeviceGuard guard(q.device());
   const Tensor q1 = unit(q), k1 = unit(k), v1 = unit(v), ld = log_decay.contiguous();
@@ -318,6 +331,7 @@ struct KeyedDropout : torch::autograd::Function<KeyedDropout> {
     TORCH_CHECK(!at::GradMode::is_enabled(), "keyed_dropout is differentiable once");
     const auto key = ctx->saved_data["key"].toIntVector();
     const Tensor& dy = grads[0];
+    check_tangents("keyed_dropout", {dy});
     Tensor dx;
     if (ctx->needs_input_grad(0))
       dx = dropout(dy, Tensor(), ctx->get_saved_variables()[0], {key[0], key[2], (uint64_t)key[1]});
@@ -328,6 +342,7 @@ struct KeyedDropout : torch::autograd::Function<KeyedDropout> {
 Tensor keyed_dropout(const Tensor& x, int64_t count, uint64_t seed, const OptT& rows, int64_t substream,
                      const OptT& residual) {
   check_dropout(x, rows, residual);
+  check_tangents("keyed_dropout", {x, residual.value_or(Tensor())});
   const OptT ids = rows ? OptT(rows->reshape(-1).contiguous()) : OptT();
   if (at::GradMode::is_enabled() && (x.requires_grad() || (residual && residual->requires_grad()))) {
     check_capture("keyed_dropout", {x, residual.value_or(Tensor())});

@@ -16,7 +16,8 @@ GPU tensors go through the HIP library, on torch's current stream of their devic
 device is; a missing library raises.  CPU tensors are computed with elementary torch operations.  The calls
 never synchronise and may be captured into HIP graphs, forward and backward; RuntimeError where an eager graph of the
 default stream still holds one of the leaves, which torch cannot capture a backward pass of.  Wrong arguments raise
-ValueError (TypeError for what is no tensor) before any launch.  Gradients are not differentiable again.
+ValueError (TypeError for what is no tensor) before any launch.  Gradients are not differentiable again, and
+forward-mode derivatives are refused on the GPU (ValueError); the CPU path carries them.
 Results do not depend on timing: the same call gives the same bits.
 """
 from __future__ import annotations
