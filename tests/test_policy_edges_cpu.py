@@ -34,3 +34,53 @@ def test_forward_mode_is_refused_before_a_launch():
         out, _ = ops.decay_attention(q, k, dual(v), ld)
         lin, _ = ops.decay_attention(q, k, torch.ones_like(v), ld)
         torch.testing.assert_close(fwd.unpack_dual(out).tangent, lin)
+
+
+def grads_of(x, dout, dfinal):
+    names = ("q", "k", "v", "initial_state")
+    leaves = {n: x[n].detach().requires_grad_() for n in names}
+    out, state = ops.decay_attention(**{**x, **leaves}, return_state=True)
+    return dict(zip(("out", "state", "dq", "dk", "dv", "ds0"),
+                    (out, state, *torch.autograd.grad([out, state], list(leaves.values()), [dout, dfinal]))))
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+def test_padding_is_not_read(value):
+    """whatever the padding and its output gradients hold: the same outputs and gradients, and zeros for the padding"""
+    x = make(3, 9, 4, 2, 6, 5, starts=0.2)
+    x["lengths"] = torch.tensor([9, 4, 0], dtype=torch.int32)
+    g = torch.Generator().manual_seed(2)
+    dout, dfinal = torch.randn((3, 9, 4, 5), generator=g), torch.randn((3, 4, 6, 5), generator=g)
+    clean = grads_of(x, dout, dfinal)
+    y = {n: z.clone() for n, z in x.items()}
+    d2 = dout.clone()
+    for z in (y["q"], y["k"], y["v"], d2):
+        z[1, 4:] = value
+        z[2] = value
+    y["starts"][1, 4:] = True
+    y["starts"][2] = True
+    got = grads_of(y, d2, dfinal)
+    for n, z in got.items():
+        assert torch.equal(z, clean[n]), n
+    for n in ("out", "dq", "dk", "dv"):
+        assert got[n][1, 4:].abs().max() == 0 and got[n][2].abs().max() == 0
+
+
+def test_what_starts_hide_has_no_gradient_of_what_is_behind():
+    """values that are not finite in front of a start, and behind it: each side's results are as without them"""
+    x = make(2, 8, 2, 2, 4, 4)
+    x["starts"] = torch.zeros((2, 8), dtype=torch.bool)
+    x["starts"][:, 5] = True
+    g = torch.Generator().manual_seed(3)
+    dout, dfinal = torch.randn((2, 8, 2, 4), generator=g), torch.randn((2, 2, 4, 4), generator=g)
+    clean = grads_of(x, dout, dfinal)
+    for token, side in ((2, slice(5, 8)), (6, slice(0, 5))):
+        y = {n: z.clone() if torch.is_tensor(z) else z for n, z in x.items()}
+        d2 = dout.clone()
+        for z in (y["q"], y["k"], y["v"], d2):
+            z[:, token] = float("nan")
+        got = grads_of(y, d2, dfinal)
+        for n in ("out", "dq", "dk", "dv"):
+            assert torch.equal(got[n][:, side], clean[n][:, side]), (token, n)
+        hidden = "state" if token == 2 else "ds0"
+        assert torch.equal(got[hidden], clean[hidden])

@@ -69,6 +69,10 @@ def _attention_cpu(q, k, v, log_decay, s0, starts, lengths, scale):
     decay = log_decay.exp().view(1, h, 1, 1)
     s = qf.new_zeros((b, h, dk, v.shape[3])) if s0 is None else s0
     zero = qf.new_zeros(())
+    if lengths is not None:
+        # (in front of the loop: a zero gradient times padding that is not finite would not be zero)
+        here = (torch.arange(t, device=q.device) < lengths[:, None]).view(b, t, 1, 1)
+        qf, kf, vf = (torch.where(here, x, zero) for x in (qf, kf, vf))
     outs = []
     for i in range(t):
         old = s * decay
