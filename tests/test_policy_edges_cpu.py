@@ -84,3 +84,11 @@ def test_what_starts_hide_has_no_gradient_of_what_is_behind():
             assert torch.equal(got[n][:, side], clean[n][:, side]), (token, n)
         hidden = "state" if token == 2 else "ds0"
         assert torch.equal(got[hidden], clean[hidden])
+
+
+def test_no_tokens_return_a_state_of_their_own():
+    x = make(3, 0, 2, 1, 4, 3)
+    _, state = ops.decay_attention(**x, return_state=True)
+    assert torch.equal(state, x["initial_state"])
+    state.zero_()
+    assert x["initial_state"].abs().max() > 0

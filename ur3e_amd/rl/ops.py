@@ -67,7 +67,7 @@ def _attention_cpu(q, k, v, log_decay, s0, starts, lengths, scale):
     vf = v.float().repeat_interleave(grp, 2)
     qf = q.float() * scale
     decay = log_decay.exp().view(1, h, 1, 1)
-    s = qf.new_zeros((b, h, dk, v.shape[3])) if s0 is None else s0
+    s = qf.new_zeros((b, h, dk, v.shape[3])) if s0 is None else s0.clone()
     zero = qf.new_zeros(())
     if lengths is not None:
         # (in front of the loop: a zero gradient times padding that is not finite would not be zero)
