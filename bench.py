@@ -583,7 +583,7 @@ def main():
     ap.add_argument("--steps", type=int, default=50)
     ap.add_argument("--warmup", type=int, default=5)
     ap.add_argument("--envs-per-gpu", type=int, default=4096)
-    ap.add_argument("--envs-per-block", type=int, default=0)
+    ap.add_argument("--envs-per-block", type=int, choices=(0, -64, -128), default=0)
     ap.add_argument("--no-cpu-baseline", action="store_true")
     ap.add_argument("--cpu-sample-envs", type=int, default=4096)
     ap.add_argument("--cpu-sample-steps", type=int, default=1000)
@@ -853,8 +853,7 @@ def main():
                                                f" {batch_kinfo.get('regs')} VGPRs: {batch_kinfo.get('envs_per_cu')} envs/CU)"
                                             " + full-capacity fallback; above the resident slot count the compact tier runs as a"
                                             " substep work queue", -128: "full-capacity, 128 lanes per env",
-                                            -64: "full-capacity, 64 lanes per env"}.get(
-                           batch.cfg.envs_per_block, f"v1 lane-per-env, {batch.cfg.envs_per_block} envs/wave"),
+                                            -64: "full-capacity, 64 lanes per env"}[batch.cfg.envs_per_block],
                        "kernel_resources": batch_kinfo,
                        "fallback_kernel_resources": full_kinfo,
                        "queue_split_percent": args.queue_split if args.queue_split is not None else "library default",

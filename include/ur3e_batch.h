@@ -95,7 +95,8 @@ typedef struct ur3e_config_t {
                               one that exceeds that by the full-capacity tier;
                             -128 = full-capacity tier only, 128-lane workgroup per env;
                             -64 = full-capacity tier only, 64-lane wavefront per env;
-                            1..64 = one env per lane, that many envs per wavefront (v1) */
+                            > 0 (one env per lane) is refused: its scratch could not be allocated on
+                              one run, cause unknown */
   int tier_con_cap;      /* diagnostic (0 = off): > 0: the compact tier treats more than this many
                             contacts as overflow (its envs run in the grasp tier); < 0: the compact
                             and the grasp tier both treat more than -tier_con_cap contacts as
@@ -106,7 +107,7 @@ typedef struct ur3e_config_t {
   int sensors;           /* 1: compute mjData.sensordata every forward (touch, actuatorfrc, torque via
                             mj_rnePostConstraint; assets/main.xml:384-405) for ur3e_batch_get_sensordata.
                             The torque sensors need the full-capacity layout, so the handle runs the
-                            full-capacity tier (envs_per_block 0 -> 128 lanes per env; > 0 rejected) */
+                            full-capacity tier (envs_per_block 0 -> 128 lanes per env) */
   int schedule;          /* two-tier step launch: 0 (default, auto) = gym tasks with frame_skip > 1 on
                             main.xml with more envs than resident workgroup slots run as a substep work
                             queue (a resident pool of workgroups pulls (substep, env) units, state handed

@@ -6,7 +6,7 @@ from ur3e_amd import runtime as rt
 md, mc = rt.load_model("main")
 n = int(sys.argv[1]) if len(sys.argv) > 1 else 4096
 out = {}
-for epb in [int(x) for x in (sys.argv[2].split(",") if len(sys.argv) > 2 else "64,16,4,1".split(","))]:
+for epb in [int(x) for x in (sys.argv[2].split(",") if len(sys.argv) > 2 else "0,-128,-64".split(","))]:
     cfg = rt.make_config(task=rt.TASK_GYM_V2, frame_skip=2, model=md, seed=1, envs_per_block=epb)
     b = rt.Batch(mc, cfg, n)
     lo = torch.tensor([0.04799994, -0.11650084, 0.0, 0.0], dtype=torch.float64, device="cuda")

@@ -2441,9 +2441,12 @@ extern "C" int ur3e_batch_create(const ur3e_model_t* model, const ur3e_config_t*
   int rc = check_model(model);
   if (rc) return rc;
   if (cfg->task < 0 || cfg->task > UR3E_TASK_MOVE_L) return fail(UR3E_EINVAL, "unknown task");
+  /* One env per lane: one run was aborted at the layout's first dispatch, because the runtime could not allocate its 74 KB of
+     scratch a lane.  The cause is not known, so the layout stays off. */
+  if (cfg->envs_per_block > 0)
+    return fail(UR3E_EINVAL, "envs_per_block > 0 (one env per lane) is switched off: its 74 KB of scratch a lane could not be "
+                             "allocated on one run (HSA_STATUS_ERROR_OUT_OF_RESOURCES); use 0, -64 or -128");
   const int gym_other = cfg->task >= UR3E_TASK_GYM_V0 && cfg->task <= UR3E_TASK_IMIT_DIRECT;
-  if (gym_other && cfg->envs_per_block > 0)
-    return fail(UR3E_EINVAL, "ur3e-v0 / imitation tasks need a workgroup-per-env layout (envs_per_block <= 0)");
   if (gym_other && (model->id_site_tcp < 0 || model->id_site_handle < 0 ||
                                         model->id_body_ghost < 0 || model->id_body_fish < 0 ||
                                         model->id_site_rpad < 0))
@@ -2455,15 +2458,10 @@ extern "C" int ur3e_batch_create(const ur3e_model_t* model, const ur3e_config_t*
       model->id_site_tcp < 0)
     return fail(UR3E_EMODEL, "task-space control needs the tcp site");
   if (cfg->reset_key >= model->nkey) return fail(UR3E_EINVAL, "reset_key out of range");
-  if (cfg->envs_per_block > 64) return fail(UR3E_EINVAL, "envs_per_block > 64");
-  if (model->nmesh > 0 && cfg->envs_per_block > 0)
-    return fail(UR3E_EINVAL, "convex mesh geoms need a workgroup-per-env layout (envs_per_block <= 0)");
   if (model->nmesh > UR3E_MAXMESH || model->nmeshvert > UR3E_MAXMESHVERT)
     return fail(UR3E_EMODEL, "convex meshes exceed the model image capacities");
   /* 0: two-tier (default); -64: full-capacity tier, 64 lanes; other negative: full-capacity tier,
-     128 lanes; 1..64: v1 lane-per-env */
-  if (cfg->sensors && cfg->envs_per_block > 0)
-    return fail(UR3E_EINVAL, "sensors need a workgroup-per-env layout (envs_per_block <= 0)");
+     128 lanes */
   if (cfg->sensors && model->nsensordata > UR3E_MAXSENSORDATA) return fail(UR3E_EMODEL, "too much sensordata");
   /* sensors: the torque sensors need mj_rnePostConstraint's body quantities after the solve, which
      only the full-capacity layout keeps, so a handle with sensors on runs the full-capacity tier */
