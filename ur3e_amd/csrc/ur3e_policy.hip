@@ -91,7 +91,7 @@ template <class T, bool WHOLE> struct Eight {
 struct Tok {
   const void* p;
   long long sb, st, sh;
-  int hdiv; /* head = query head / hdiv */
+  int hdiv = 1; /* head = query head / hdiv */
 };
 struct Walk {
   Tok q, k, v, o;           /* o.p is written */
