@@ -2,7 +2,8 @@
 import pytest
 import torch
 
-from test_gpu_policy_ops import DT, make, run
+import policy_variants as pv
+from test_gpu_policy_ops import DT, check_all, make, run
 
 pytestmark = pytest.mark.gpu
 
@@ -118,3 +119,73 @@ def test_forward_mode_is_refused():
         with fwd._set_fwd_grad_enabled(False):
             off, _ = ops.decay_attention(q, x["k"], x["v"], ld)
         assert torch.equal(off, out)
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+def test_exact_over_two_rounds_of_the_join(dtype):
+    """More than 512 splits, which the 16 waves of the join take in two rounds.  Without decay, with q, k, v and dout of -1, 0 and 1 and an
+    initial state of whole numbers, every sum is a whole number; the states stay below 2^11, exact in any of the kernel's forms,
+    and an output is the exact one rounded once."""
+    from ur3e_amd.rl import ops
+    t, d = 80000, 16
+    assert all(pv.splits(1, t, 1, d, d, 2 if dtype != "f32" else 4, False, back)[0] > 512 for back in (False, True))
+    g = torch.Generator(device="cuda").manual_seed(1)
+    q, k, v, do = (torch.randint(-1, 2, (t, d), device="cuda", generator=g).double() for _ in range(4))
+    s0, df = (torch.randint(-9, 10, (d, d), device="cuda", generator=g).double() for _ in range(2))
+    starts = torch.zeros((1, t), dtype=torch.bool, device="cuda")
+    ends = [30001, 30002, t]  # of the episodes; the last one runs over both rounds
+    starts[0, ends[:-1]] = True
+    leaves = [z.to(DT[dtype]).view(1, t, 1, d).requires_grad_() for z in (q, k, v)]
+    state0 = s0.float().view(1, 1, d, d).requires_grad_()
+    out, state = ops.decay_attention(*leaves, torch.zeros(1, device="cuda"), initial_state=state0, starts=starts, scale=1.0,
+                                     return_state=True)
+    grads = torch.autograd.grad([out, state], leaves + [state0],
+                                [do.to(DT[dtype]).view(1, t, 1, d), df.float().view(1, 1, d, d)])
+    want = [torch.empty((t, d), dtype=torch.float64, device="cuda") for _ in range(4)]
+    lo = 0
+    for hi in ends:
+        s = (k[lo:hi, :, None] * v[lo:hi, None, :]).cumsum(0)
+        if lo == 0:
+            s = s + s0
+        gs = (q[lo:hi, :, None] * do[lo:hi, None, :]).flip(0).cumsum(0).flip(0)
+        if hi == t:
+            gs = gs + df
+        if lo == 0:
+            gs0 = gs[0]
+        want[0][lo:hi] = (q[lo:hi, :, None] * s).sum(1)
+        want[1][lo:hi] = (s * do[lo:hi, None, :]).sum(2)
+        want[2][lo:hi] = (gs * v[lo:hi, None, :]).sum(2)
+        want[3][lo:hi] = (gs * k[lo:hi, :, None]).sum(1)
+        assert max(s.abs().max(), gs.abs().max()) < 2 ** 11
+        lo = hi
+    assert torch.equal(state.double()[0, 0], s[-1]) and torch.equal(grads[3].double()[0, 0], gs0)
+    for got, e in zip((out, *grads[:3]), want):
+        assert torch.equal(got.detach()[0, :, 0], e.float().to(DT[dtype]))
+
+
+@pytest.mark.parametrize("dtype", ["f32", "bf16", "f16"])
+@pytest.mark.parametrize("t,far", [(40, "tokens"), (200, "tokens"), (40, "starts")])
+def test_tokens_far_apart_one_by_one(t, far, dtype):
+    """Tokens (or starts) so far apart that 16 of them are past the 2^30 bytes of an offset are taken one by one: both directions, with
+    starts, padding, an initial state and, at 200, several splits"""
+    size = 4 if dtype == "f32" else 2
+    step = (1 << 26) // size + 64 if far == "tokens" else (1 << 25) + 8
+    if torch.cuda.mem_get_info()[0] < 40 << 30:
+        pytest.skip("needs 40 GB")
+    x, dout, dfinal = make(2, t, 4, 2, 20, 24, DT[dtype], seed=t, starts=0.05, lengths=[t, t - 9])
+    if far == "tokens":
+        assert pv.splits(2, t, 4, 20, 24, size, True, False)[0] == (1 if t == 40 else pv.splits(2, t, 4, 20, 24, size, True, True)[0])
+        buf = torch.empty(step * (t - 1) + 2 * 1024, dtype=DT[dtype], device="cuda")
+        at = 0
+        for n in ("q", "k", "v"):
+            b, _, h, d = x[n].shape
+            y = buf.as_strided((b, t, h, d), (h * d, step, d, 1), at)
+            at += b * h * d
+            y.copy_(x[n])
+            x[n] = y
+        assert at <= 2 * 1024
+    else:
+        y = torch.empty(step * (t - 1) + 8, dtype=torch.bool, device="cuda").as_strided((2, t), (1, step))
+        y.copy_(x["starts"])
+        x["starts"] = y
+    check_all(x, dout, dfinal)
