@@ -198,14 +198,30 @@ def _torch_cmd():
 
 
 def _build_torch(force, verbose):
+    try:
+        import torch
+    except ImportError:
+        # the C library serves its C users without; ur3e_amd.rl.ops raises
+        print("torch is not importable: the policy operators' torch binding (ur3e_policy_torch.so) is not built")
+        return
+    cmd = _torch_cmd()
+    # what it was built with: another torch, or another command, is another binding
+    stamp = os.path.join(OBJ, "ur3e_policy_torch.cmd")
+    made_by = "\n".join([torch.__version__, *cmd])
+    try:
+        with open(stamp) as f:
+            same = f.read() == made_by
+    except OSError:
+        same = False
     deps = _depfile_deps(os.path.join(OBJ, "ur3e_policy_torch.d"))
-    if force or _newer(TORCH_LIB, [SRC_PL_TORCH] + (deps if deps is not None else HEADERS)):
-        cmd = _torch_cmd()
+    if force or not same or _newer(TORCH_LIB, [SRC_PL_TORCH] + (deps if deps is not None else HEADERS)):
         if verbose:
             print(" ".join(cmd))
         t0 = time.time()
         subprocess.run(cmd, check=True)
         os.utime(TORCH_LIB, (t0, t0))
+        with open(stamp, "w") as f:
+            f.write(made_by)
 
 
 def build(force: bool = False, verbose: bool = False, trace: bool = False) -> str:
