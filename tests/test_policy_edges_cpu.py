@@ -92,3 +92,13 @@ def test_no_tokens_return_a_state_of_their_own():
     assert torch.equal(state, x["initial_state"])
     state.zero_()
     assert x["initial_state"].abs().max() > 0
+
+
+def test_philox_known_answers_of_any_block():
+    """Random123's kat_vectors for philox4x32 with 10 rounds: counters and keys of ones, and of pi's digits"""
+    for first, row, sub, seed, want in (
+            (0, 0, 0, 0, "6627e8d5 e169c58d bc57ac4c 9b00dbd8"),
+            (0xffffffff, -1, 0xffffffff, (1 << 64) - 1, "408f276d 41c83b0e a20bc7c6 6d5451fd"),
+            (0x243f6a88, 0x13198a2e85a308d3, 0x03707344, 0x299f31d0a4093822, "d16cfe09 94fdcceb 5001e420 24126ea1")):
+        words = ops._philox_cpu(seed, torch.tensor([row]), 1, sub, first=first)[0, 0].tolist()
+        assert [f"{w:08x}" for w in words] == want.split()

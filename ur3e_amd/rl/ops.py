@@ -154,10 +154,10 @@ def keep_count(p: float) -> int:
     return int(math.floor((1.0 - p) * 65536.0 + 0.5))
 
 
-def _philox_cpu(seed, rows, blocks, substream):
-    """Philox4x32-10 words [rows, blocks, 4] in int64 (the wrapped products keep the words' bits)"""
+def _philox_cpu(seed, rows, blocks, substream, first=0):
+    """Philox4x32-10 words [rows, blocks, 4] of the blocks from `first` on, in int64 (the wrapped products keep the words' bits)"""
     m = 0xFFFFFFFF
-    c0 = torch.arange(blocks).expand(rows.numel(), blocks)
+    c0 = torch.arange(first, first + blocks).expand(rows.numel(), blocks)
     c1 = (rows & m)[:, None].expand_as(c0)
     c2 = ((rows >> 32) & m)[:, None].expand_as(c0)
     c3 = torch.full_like(c0, substream)
