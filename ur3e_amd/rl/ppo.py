@@ -107,6 +107,8 @@ class MemoryNet(nn.Module):
                  substream: int = 0):
         super().__init__()
         width = net_arch[0]
+        if heads < 1:
+            raise ValueError(f"heads must be at least 1, got {heads}")
         if len(net_arch) != 2 or width % heads or width // heads > ops.MAX_DIM:
             raise ValueError(f"a memory needs two layers, the first of {heads} heads of at most {ops.MAX_DIM} "
                              f"channels: net_arch={tuple(net_arch)}")
