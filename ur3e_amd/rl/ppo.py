@@ -226,7 +226,7 @@ class PPO:
         self.max_grad_norm = max_grad_norm
         self.group = group
         torch.manual_seed(seed)
-        kw = dict(dropout=dropout, seed=int(seed) % (1 << 64))  # (a mask's key; torch takes negative seeds as well)
+        kw = dict(dropout=dropout, seed=seed % (1 << 64))  # (a mask's key; torch takes negative seeds as well)
         self.policy = (MemoryActorCritic(self.obs_dim, self.act_dim, net_arch, heads=heads, **kw) if self.memory else
                        ActorCritic(self.obs_dim, self.act_dim, net_arch, **kw)).to(self.device)
         if group is not None:  # identical replicas: broadcast rank 0's initial weights
