@@ -12,7 +12,9 @@
  * most 0; -inf keeps the token alone.  What a NaN or an infinity reaches by the formula is not finite, and nothing else.
  *
  * Element types: 0 float, 1 bfloat16, 2 IEEE half, the same for every token tensor of a call.  States,
- * log_decay and all sums are float.  All pointers are device pointers on the current HIP device; strides
+ * log_decay and all sums are float.  With 16-bit tokens a float operand of a product (scores, the state where it is read out,
+ * keys that enter a state without s_out or ds0) is taken to 17 bits, as two bfloat16 parts; keys that enter a state which
+ * leaves to 25, as three.  With float tokens every product is float.  All pointers are device pointers on the current HIP device; strides
  * are in elements, the channels of a token are contiguous, token strides are not negative.  Outputs overlap nothing
  * else.  Work is enqueued on `stream`; nothing is kept between calls, and a call may be captured into a graph; calls that
  * may run at once need workspaces of their own.  Results do not depend on timing (no atomics).

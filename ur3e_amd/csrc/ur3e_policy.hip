@@ -25,10 +25,10 @@
  *     dq = walk(do, v, k) on S^T,  dk = reversed walk(v, do, q) on G^T,  dv = reversed walk(k, q, do) on G.
  *
  * What bounds it (MI355X, a copy of 4 GiB runs at 4.75 TB/s): 2,048 sequences x 512 tokens x 4 heads of 64 channels take,
- * forward, 487 us in bfloat16 (4.4 TB/s) and 930 us in float (4.6), bound by memory, and 484 us in half (4.4).  Their
+ * forward, 481 us in bfloat16 (4.5 TB/s) and 918 us in float (4.7), bound by memory, and 484 us in half (4.4).  Their
  * gradients take 1.15 ms in bfloat16 (3.3 TB/s of the tensors; the walks run against each other in time and read some of
- * them twice), 2.45 ms in float, whose matrix instructions alone take 1.64, and 1.28 ms in half.  With 128 channels the
- * vector instructions around the products bound it: 1.54 ms in bfloat16 (2.8 TB/s).  Short calls are chains of latencies: a
+ * them twice), 2.44 ms in float, whose matrix instructions alone take 1.64, and 1.28 ms in half.  With 128 channels the
+ * vector instructions around the products bound it: 1.55 ms in bfloat16 (2.8 TB/s).  Short calls are chains of latencies: a
  * chunk of 16 float tokens takes a lone wave 3.3 us, 2.1 us in a slab of 16 value channels. */
 #include <hip/hip_runtime.h>
 
@@ -229,7 +229,9 @@ template <class T> struct Peak {
 
 /* bfloat16 fragments of 16-bit tensors, two elements to a dword.  A 32-bit operand enters the matrix instructions
    as the sum of its leading parts of 8 bits each: two (error 2^-17) for scores and state, whose results are rounded
-   to 2^-9 or 2^-11 on the way out, three (2^-25) for what is added to a state that leaves. */
+   to 2^-9 or 2^-11 on the way out, three (2^-25) for what is added to a state that leaves.  (Outputs of the plain form and of
+   these kernels are the same 0.0017 from the definition in bfloat16, one rounding, and 1.1e-4 from each other, where sums that
+   differ by 2^-17 round to either side.) */
 /* the K = 32 shape throughout, half empty where four elements are all there is: a K = 16 instruction right behind
    a K = 32 one on the same accumulators read them before the first had written (the compiler had put one wait
    state between the two; measured at one tile, where nothing else stands between them) */
@@ -991,8 +993,8 @@ template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(Wal
 }
 /* Few sequences wait for the chain: the waves of a workgroup take 32 splits each of the same 64 elements, all loads at
    once, chain their own from zero and pass on the result and the product of their factors; each then starts from
-   what the waves in front make of the state.  The 219 splits of one demonstration of 10,500 tokens take 7.1 us, by the
-   kernel above 15.7. */
+   what the waves in front make of the state.  The 165 splits of one demonstration of 10,500 tokens take 7.6 us, by the
+   kernel above 22.0, an element a thread 16.0. */
 #define JOIN_WAVES 16
 __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attn_join_wide(WalkArgs a) {
   constexpr int LOT = 32;
@@ -1176,7 +1178,7 @@ __device__ __forceinline__ void philox(unsigned c0, unsigned c1, unsigned c2, un
    5.2 TB/s: memory bounds it, with ten rounds of products per 8 elements beside.
    WHOLE: rows of whole blocks on boundaries of 16 bytes.  ROWS: at least 8 columns on any boundary; the last block of a row
    reads the last 8 columns, its own behind the `back` that the block in front stores (39,049 x 405 bfloat16:
-   15.1 us, 4.2 TB/s; element by element 38 us).  PARTS: less than 8 columns. */
+   13.6 us, 4.7 TB/s; element by element 38 us).  PARTS: less than 8 columns. */
 enum Layout { WHOLE, ROWS, PARTS };
 template <class T, Layout LAY>
 __global__ __launch_bounds__(256) void k_keyed_dropout(long long rows, int cols, const T* x, long long xs, const T* res,
@@ -1356,6 +1358,9 @@ template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase pha
     PL_CHK(hipGetLastError());
     const int elems = a.kdim * a.vdim;
     const unsigned bh = (unsigned)(a.b * a.h), nw = (unsigned)a.nw;
+    /* From 2^18 elements on the bytes count, below it the chain (64 x 64 states, four elements a thread and the wide one: 2^17
+       elements, 64 splits 12.1 and 11.0 us; 2^18, 32 splits 10.9 and 11.6; 2^19, 16 splits 10.7 and 13.8; 2^21, 4 splits 10.6 and
+       32.3).  Up to 32 splits one wave chains them all, and the hand-over between waves has nothing to do. */
     if ((long long)bh * nw * elems >= 64 * 4096)
       hipLaunchKernelGGL((k_attn_join<4, 8>), dim3((elems + 255) / 256, bh, nw), dim3(64), 0, s, a);
     else if (a.nsplit > 32)
@@ -1665,6 +1670,8 @@ extern "C" int ur3e_attn_step(const ur3e_attn_t* a, const ur3e_tokens_t* out, co
   int cl = 0;
   while ((1 << cl) < groups && cl < 6) cl++;
   auto slabs = [&] { return (groups + (1 << cl) - 1) >> cl; };
+  /* A wave a SIMD (1,024) where that leaves 64 bytes of a row to a wave, four groups (one env's head of 64 x 64: 4.1 us, a
+     group alone 5.5; 256 heads of 128 x 128: 7.2, 8 groups 7.1, 16 groups 8.2, one 19.0) */
   while (cl > 2 && (long long)a->b * a->heads * slabs() < 1024) cl--;
   const dim3 grid((unsigned)(((long long)a->b * a->heads * slabs() + 3) / 4));
   hipStream_t st = (hipStream_t)stream;

@@ -106,9 +106,14 @@ def decay_attention(q, k, v, log_decay, initial_state=None, starts=None, lengths
     scale: of the outputs, default dk ** -0.5.
 
     Returns (out [B, T, H, dv] of q's type, state): the state [B, H, dk, dv] float32 behind each sequence's
-    last token, or None without `return_state`.  States and sums are float32.  What a NaN or an infinity reaches by the
-    formula is not finite (a NaN where the formula may say infinity); nothing else is touched by it.
-    B * H must be below 2**22 and T at most 2**30.
+    last token, or None without `return_state`.  States and sums are float32.  On the GPU, with 16-bit tokens, a float32
+    operand of a product is taken to 17 bits: the scores, the state where it is read out, and keys that enter a state which is
+    not returned (to 25 bits where it is); outputs and gradients are then rounded to 8 bits (bfloat16) or 11 (float16).
+    With float32 tokens every product is float32.
+    What a NaN or an infinity reaches by the formula is not finite (a NaN where the formula may say infinity); nothing else
+    is touched by it.
+    B * H must be below 2**22 and T at most 2**30; with shared heads (H != Hk) or less than 4 channels, B * T * H times a
+    quarter of the channels, rounded up, below 2**32 - 256.
     """
     _tensor("decay_attention", "q", q)
     if scale is None:
