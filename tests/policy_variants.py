@@ -60,7 +60,7 @@ def kernels(b, t, h, dk, dv, dtype, ragged, state, grad):
         out.add((dtype, kt, vt, is_state, 2 if pairs else 1, True if es == 4 else fine))
         if is_state:
             elems = kdim * vdim
-            out.add("join<4,8>" if b * h * nw * elems >= 64 * 4096 else "join_wide" if n > 32 else "join<1,32>")
+            out.add("join" if b * h * nw * elems >= 64 * 4096 else "join of several waves" if n > 32 else "join of one wave")
     n, _ = splits(b, t, h, dk, dv, es, ragged, False)
     if n > 1:
         walk(dk, dv, 1, n, True, state)
@@ -80,7 +80,7 @@ def kernels(b, t, h, dk, dv, dtype, ragged, state, grad):
 def every(dtype):
     """all that are compiled for a type"""
     es = 4 if dtype == "f32" else 2
-    out = {"join<4,8>", "join_wide", "join<1,32>"}
+    out = {"join", "join of one wave", "join of several waves"}
     for kt in (1, 2, 4, 8):
         for vt in (1, 2, 4) if kt < 8 else (1, 2):
             for fine in (True,) if es == 4 else (True, False):

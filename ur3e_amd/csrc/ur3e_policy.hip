@@ -952,10 +952,11 @@ template <class T> __global__ __launch_bounds__(256) void k_attn_pack(PackArgs a
 /* States that enter each split: ws[s] holds split s - 1's own sum (k_attn_walk, STATE) and becomes
    X_s = wf[s] X_{s-1} + ws[s], X_0 = s_in.  Nothing but the chain of multiply-adds depends on the split in front.
 
-   Many sequences: a thread owns VW elements and runs along the splits, whose sums it loads LOT at a time, the next
+   Many elements: a thread owns VW of them and runs along the splits, whose sums it loads LOT at a time, the next
    lot while one is chained; the bytes bound it (both directions of eight demonstrations of 10,500 tokens: 15.6 us). */
 __device__ __forceinline__ float carry_on(float f, float x, float u) { return (f < 0.0f ? 0.0f : f * x) + u; }
-template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(WalkArgs a) {
+__global__ __launch_bounds__(64) void k_attn_join(WalkArgs a) {
+  constexpr int VW = 4, LOT = 8;
   const Walk w = a.w[blockIdx.z];
   const long long bh = blockIdx.y;
   const int elems = a.kdim * a.vdim, next_state = room(elems), nsplit = a.nsplit;
@@ -991,10 +992,10 @@ template <int VW, int LOT> __global__ __launch_bounds__(64) void k_attn_join(Wal
     l = next;
   }
 }
-/* Few sequences wait for the chain: the waves of a workgroup take 32 splits each of the same 64 elements, all loads at
+/* Few elements wait for the chain: the waves of a workgroup take 32 splits each of the same 64 elements, all loads at
    once, chain their own from zero and pass on the result and the product of their factors; each then starts from
    what the waves in front make of the state.  The 165 splits of one demonstration of 10,500 tokens take 7.6 us, by the
-   kernel above 22.0, an element a thread 16.0. */
+   kernel above 22.0. */
 #define JOIN_WAVES 16
 __global__ __launch_bounds__(64 * JOIN_WAVES) void k_attn_join_wide(WalkArgs a) {
   constexpr int LOT = 32;
@@ -1360,13 +1361,12 @@ template <class T, int KT, int VT> static int walk_launch(WalkArgs& a, Phase pha
     const unsigned bh = (unsigned)(a.b * a.h), nw = (unsigned)a.nw;
     /* From 2^18 elements on the bytes count, below it the chain (64 x 64 states, four elements a thread and the wide one: 2^17
        elements, 64 splits 12.1 and 11.0 us; 2^18, 32 splits 10.9 and 11.6; 2^19, 16 splits 10.7 and 13.8; 2^21, 4 splits 10.6 and
-       32.3).  Up to 32 splits one wave chains them all, and the hand-over between waves has nothing to do. */
+       32.3).  A wave of the wide one for each 32 splits, up to 16. */
+    const int join_waves = a.nsplit <= 32 * JOIN_WAVES ? (a.nsplit + 31) / 32 : JOIN_WAVES;
     if ((long long)bh * nw * elems >= 64 * 4096)
-      hipLaunchKernelGGL((k_attn_join<4, 8>), dim3((elems + 255) / 256, bh, nw), dim3(64), 0, s, a);
-    else if (a.nsplit > 32)
-      hipLaunchKernelGGL(k_attn_join_wide, dim3((elems + 63) / 64, bh, nw), dim3(64 * ((a.nsplit + 31) / 32 < JOIN_WAVES ? (a.nsplit + 31) / 32 : JOIN_WAVES)), 0, s, a);
+      hipLaunchKernelGGL(k_attn_join, dim3((elems + 255) / 256, bh, nw), dim3(64), 0, s, a);
     else
-      hipLaunchKernelGGL((k_attn_join<1, 32>), dim3((elems + 63) / 64, bh, nw), dim3(64), 0, s, a);
+      hipLaunchKernelGGL(k_attn_join_wide, dim3((elems + 63) / 64, bh, nw), dim3(64 * join_waves), 0, s, a);
   } else {
     walk_kernel<T, KT, VT, false>(a, fine, grid, block, s);
   }
