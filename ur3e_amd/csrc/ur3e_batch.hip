@@ -3,9 +3,8 @@
  *
  * One fused kernel per env-step (k_env_step): controller -> frame_skip physics
  * substeps -> observation / reward / termination -> in-kernel SB3 auto-reset.
- * One environment per wavefront lane; `envs_per_block` lanes of each 64-wide
- * wavefront are populated, trading lane packing for CU coverage (at 4096 envs
- * 16 envs/wave puts one wave on every one of the 256 CUs).
+ * The layouts that run hold an environment in a wavefront or a workgroup (ur3e_wave.h).  k_env_step's own, one environment per
+ * wavefront lane with `epb` lanes of a wave populated, is switched off (ur3e_batch_create).
  *
  * Persistent per-env state lives in HBM structure-of-arrays ([field][env]) so
  * a wave's 64 lanes touch consecutive doubles: qpos[nq], qvel[nv],

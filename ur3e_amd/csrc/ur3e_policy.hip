@@ -25,10 +25,10 @@
  *     dq = walk(do, v, k) on S^T,  dk = reversed walk(v, do, q) on G^T,  dv = reversed walk(k, q, do) on G.
  *
  * What bounds it (MI355X, a copy of 4 GiB runs at 4.75 TB/s): 2,048 sequences x 512 tokens x 4 heads of 64 channels take,
- * forward, 481 us in bfloat16 (4.5 TB/s) and 918 us in float (4.7), bound by memory, and 484 us in half (4.4).  Their
- * gradients take 1.15 ms in bfloat16 (3.3 TB/s of the tensors; the walks run against each other in time and read some of
- * them twice), 2.44 ms in float, whose matrix instructions alone take 1.64, and 1.28 ms in half.  With 128 channels the
- * vector instructions around the products bound it: 1.55 ms in bfloat16 (2.8 TB/s).  Short calls are chains of latencies: a
+ * forward, 482 us in bfloat16 (4.5 TB/s) and 931 us in float (4.6), bound by memory, and 487 us in half (4.4).  Their
+ * gradients take 1.14 ms in bfloat16 (3.3 TB/s of the tensors; the walks run against each other in time and read some of
+ * them twice), 2.47 ms in float, whose matrix instructions alone take 1.64, and 1.28 ms in half.  With 128 channels the
+ * vector instructions around the products bound it: 1.54 ms in bfloat16 (2.8 TB/s).  Short calls are chains of latencies: a
  * chunk of 16 float tokens takes a lone wave 3.3 us, 2.1 us in a slab of 16 value channels. */
 #include <hip/hip_runtime.h>
 
